@@ -5,6 +5,7 @@ from __future__ import annotations
 import concurrent.futures as cf
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -49,17 +50,23 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found; libflare_b200.so cannot be built")
 
 
+def _sources(path: str, seen: list[str]) -> list[str]:
+    """`path` and what it includes from this repository, each file once."""
+    path = os.path.normpath(path)
+    if path not in seen:
+        seen.append(path)
+        with open(path, encoding="utf-8") as f:
+            for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', f.read(), re.M):
+                _sources(os.path.join(os.path.dirname(path), name), seen)
+    return seen
+
+
 def _digest(src: str, defines: list[str]) -> str:
     h = hashlib.sha256()
     h.update(" ".join(NVCC_FLAGS + defines).encode())
-    with open(os.path.join(CSRC, src), "rb") as f:
-        h.update(f.read())
-    for name in sorted(os.listdir(CSRC)):
-        if name.endswith((".cuh", ".h")):
-            with open(os.path.join(CSRC, name), "rb") as f:
-                h.update(f.read())
-    with open(os.path.join(HERE, "..", "include", "flare_b200.h"), "rb") as f:
-        h.update(f.read())
+    for path in _sources(os.path.join(CSRC, src), []):
+        with open(path, "rb") as f:
+            h.update(f.read())
     return h.hexdigest()
 
 
