@@ -32,6 +32,9 @@ UNITS = [
     ("narrow_mma.cu", [], "narrow_mma"),
     ("decode_step.cu", [], "decode_step"),
     ("state_ops.cu", [], "state_ops"),
+    ("causal_conv.cu", [], "causal_conv"),
+    ("selective_scan.cu", [], "selective_scan"),
+    *[("selective_scan.cu", [f"-DFLARE_SCAN_TYPE={t}"], f"selective_scan_{t.strip(chr(95))}") for t in ("float", "__nv_bfloat16", "__half")],
     ("prefill_tc.cu", [], "prefill_tc_host"),
     *[("prefill_tc.cu", [f"-DFLARE_TC_UNIT={u}", f"-DFLARE_TC_MODE={m}"], f"prefill_tc_unit{u}_mode{m}") for u in range(8) for m in range(3)],
     ("noalloc.cu", [], "noalloc"),

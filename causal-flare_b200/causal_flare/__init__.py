@@ -17,6 +17,14 @@ from .semi_autoregressive.inference import (
     flare_semi_autoregressive_decode_trition,
     flare_semi_autoregressive_prefill_trition,
 )
+from .state_space import (
+    flare_causal_conv,
+    flare_causal_conv_decode,
+    flare_causal_conv_prefill,
+    flare_selective_scan,
+    flare_selective_scan_decode,
+    flare_selective_scan_prefill,
+)
 
 __version__ = "0.0.1"
 
@@ -26,7 +34,13 @@ __all__ = [
     "flare_autoregressive_triton",
     "flare_autoregressive_decode_triton",
     "flare_autoregressive_prefill_triton",
+    "flare_causal_conv",
+    "flare_causal_conv_decode",
+    "flare_causal_conv_prefill",
     "flare_recurrent_triton",
+    "flare_selective_scan",
+    "flare_selective_scan_decode",
+    "flare_selective_scan_prefill",
     "flare_semi_autoregressive_decode_trition",
     "flare_semi_autoregressive_prefill_trition",
     "flare_semi_autoregressive_trition",

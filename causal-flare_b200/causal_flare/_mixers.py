@@ -1,0 +1,124 @@
+"""ctypes binding and argument checks of the causal token mixers beside FLARE (include/flare_b200_mixers.h)."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+IDENTITY, SILU = 0, 1
+_ACTIVATIONS = {None: IDENTITY, "silu": SILU}
+
+
+class ConvArgs(C.Structure):
+    _fields_ = [
+        *((name, C.c_void_p) for name in ("x", "weight", "bias", "documents", "lengths", "state_in", "state_out", "y", "dy", "dx",
+                                          "dweight", "dbias", "workspace")),
+        ("workspace_bytes", C.c_size_t),
+        *((name, C.c_int32) for name in ("B", "N", "C", "W")),
+        *((name, C.c_int64) for name in ("x_stride_b", "x_stride_n", "dy_stride_b", "dy_stride_n")),
+        *((name, C.c_int32) for name in ("dtype", "weight_dtype", "activation")),
+    ]
+
+
+class ScanArgs(C.Structure):
+    _fields_ = [
+        *((name, C.c_void_p) for name in ("x", "dt", "z", "b", "c", "A", "D", "dt_bias", "documents", "lengths", "state_in", "state_out", "y",
+                                          "keep", "dy", "dx", "ddt", "dz", "db", "dc", "dA", "dD", "ddt_bias", "workspace")),
+        ("workspace_bytes", C.c_size_t),
+        *((name, C.c_int32) for name in ("B", "N", "C", "S", "G")),
+        *((f"{name}_stride_{axis}", C.c_int64) for name, axes in (("x", "bn"), ("dt", "bn"), ("z", "bn"), ("b", "bng"), ("c", "bng"), ("dy", "bn"))
+          for axis in axes),
+        ("dtype", C.c_int32), ("dt_softplus", C.c_int32),
+    ]
+
+
+_STRUCTS = (ConvArgs, ScanArgs)
+_CALLS = {"flare_conv_forward": ConvArgs, "flare_conv_backward": ConvArgs, "flare_conv_decode": ConvArgs,
+          "flare_scan_forward": ScanArgs, "flare_scan_backward": ScanArgs, "flare_scan_decode": ScanArgs}
+_SIZES = {"flare_conv_backward_workspace_bytes": ConvArgs, "flare_scan_keep_bytes": ScanArgs,
+          "flare_scan_forward_workspace_bytes": ScanArgs, "flare_scan_backward_workspace_bytes": ScanArgs}
+
+_bound = None
+
+
+def load() -> C.CDLL:
+    """The shared library with these entry points bound; raises if its structs differ from ours."""
+    global _bound
+    if _bound is None:
+        lib = _lib.load()
+        for name, struct in _CALLS.items():
+            getattr(lib, name).restype, getattr(lib, name).argtypes = C.c_int, [C.POINTER(struct), C.c_void_p]
+        for name, struct in _SIZES.items():
+            getattr(lib, name).restype, getattr(lib, name).argtypes = C.c_size_t, [C.POINTER(struct)]
+        lib.flare_mixers_abi_sizeof.restype, lib.flare_mixers_abi_sizeof.argtypes = C.c_size_t, [C.c_int]
+        for which, struct in enumerate(_STRUCTS):
+            if lib.flare_mixers_abi_sizeof(which) != C.sizeof(struct):
+                raise RuntimeError(f"ABI mismatch for {struct.__name__}: library {lib.flare_mixers_abi_sizeof(which)} bytes, "
+                                   f"binding {C.sizeof(struct)} bytes")
+        _bound = lib
+    return _bound
+
+
+def run(name: str, args, device, workspace: str | None = None) -> None:
+    """Launch an entry point on the device's current stream, with a workspace of what `workspace` (a size query) asks for."""
+    lib = load()
+    ws = None
+    with torch.cuda.device(device):
+        if workspace is not None:
+            need = getattr(lib, workspace)(C.byref(args))
+            if need:
+                ws = torch.empty(need, dtype=torch.uint8, device=device)
+                args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        _lib.check(getattr(lib, name)(C.byref(args), _lib.stream_handle(device)), name)
+    # `ws` is stream-ordered torch memory: safe to release after the launches are enqueued.
+
+
+# ---- argument checks -------------------------------------------------------------------------------------------------
+
+
+def on_gpu(name: str, x: torch.Tensor) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} requires CUDA tensors.")
+
+
+def same_device(name: str, x: torch.Tensor, **others) -> None:
+    for what, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} expects {what} on {x.device}. Got {t.device}.")
+
+
+def same_dtype(name: str, x: torch.Tensor, **others) -> None:
+    _lib.dtype_code(x.dtype)
+    for what, t in others.items():
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"{name} expects {what} in the inputs' type {x.dtype}. Got {t.dtype}.")
+
+
+def has_shape(name: str, what: str, t, shape) -> None:
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} expects {what} {list(shape)}. Got {list(t.shape)}.")
+
+
+def activation_code(name: str, activation) -> int:
+    try:
+        return _ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"{name} supports activation=None and 'silu'. Got {activation!r}.") from None
+
+
+def whole_numbers(name: str, what: str, t, shape):
+    """Ids or lengths as the kernels read them: int32, contiguous (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+        raise ValueError(f"{name} expects {what} of an integer type. Got {t.dtype}.")
+    has_shape(name, what, t, shape)
+    return t.to(torch.int32).contiguous()
+
+
+def rows(t):
+    """`t`, with its innermost dimension contiguous."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
