@@ -33,6 +33,10 @@ UNITS = [
     ("decode_step.cu", [], "decode_step"),
     ("state_ops.cu", [], "state_ops"),
     ("causal_conv.cu", [], "causal_conv"),
+    ("attention.cu", [], "attention"),
+    ("attention_fwd.cu", [], "attention_fwd_dispatch"),
+    ("attention_bwd.cu", [], "attention_bwd_dispatch"),
+    *[(f"attention_{d}.cu", [f"-DFLARE_ATTN_DB={db}"], f"attention_{d}_{db}") for db in (2, 1) for d in ("bwd", "fwd")],
     ("selective_scan.cu", [], "selective_scan"),
     *[("selective_scan.cu", [f"-DFLARE_SCAN_TYPE={t}"], f"selective_scan_{t.strip(chr(95))}") for t in ("float", "__nv_bfloat16", "__half")],
     ("prefill_tc.cu", [], "prefill_tc_host"),

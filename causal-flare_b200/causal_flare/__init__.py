@@ -17,6 +17,7 @@ from .semi_autoregressive.inference import (
     flare_semi_autoregressive_decode_trition,
     flare_semi_autoregressive_prefill_trition,
 )
+from .attention import flare_causal_attention, flare_causal_attention_decode, flare_causal_attention_prefill
 from .state_space import (
     flare_causal_conv,
     flare_causal_conv_decode,
@@ -34,6 +35,9 @@ __all__ = [
     "flare_autoregressive_triton",
     "flare_autoregressive_decode_triton",
     "flare_autoregressive_prefill_triton",
+    "flare_causal_attention",
+    "flare_causal_attention_decode",
+    "flare_causal_attention_prefill",
     "flare_causal_conv",
     "flare_causal_conv_decode",
     "flare_causal_conv_prefill",

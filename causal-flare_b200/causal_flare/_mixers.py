@@ -35,11 +35,37 @@ class ScanArgs(C.Structure):
     ]
 
 
-_STRUCTS = (ConvArgs, ScanArgs)
+class AttentionArgs(C.Structure):
+    _fields_ = [
+        *((name, C.c_void_p) for name in ("q", "k", "v", "y", "lse", "documents", "prefix", "cached", "lengths", "slopes", "dy", "dq", "dk", "dv",
+                                          "workspace")),
+        ("workspace_bytes", C.c_size_t),
+        *((name, C.c_int32) for name in ("B", "Nq", "Nk", "H", "J", "D")),
+        *((f"{name}_stride_{axis}", C.c_int64) for name in ("q", "k", "v", "dy") for axis in "bnh"),
+        ("scale", C.c_float), ("cap", C.c_float), ("window", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+class CacheArgs(C.Structure):
+    _fields_ = [
+        *((name, C.c_void_p) for name in ("q", "new_k", "new_v", "k_cache", "v_cache", "y", "cached", "lengths", "slopes", "workspace")),
+        ("workspace_bytes", C.c_size_t),
+        *((name, C.c_int32) for name in ("B", "N", "H", "J", "D", "L")),
+        ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64),
+        *((f"{name}_stride_{axis}", C.c_int64) for name in ("new_k", "new_v", "k", "v") for axis in "bnh"),
+        ("scale", C.c_float), ("cap", C.c_float), ("window", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+_STRUCTS = (ConvArgs, ScanArgs, AttentionArgs, CacheArgs)
 _CALLS = {"flare_conv_forward": ConvArgs, "flare_conv_backward": ConvArgs, "flare_conv_decode": ConvArgs,
-          "flare_scan_forward": ScanArgs, "flare_scan_backward": ScanArgs, "flare_scan_decode": ScanArgs}
+          "flare_scan_forward": ScanArgs, "flare_scan_backward": ScanArgs, "flare_scan_decode": ScanArgs,
+          "flare_attention_forward": AttentionArgs, "flare_attention_backward": AttentionArgs,
+          "flare_attention_append": CacheArgs, "flare_attention_decode": CacheArgs}
 _SIZES = {"flare_conv_backward_workspace_bytes": ConvArgs, "flare_scan_keep_bytes": ScanArgs,
-          "flare_scan_forward_workspace_bytes": ScanArgs, "flare_scan_backward_workspace_bytes": ScanArgs}
+          "flare_scan_forward_workspace_bytes": ScanArgs, "flare_scan_backward_workspace_bytes": ScanArgs,
+          "flare_attention_forward_workspace_bytes": AttentionArgs, "flare_attention_backward_workspace_bytes": AttentionArgs,
+          "flare_attention_decode_workspace_bytes": CacheArgs}
 
 _bound = None
 
@@ -122,3 +148,18 @@ def whole_numbers(name: str, what: str, t, shape):
 def rows(t):
     """`t`, with its innermost dimension contiguous."""
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def tiled_layout(t) -> bool:
+    """Can tiled copies fetch the rows of ``t`` where they are?  (16-byte aligned rows, none of them shared)"""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        size == 1 or (stride > 0 and stride % 8 == 0) for size, stride in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def tiled(t):
+    return t if tiled_layout(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def put_strides(a, name: str, t, axes: str) -> None:
+    for axis, size, stride in zip(axes, t.shape, t.stride()):
+        setattr(a, f"{name}_stride_{axis}", stride if size > 1 else 0)

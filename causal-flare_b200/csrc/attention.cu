@@ -1,0 +1,644 @@
+// Attention, everything but the tensor-core walks: who sees whom, <dy, y>, caches, single tokens, and the entry points.
+#include "attention.cuh"
+
+#include <limits.h>
+#include <string.h>
+
+#include "prefill_tc.cuh"
+
+namespace flare {
+namespace attn {
+namespace {
+
+using namespace mixer;
+
+// ---- who sees whom ---------------------------------------------------------------------------------------------------
+
+struct PlanParams {
+  Masks m;
+  int2* range;
+  int2* query_span;
+  int2* key_span;
+  uint8_t* dirty;
+  int32_t* ends;
+  const uint8_t* prefix;
+  const int32_t* lengths;
+  int Nq, Nk, window;
+};
+
+constexpr int kPlanThreads = 1024, kPlanPer = 4, kPlanChunk = kPlanThreads * kPlanPer;
+
+// Running maximum over a block's threads (MIN: minimum, from the last thread to the first): what lies in front of (MIN: behind)
+// this thread's values, `carry` included; `carry` then takes the whole chunk in.
+template <bool MIN>
+__device__ __forceinline__ int block_running(int v, int& carry, int* warps) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const auto pick = [](int a, int b) { return MIN ? min(a, b) : max(a, b); };
+  int run = v;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int got = MIN ? __shfl_down_sync(0xffffffffu, run, o) : __shfl_up_sync(0xffffffffu, run, o);
+    if (MIN ? lane + o < 32 : lane >= o) run = pick(run, got);
+  }
+  __syncthreads();
+  if (lane == (MIN ? 0 : 31)) warps[warp] = run;
+  __syncthreads();
+  int before = carry, all = carry;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (MIN ? w > warp : w < warp) before = pick(before, warps[w]);
+    all = pick(all, warps[w]);
+  }
+  carry = all;
+  const int next = MIN ? __shfl_down_sync(0xffffffffu, run, 1) : __shfl_up_sync(0xffffffffu, run, 1);
+  return lane == (MIN ? 31 : 0) ? before : pick(before, next);
+}
+
+// One block per row.  A token's keys begin with its run of ids (or its window) and end behind itself, or behind the prefix
+// that it is part of: the next token that is none, or that begins another run.  Latency of a few dozen steps: 2 us for 4096 tokens.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
+  pdl_begin();
+  __shared__ int warps[kPlanThreads / 32];
+  const int b = blockIdx.x, tid = threadIdx.x, Nqp = p.m.Nqp;
+  const int32_t* ids = p.m.documents != nullptr ? p.m.documents + (int64_t)b * p.Nq : nullptr;
+  const uint8_t* prefix = p.prefix != nullptr ? p.prefix + (int64_t)b * p.Nq : nullptr;
+  int cached = 0, len = p.Nq;
+  if (p.m.cached != nullptr) cached = p.m.cached[b];
+  if (p.lengths != nullptr) len = max(0, min(p.Nq, p.lengths[b]));
+  if (cached < 0 || cached > p.Nk) len = 0;
+  len = min(len, p.Nk - cached);
+  const int end = len > 0 ? cached + len : 0;
+  int2* const range = p.range + (int64_t)b * Nqp;
+  if (tid == 0) p.ends[b] = end;
+  const auto border = [&](int i) { return i == 0 || (ids != nullptr && ids[i] != ids[i - 1]); };
+  // forward: first token of the run, last token that is no prefix
+  int start_carry = 0, gap_carry = -1;
+  for (int c0 = 0; c0 < Nqp; c0 += kPlanChunk) {
+    const int i0 = c0 + tid * kPlanPer;
+    int start[kPlanPer], gap[kPlanPer], s = -1, g = -1;
+#pragma unroll
+    for (int k = 0; k < kPlanPer; ++k) {
+      const int i = i0 + k;
+      if (i < len) {
+        if (border(i)) s = i;
+        if (prefix == nullptr || prefix[i] == 0) g = i;
+      }
+      start[k] = s;
+      gap[k] = g;
+    }
+    const int s0 = block_running<false>(s, start_carry, warps), g0 = block_running<false>(g, gap_carry, warps);
+#pragma unroll
+    for (int k = 0; k < kPlanPer; ++k) {
+      const int i = i0 + k;
+      if (i >= Nqp) break;
+      int2 r = make_int2(end, end);  // nobody
+      if (i < len) {
+        const int at = cached + i;
+        if (ids != nullptr && ids[i] < 0) {
+          r = make_int2(i, i);
+        } else {
+          const int begin = max(s0, start[k]);
+          r.x = p.m.cached != nullptr ? 0 : begin;
+          if (p.window > 0) r.x = max(r.x, at - p.window + 1);
+          r.y = max(g0, gap[k]) < begin ? -1 : at + 1;  // (-1: part of the prefix, see below)
+        }
+      }
+      range[i] = r;
+    }
+  }
+  if (prefix != nullptr) {
+    int stop_carry = len;
+    for (int c0 = (Nqp - 1) / kPlanChunk * kPlanChunk; c0 >= 0; c0 -= kPlanChunk) {
+      const int i0 = c0 + tid * kPlanPer;
+      int stop[kPlanPer], s = INT_MAX;  // first stop behind token i
+#pragma unroll
+      for (int k = kPlanPer - 1; k >= 0; --k) {
+        stop[k] = s;
+        const int i = i0 + k;
+        if (i < len && (prefix[i] == 0 || border(i))) s = i;
+      }
+      const int s0 = block_running<true>(s, stop_carry, warps);
+#pragma unroll
+      for (int k = 0; k < kPlanPer; ++k) {
+        const int i = i0 + k;
+        if (i < len && range[i].y == -1) range[i].y = cached + min(s0, stop[k]);
+      }
+    }
+  }
+  __syncthreads();
+  // tiles of 128 queries: a warp each
+  const int lane = tid & 31;
+  for (int t = tid >> 5; t < Nqp / 128; t += kPlanThreads / 32) {
+    int lo = INT_MAX, hi = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int2 r = range[t * 128 + k * 32 + lane];
+      if (r.y > r.x) {
+        lo = min(lo, r.x);
+        hi = max(hi, r.y);
+      }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) p.query_span[(int64_t)b * (Nqp / 128) + t] = hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
+  }
+  // tiles of 128 keys: the first query whose keys end behind the tile's first, and the first whose keys begin behind its last
+  for (int t = tid; t < p.m.Nkp / 128; t += kPlanThreads) {
+    int2 s = make_int2(0, 0);
+    if (p.m.cached == nullptr) {
+      int a = 0, z = p.Nq;
+      while (a < z) {
+        const int mid = (a + z) / 2;
+        if (range[mid].y > t * 128) z = mid;
+        else a = mid + 1;
+      }
+      s.x = a;
+      z = p.Nq;
+      while (a < z) {
+        const int mid = (a + z) / 2;
+        if (range[mid].x >= t * 128 + 128) z = mid;
+        else a = mid + 1;
+      }
+      s.y = a;
+    }
+    p.key_span[(int64_t)b * (p.m.Nkp / 128) + t] = s;
+  }
+  for (int t = tid >> 5; t < p.m.Nkp / 64; t += kPlanThreads / 32) {
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int j = t * 64 + k * 32 + lane;
+      bad |= j < p.Nk && (j >= end || (ids != nullptr && ids[j] < 0));
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) p.dirty[(int64_t)b * (p.m.Nkp / 64) + t] = bad;
+  }
+}
+
+// delta = <dy, y>, half a warp per row and head; 0 for queries without keys (their dy may hold anything)
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(const AttnParams p, const T* dy, int64_t sb, int64_t sn, int64_t sh, float* delta) {
+  pdl_begin();
+  const int lane = threadIdx.x & 15;
+  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, total = (int64_t)p.B * p.masks.Nqp * p.H;
+  const bool live = idx < total;
+  const int64_t row = live ? idx / p.H : 0;
+  const int h = live ? (int)(idx - row * p.H) : 0, b = (int)(row / p.masks.Nqp), i = (int)(row - (int64_t)b * p.masks.Nqp);
+  const int2 r = p.masks.range[(int64_t)b * p.masks.Nqp + i];
+  float sum = 0.0f;
+  if (live && i < p.Nq && r.y > r.x && lane * 8 < p.D) {
+    float a[8], c[8];
+    unpack8(load_raw8<T>(dy + b * sb + i * sn + h * sh + lane * 8, 8, true), a);
+    unpack8(load_raw8<T>(reinterpret_cast<const T*>(p.y) + (((int64_t)b * p.Nq + i) * p.H + h) * p.D + lane * 8, 8, true), c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = fmaf(a[k], c[k], sum);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (live && lane == 0) delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum;
+}
+
+struct Layout {
+  size_t range, query_span, key_span, dirty, ends, delta, bytes;
+  int Nqp, Nkp;
+};
+Layout layout(const flare_attention_args_t& a, bool backward) {
+  Layout l;
+  l.Nqp = (a.Nq + 127) / 128 * 128;
+  l.Nkp = (a.Nk + 127) / 128 * 128;
+  size_t at = 0;
+  const auto take = [&](size_t n) {
+    const size_t here = at;
+    at += align_up(n, 256);
+    return here;
+  };
+  l.range = take((size_t)a.B * l.Nqp * sizeof(int2));
+  l.query_span = take((size_t)a.B * (l.Nqp / 128) * sizeof(int2));
+  l.key_span = take((size_t)a.B * (l.Nkp / 128) * sizeof(int2));
+  l.dirty = take((size_t)a.B * (l.Nkp / 64));
+  l.ends = take((size_t)a.B * 4);
+  l.delta = take(backward ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
+  l.bytes = at;
+  return l;
+}
+
+bool strides_fit(const void* p, std::initializer_list<int64_t> strides) {
+  if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u)) return false;
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return false;
+  return true;
+}
+
+int check(const flare_attention_args_t* args) {
+  if (args == nullptr) return FLARE_ERR_BAD_POINTER;
+  const flare_attention_args_t& a = *args;
+  if (a.B <= 0 || a.Nq <= 0 || a.Nk <= 0 || a.H <= 0 || a.J <= 0 || a.D <= 0 || a.H % a.J) return FLARE_ERR_BAD_SHAPE;
+  if (a.D % 8 || a.D > 128 || a.Nq > INT_MAX - 8192 || a.Nk > INT_MAX - 8192) return FLARE_ERR_UNSUPPORTED;
+  if (a.dtype != FLARE_BF16 && a.dtype != FLARE_F16) return FLARE_ERR_BAD_DTYPE;
+  if (!(a.scale > 0.0f) || !(a.cap >= 0.0f) || a.window < 0) return FLARE_ERR_BAD_CONFIG;
+  if (a.cached == nullptr ? a.Nk != a.Nq : a.documents != nullptr) return FLARE_ERR_BAD_CONFIG;
+  if (!strides_fit(a.q, {a.q_stride_b, a.q_stride_n, a.q_stride_h}) || !strides_fit(a.k, {a.k_stride_b, a.k_stride_n, a.k_stride_h}) ||
+      !strides_fit(a.v, {a.v_stride_b, a.v_stride_n, a.v_stride_h}) || !strides_fit(a.y, {}))
+    return FLARE_ERR_BAD_POINTER;
+  return FLARE_OK;
+}
+
+// parameters, and the masks' kernel
+int begin(const flare_attention_args_t& a, const Layout& l, AttnParams& p, cudaStream_t stream) {
+  memset(&p, 0, sizeof(p));
+  uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
+  PlanParams plan;
+  plan.range = reinterpret_cast<int2*>(ws + l.range);
+  plan.query_span = reinterpret_cast<int2*>(ws + l.query_span);
+  plan.key_span = reinterpret_cast<int2*>(ws + l.key_span);
+  plan.dirty = ws + l.dirty;
+  plan.ends = reinterpret_cast<int32_t*>(ws + l.ends);
+  p.masks = {plan.range, plan.query_span, plan.key_span, plan.dirty, plan.ends, a.documents, a.cached, l.Nqp, l.Nkp};
+  plan.m = p.masks;
+  plan.prefix = a.prefix;
+  plan.lengths = a.lengths;
+  plan.Nq = a.Nq; plan.Nk = a.Nk; plan.window = a.window;
+  p.slopes = a.slopes;
+  p.lse = a.lse;
+  p.y = a.y; p.dq = a.dq; p.dk = a.dk; p.dv = a.dv;
+  p.B = a.B; p.Nq = a.Nq; p.Nk = a.Nk; p.H = a.H; p.J = a.J; p.D = a.D;
+  p.scale = a.scale; p.cap = a.cap;
+  if (const int rc = tc_error_word(&p.err)) return rc;
+  LaunchTimer timer("attention_plan_kernel", stream);
+  FLARE_CUDA_CHECK(launch_pdl(plan_kernel, dim3((unsigned)a.B), dim3(kPlanThreads), 0, stream, plan));
+  return FLARE_OK;
+}
+
+// ---- caches and single tokens --------------------------------------------------------------------------------------------
+
+__global__ void __launch_bounds__(256) append_kernel(const flare_cache_args_t a) {
+  pdl_begin();
+  const int pieces = a.D >> 3;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = (int64_t)a.N * a.J * pieces;
+  if (idx >= a.B * per) return;
+  const int64_t b = idx / per;
+  int64_t r = idx - b * per;
+  const int t = (int)(r / (a.J * pieces));
+  r -= (int64_t)t * a.J * pieces;
+  const int j = (int)(r / pieces), c = (int)(r % pieces) * 8;
+  const int len = a.lengths != nullptr ? a.lengths[b] : a.N;
+  const int64_t at = (int64_t)(a.cached != nullptr ? a.cached[b] : 0) + t;
+  // (a row that begins outside its cache is left alone: its tokens see nothing, either)
+  if (t >= len || at - t < 0 || at >= a.L) return;
+  const uint16_t* k = reinterpret_cast<const uint16_t*>(a.new_k) + b * a.new_k_stride_b + t * a.new_k_stride_n + j * a.new_k_stride_h + c;
+  const uint16_t* v = reinterpret_cast<const uint16_t*>(a.new_v) + b * a.new_v_stride_b + t * a.new_v_stride_n + j * a.new_v_stride_h + c;
+  uint16_t* ko = reinterpret_cast<uint16_t*>(a.k_cache) + b * a.k_stride_b + at * a.k_stride_n + j * a.k_stride_h + c;
+  uint16_t* vo = reinterpret_cast<uint16_t*>(a.v_cache) + b * a.v_stride_b + at * a.v_stride_n + j * a.v_stride_h + c;
+  *reinterpret_cast<uint4*>(ko) = *reinterpret_cast<const uint4*>(k);
+  *reinterpret_cast<uint4*>(vo) = *reinterpret_cast<const uint4*>(v);
+}
+
+struct DecodeParams {
+  flare_cache_args_t a;
+  float* part;  // [splits][B][H][D + 2]: unnormalised sums, maximum (log 2), denominator; null: one split, y is written
+  int splits, head_groups;
+};
+
+constexpr int kDecodeWarps = 4, kHeads = 16;  // heads of a block: the rows of a product
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// One token.  Bound by memory: every key and value in sight is read once, by one block for up to 16 query heads that share
+// them.  A warp takes 16 keys at a time, straight from memory into the operands of m16n8k16 products: heads are the rows, so the
+// scores come out as the A operand that the product with V takes.  A thread's 16-byte piece of a key covers the contraction in an
+// order of its own (the queries are laid out in the same one); pairs of keys of V are formed by byte permutes.  Rows are cut into `splits` parts
+// for the SMs, whose sums a second kernel joins; the warps of a block join theirs in shared memory.
+template <int DB, bool F16>
+__global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeParams p) {
+  pdl_begin();
+  const flare_cache_args_t& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int split = blockIdx.x, j = blockIdx.y / p.head_groups, b = blockIdx.z, group = a.H / a.J;
+  const int h0 = j * group + (blockIdx.y % p.head_groups) * kHeads, heads = min(kHeads, (j + 1) * group - h0);
+  const int position = a.cached[b];
+  const bool idle = position < 0 || position >= a.L;
+  __shared__ float joined[kDecodeWarps][kHeads][64 * DB + 2];
+  const uint16_t* const new_k = reinterpret_cast<const uint16_t*>(a.new_k) + b * a.new_k_stride_b + j * a.new_k_stride_h;
+  const uint16_t* const new_v = reinterpret_cast<const uint16_t*>(a.new_v) + b * a.new_v_stride_b + j * a.new_v_stride_h;
+  const uint16_t* const keys = reinterpret_cast<const uint16_t*>(a.k_cache) + b * a.k_stride_b + j * a.k_stride_h;
+  const uint16_t* const values = reinterpret_cast<const uint16_t*>(a.v_cache) + b * a.v_stride_b + j * a.v_stride_h;
+  // the token's row of the cache, which no block of this launch reads
+  if (!idle && split == 0 && blockIdx.y % p.head_groups == 0 && threadIdx.x < (a.D >> 3)) {
+    const int d = threadIdx.x * 8;
+    uint16_t* ko = reinterpret_cast<uint16_t*>(a.k_cache) + b * a.k_stride_b + position * a.k_stride_n + j * a.k_stride_h + d;
+    uint16_t* vo = reinterpret_cast<uint16_t*>(a.v_cache) + b * a.v_stride_b + position * a.v_stride_n + j * a.v_stride_h + d;
+    *reinterpret_cast<uint4*>(ko) = *reinterpret_cast<const uint4*>(new_k + d);
+    *reinterpret_cast<uint4*>(vo) = *reinterpret_cast<const uint4*>(new_v + d);
+  }
+  const int first = a.window > 0 ? max(0, position - a.window + 1) : 0;
+  const int chunks = idle ? 0 : (position - first + 16) / 16;  // of 16 keys, the new one among them
+  const int per = (chunks + p.splits - 1) / p.splits, begin = split * per, end = min(chunks, begin + per);
+
+  // queries: k-step s of segment g (32 columns) takes columns 8 c + 4 s .. + 3
+  uint32_t q[2 * DB][2][4];
+#pragma unroll
+  for (int g = 0; g < 2 * DB; ++g)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {  // rows r and r + 8
+      const int h = r + half * 8, d = g * 32 + c * 8;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (h < heads && d < a.D) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + b * a.q_stride_b + (h0 + h) * a.q_stride_h + d);
+      q[g][0][half] = v.x; q[g][0][half + 2] = v.y;
+      q[g][1][half] = v.z; q[g][1][half + 2] = v.w;
+    }
+  const float plain = a.scale * kLog2e, cap_in = a.cap > 0.0f ? 2.0f * kLog2e * a.scale / a.cap : 0.0f, cap_out = a.cap * kLog2e;
+  float slope[2] = {0.0f, 0.0f};
+  if (a.slopes != nullptr)
+    for (int half = 0; half < 2; ++half)
+      if (r + half * 8 < heads) slope[half] = a.slopes[h0 + r + half * 8] * kLog2e;
+  float o[DB * 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int n = 0; n < DB * 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+
+  for (int chunk = begin + warp; chunk < end; chunk += kDecodeWarps) {
+    const int key0 = first + chunk * 16;
+    uint4 kr[2][2 * DB], vr[4][DB];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int key = key0 + n * 8 + r;
+      const uint16_t* row = key < position ? keys + key * a.k_stride_n : new_k;
+#pragma unroll
+      for (int g = 0; g < 2 * DB; ++g) {
+        const int d = g * 32 + c * 8;
+        kr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int key = key0 + 2 * c + (n & 1) + (n >> 1) * 8;
+      const uint16_t* row = key < position ? values + key * a.v_stride_n : new_v;
+#pragma unroll
+      for (int g = 0; g < DB; ++g) {
+        const int d = g * 64 + r * 8;
+        vr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    float s[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 2 * DB; ++g) {
+        mma16816<F16>(s[n], q[g][0], kr[n][g].x, kr[n][g].y);
+        mma16816<F16>(s[n], q[g][1], kr[n][g].z, kr[n][g].w);
+      }
+    }
+    // s[n][2 half + i]: head r + 8 half, key key0 + 8 n + 2 c + i
+    float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + n * 8 + 2 * c + (e & 1);
+        float x = s[n][e];
+        if (a.cap > 0.0f) x = fmaf(-2.0f * cap_out, __fdividef(1.0f, exp2f(x * cap_in) + 1.0f), cap_out);
+        else x *= plain;
+        x = fmaf(-slope[e >> 1], (float)(position - key), x);
+        s[n][e] = key <= position ? x : -INFINITY;
+        most[e >> 1] = fmaxf(most[e >> 1], s[n][e]);
+      }
+    float scale[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      most[half] = fmaxf(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
+      most[half] = fmaxf(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
+      const float to = fmaxf(top[half], most[half]);
+      scale[half] = top[half] == -INFINITY ? 0.0f : exp2f(top[half] - to);
+      top[half] = to;
+      sum[half] *= scale[half];
+    }
+    const float frame[2] = {top[0] == -INFINITY ? 0.0f : top[0], top[1] == -INFINITY ? 0.0f : top[1]};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = exp2f(s[n][e] - frame[e >> 1]);
+        sum[e >> 1] += s[n][e];
+      }
+    const uint32_t w[4] = {pack_pair<F16>(s[0][0], s[0][1]), pack_pair<F16>(s[0][2], s[0][3]), pack_pair<F16>(s[1][0], s[1][1]),
+                           pack_pair<F16>(s[1][2], s[1][3])};
+#pragma unroll
+    for (int g = 0; g < DB; ++g) {
+      const uint32_t v0[4] = {vr[0][g].x, vr[0][g].y, vr[0][g].z, vr[0][g].w}, v1[4] = {vr[1][g].x, vr[1][g].y, vr[1][g].z, vr[1][g].w};
+      const uint32_t v2[4] = {vr[2][g].x, vr[2][g].y, vr[2][g].z, vr[2][g].w}, v3[4] = {vr[3][g].x, vr[3][g].y, vr[3][g].z, vr[3][g].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float(&acc)[4] = o[g * 8 + e];
+        acc[0] *= scale[0]; acc[1] *= scale[0];
+        acc[2] *= scale[1]; acc[3] *= scale[1];
+        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+        mma16816<F16>(acc, w, __byte_perm(v0[e >> 1], v1[e >> 1], sel), __byte_perm(v2[e >> 1], v3[e >> 1], sel));
+      }
+    }
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 1);
+    sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 2);
+  }
+  // o[g * 8 + e][2 half + i]: head r + 8 half, column 64 g + 8 (2 c + i) + e
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float* const row = joined[warp][r + half * 8];
+#pragma unroll
+    for (int n = 0; n < DB * 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) row[(n >> 3) * 64 + (2 * c + i) * 8 + (n & 7)] = o[n][2 * half + i];
+    if (c == 0) {
+      row[64 * DB] = top[half];
+      row[64 * DB + 1] = sum[half];
+    }
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < heads * a.D; idx += 32 * kDecodeWarps) {
+    const int h = idx / a.D, d = idx - h * a.D;
+    float t = -INFINITY, l = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) t = fmaxf(t, joined[w][h][64 * DB]);
+    const float frame = t == -INFINITY ? 0.0f : t;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      const float f = exp2f(joined[w][h][64 * DB] - frame);
+      l = fmaf(joined[w][h][64 * DB + 1], f, l);
+      v = fmaf(joined[w][h][d], f, v);
+    }
+    const int64_t row = (int64_t)b * a.H + h0 + h;
+    if (p.part == nullptr) {
+      store1(a.y, a.dtype, row * a.D + d, idle ? 0.0f : v / l);
+    } else {
+      float* const out = p.part + ((int64_t)split * a.B * a.H + row) * (a.D + 2);
+      out[d] = v;
+      if (d == 0) {
+        out[a.D] = t;
+        out[a.D + 1] = l;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) decode_join_kernel(const DecodeParams p) {
+  pdl_begin();
+  const flare_cache_args_t& a = p.a;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.H;
+  if (idx >= rows * a.D) return;
+  const int64_t row = idx / a.D;
+  const int d = (int)(idx - row * a.D);
+  float t = -INFINITY, l = 0.0f, v = 0.0f;
+  for (int s = 0; s < p.splits; ++s) t = fmaxf(t, p.part[(s * rows + row) * (a.D + 2) + a.D]);
+  const float frame = t == -INFINITY ? 0.0f : t;
+  for (int s = 0; s < p.splits; ++s) {
+    const float* in = p.part + (s * rows + row) * (a.D + 2);
+    const float f = exp2f(in[a.D] - frame);
+    l = fmaf(in[a.D + 1], f, l);
+    v = fmaf(in[d], f, v);
+  }
+  store1(a.y, a.dtype, idx, l == 0.0f ? 0.0f : v / l);  // (0: an idle row)
+}
+
+int check_cache(const flare_cache_args_t* args, bool decode) {
+  if (args == nullptr) return FLARE_ERR_BAD_POINTER;
+  const flare_cache_args_t& a = *args;
+  if (a.B <= 0 || a.J <= 0 || a.D <= 0 || a.L <= 0 || (decode ? a.H <= 0 || a.H % a.J : a.N <= 0)) return FLARE_ERR_BAD_SHAPE;
+  if (a.D % 8 || a.D > 128 || a.L > INT_MAX - 8192 || a.B > 65535) return FLARE_ERR_UNSUPPORTED;
+  if (a.dtype != FLARE_BF16 && a.dtype != FLARE_F16) return FLARE_ERR_BAD_DTYPE;
+  if (!strides_fit(a.new_k, {a.new_k_stride_b, a.new_k_stride_n, a.new_k_stride_h}) || !strides_fit(a.new_v, {a.new_v_stride_b, a.new_v_stride_n, a.new_v_stride_h}) ||
+      !strides_fit(a.k_cache, {a.k_stride_b, a.k_stride_n, a.k_stride_h}) || !strides_fit(a.v_cache, {a.v_stride_b, a.v_stride_n, a.v_stride_h}))
+    return FLARE_ERR_BAD_POINTER;
+  if (!decode) return FLARE_OK;
+  if (!(a.scale > 0.0f) || !(a.cap >= 0.0f) || a.window < 0) return FLARE_ERR_BAD_CONFIG;
+  if (!strides_fit(a.q, {a.q_stride_b, a.q_stride_h}) || a.y == nullptr || a.cached == nullptr) return FLARE_ERR_BAD_POINTER;
+  return FLARE_OK;
+}
+
+// Four blocks for every SM, of 64 keys at least: a block's warps then have 32 KB on their way.
+DecodeParams plan_decode(const flare_cache_args_t& a) {
+  DecodeParams p;
+  p.a = a;
+  p.part = nullptr;
+  p.head_groups = (a.H / a.J + kHeads - 1) / kHeads;
+  const int64_t blocks = (int64_t)a.B * a.J * p.head_groups;
+  const int sight = a.window > 0 && a.window < a.L ? a.window : a.L;
+  int64_t splits = ((int64_t)sm_count() * 4 + blocks - 1) / blocks;
+  if (splits > (sight + 63) / 64) splits = (sight + 63) / 64;
+  p.splits = (int)splits;
+  return p;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace flare
+
+using namespace flare;
+using namespace flare::attn;
+
+extern "C" {
+
+size_t flare_attention_forward_workspace_bytes(const flare_attention_args_t* args) {
+  if (args == nullptr || args->B <= 0 || args->Nq <= 0 || args->Nk <= 0) return 0;
+  return layout(*args, false).bytes;
+}
+size_t flare_attention_backward_workspace_bytes(const flare_attention_args_t* args) {
+  if (args == nullptr || args->B <= 0 || args->Nq <= 0 || args->Nk <= 0 || args->H <= 0) return 0;
+  return layout(*args, true).bytes;
+}
+
+int flare_attention_forward(const flare_attention_args_t* args, flare_stream_t stream) {
+  if (const int rc = check(args)) return rc;
+  const flare_attention_args_t& a = *args;
+  const Layout l = layout(a, false);
+  if (a.workspace == nullptr || a.workspace_bytes < l.bytes || (reinterpret_cast<uintptr_t>(a.workspace) & 255u)) return FLARE_ERR_WORKSPACE;
+  AttnParams p;
+  if (const int rc = begin(a, l, p, stream)) return rc;
+  return launch_forward_tc(a, p, stream);
+}
+
+int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t stream) {
+  if (const int rc = check(args)) return rc;
+  const flare_attention_args_t& a = *args;
+  if (a.cached != nullptr || a.lengths != nullptr) return FLARE_ERR_BAD_CONFIG;
+  if (!strides_fit(a.dy, {a.dy_stride_b, a.dy_stride_n, a.dy_stride_h}) || !strides_fit(a.dq, {}) || !strides_fit(a.dk, {}) ||
+      !strides_fit(a.dv, {}) || !strides_fit(a.lse, {}))
+    return FLARE_ERR_BAD_POINTER;
+  const Layout l = layout(a, true);
+  if (a.workspace == nullptr || a.workspace_bytes < l.bytes || (reinterpret_cast<uintptr_t>(a.workspace) & 255u)) return FLARE_ERR_WORKSPACE;
+  AttnParams p;
+  if (const int rc = begin(a, l, p, stream)) return rc;
+  float* const delta = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.workspace) + l.delta);
+  p.delta = delta;
+  const int64_t blocks = ((int64_t)a.B * l.Nqp * a.H * 16 + 255) / 256;
+  if (blocks > INT_MAX) return FLARE_ERR_UNSUPPORTED;
+  {
+    LaunchTimer timer("attention_delta_kernel", stream);
+    if (a.dtype == FLARE_F16)
+      FLARE_CUDA_CHECK(launch_pdl(delta_kernel<__half>, dim3((unsigned)blocks), dim3(256), 0, stream, p, reinterpret_cast<const __half*>(a.dy),
+                                  a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, delta));
+    else
+      FLARE_CUDA_CHECK(launch_pdl(delta_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, stream, p,
+                                  reinterpret_cast<const __nv_bfloat16*>(a.dy), a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, delta));
+  }
+  return launch_backward_tc(a, p, stream);
+}
+
+int flare_attention_append(const flare_cache_args_t* args, flare_stream_t stream) {
+  if (const int rc = check_cache(args, false)) return rc;
+  const flare_cache_args_t& a = *args;
+  const int64_t blocks = ((int64_t)a.B * a.N * a.J * (a.D >> 3) + 255) / 256;
+  if (blocks > INT_MAX) return FLARE_ERR_UNSUPPORTED;
+  LaunchTimer timer("attention_append_kernel", stream);
+  FLARE_CUDA_CHECK(launch_pdl(append_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a));
+  return FLARE_OK;
+}
+
+size_t flare_attention_decode_workspace_bytes(const flare_cache_args_t* args) {
+  if (check_cache(args, true)) return 0;
+  const DecodeParams p = plan_decode(*args);
+  return p.splits > 1 ? (size_t)p.splits * args->B * args->H * (args->D + 2) * sizeof(float) : 0;
+}
+
+int flare_attention_decode(const flare_cache_args_t* args, flare_stream_t stream) {
+  if (const int rc = check_cache(args, true)) return rc;
+  const flare_cache_args_t& a = *args;
+  DecodeParams p = plan_decode(a);
+  if (p.splits > 1) {
+    if (a.workspace == nullptr || a.workspace_bytes < flare_attention_decode_workspace_bytes(args)) return FLARE_ERR_WORKSPACE;
+    p.part = reinterpret_cast<float*>(a.workspace);
+  }
+  if ((int64_t)a.J * p.head_groups > 65535) return FLARE_ERR_UNSUPPORTED;
+  auto* const kernel = a.D <= 64 ? (a.dtype == FLARE_F16 ? decode_kernel<1, true> : decode_kernel<1, false>)
+                                 : (a.dtype == FLARE_F16 ? decode_kernel<2, true> : decode_kernel<2, false>);
+  {
+    LaunchTimer timer("attention_decode_kernel", stream);
+    FLARE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)p.splits, (unsigned)(a.J * p.head_groups), (unsigned)a.B), dim3(32 * kDecodeWarps), 0, stream, p));
+  }
+  if (p.splits == 1) return FLARE_OK;
+  const int64_t blocks = ((int64_t)a.B * a.H * a.D + 255) / 256;
+  if (blocks > INT_MAX) return FLARE_ERR_UNSUPPORTED;
+  LaunchTimer timer("attention_decode_join_kernel", stream);
+  FLARE_CUDA_CHECK(launch_pdl(decode_join_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p));
+  return FLARE_OK;
+}
+
+}  // extern "C"

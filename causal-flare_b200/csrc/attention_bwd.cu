@@ -1,0 +1,337 @@
+// Attention backward on tcgen05, deterministic: one kernel for dK and dV, one for dQ, the same code on either side.
+//
+//   P = exp2(scores - lse),  dS = P (dP - delta), dP = dY V^T, delta = <dY, y>; behind the cap dS *= 1 - tanh^2 = 4 r (1 - r)
+//   dV = P^T dY,  dK = scale dS^T Q,  dQ = scale dS K
+//
+// A CTA keeps 128 rows of its own side (KEYS: K and V; else Q and dY) and walks tiles of 64 rows of the other: S = X0 Y0^T and
+// dP = X1 Y1^T into tensor memory, rows of the own side on the lanes; the threads turn them into P and dS, laid down over S and dP
+// as packed 16-bit values, from where the products that are summed over the walk take their A operand (dV += P Y1,
+// dK or dQ += dS Y0): neither P nor dS passes through shared memory, and no gradient is added by two CTAs (a key head's dK and dV walk its
+// query heads one after the other).  The price is S and dP twice, 14 instead of 10 products of D operations for a pair.  Two groups of
+// four warps work on every other tile, so that one's exponentials run under the other's products.
+//
+// Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384.  P and dS are rounded once, to the type of the
+// operands they meet (fp16: what of dS lies below 2^-14 keeps an absolute 2^-25, as the gradients themselves do); everything in front
+// of that, and the sums, is fp32.
+#include "attention_tc.cuh"
+
+namespace flare {
+namespace attn {
+
+#ifdef FLARE_ATTN_DB
+
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr int kStages = 4, kWalk = 64;
+
+struct Stats {  // of a tile of queries (KEYS)
+  float lse[kWalk], delta[kWalk];
+  int2 keys[kWalk];
+};
+struct Misc {
+  alignas(16) Stats stats[kStages];
+  uint64_t own_full, full[kStages], empty[kStages], s_full[2], w_ready[2], done;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+template <int DB>
+struct Layout {
+  static constexpr int OWN = DB * 16384, TILE = DB * 8192;
+  static constexpr int Y = 2 * OWN, MISC = Y + kStages * 2 * TILE, BYTES = MISC + (int)sizeof(Misc) + 1024;
+};
+
+// contiguous bytes, 16-byte aligned on both sides
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int DB, bool F16, bool CAP, bool BIAS, bool KEYS>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __grid_constant__ CUtensorMap tm_x1,
+                          const __grid_constant__ CUtensorMap tm_y0, const __grid_constant__ CUtensorMap tm_y1, const AttnParams p) {
+  using L = Layout<DB>;
+  constexpr uint32_t T_DS = 256, T_P = 384;
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  Misc* const misc = reinterpret_cast<Misc*>(smem + L::MISC);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&misc->own_full, 1);
+    mbar_init(&misc->done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&misc->s_full[i], 1);
+      mbar_init(&misc->w_ready[i], 4);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&misc->full[i], 1);
+      mbar_init(&misc->empty[i], 1);
+    }
+    misc->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(&misc->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = misc->tmem_base;
+  pdl_wait();
+
+  // causal: the longest walks first, those of the first keys and of the last queries
+  const int group = p.H / p.J, heads = KEYS ? p.J : p.H, lanes = p.B * heads;
+  const int tile = KEYS ? blockIdx.x / lanes : gridDim.x / lanes - 1 - blockIdx.x / lanes;
+  const int b = blockIdx.x % lanes / heads, head = blockIdx.x % heads, x0 = tile * 128;
+  const int2 span = KEYS ? p.masks.key_span[b * (p.masks.Nkp >> 7) + tile] : p.masks.query_span[b * (p.masks.Nqp >> 7) + tile];
+  const int first = span.x / kWalk, per_head = span.y > span.x ? (span.y + kWalk - 1) / kWalk - first : 0;
+  const int total = KEYS ? per_head * group : per_head;
+  const auto row_of = [&](int n) { return (first + (KEYS ? n % per_head : n)) * kWalk; };
+  const auto head_of = [&](int n) { return KEYS ? head * group + n / per_head : head / group; };
+  bool ok = true;
+  const auto wait_one = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, &misc->abort_flag, 8); };
+  // (whole warps give up together)
+  const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_one(bar, parity)) != 0; };
+
+  if (warp == kWarpTma) {
+    if (total > 0 && elect_one()) {
+      mbar_arrive_expect_tx(&misc->own_full, 2 * L::OWN);
+      for (int d = 0; d < DB; ++d) {
+        tma_load_4d(smem + d * 16384, &tm_x0, &misc->own_full, d * 64, head, x0, b);
+        tma_load_4d(smem + L::OWN + d * 16384, &tm_x1, &misc->own_full, d * 64, head, x0, b);
+      }
+      for (int n = 0; n < total; ++n) {
+        const int s = n % kStages, row = row_of(n), hd = head_of(n);
+        if (!(ok = wait_one(&misc->empty[s], ((n / kStages) & 1) ^ 1))) break;
+        uint8_t* const y = smem + L::Y + s * 2 * L::TILE;
+        mbar_arrive_expect_tx(&misc->full[s], 2 * L::TILE + (KEYS ? (uint32_t)sizeof(Stats) : 0u));
+        for (int d = 0; d < DB; ++d) {
+          tma_load_4d(y + d * 8192, &tm_y0, &misc->full[s], d * 64, hd, row, b);
+          tma_load_4d(y + L::TILE + d * 8192, &tm_y1, &misc->full[s], d * 64, hd, row, b);
+        }
+        if (KEYS) {
+          const int64_t at = ((int64_t)b * p.H + hd) * p.masks.Nqp + row;
+          bulk_load(misc->stats[s].lse, p.lse + at, kWalk * 4, &misc->full[s]);
+          bulk_load(misc->stats[s].delta, p.delta + at, kWalk * 4, &misc->full[s]);
+          bulk_load(misc->stats[s].keys, p.masks.range + (int64_t)b * p.masks.Nqp + row, kWalk * 8, &misc->full[s]);
+        }
+      }
+    }
+  } else if (warp == kWarpMma) {
+    constexpr uint32_t ID_S = make_idesc<F16>(128, kWalk, 0, 0);
+    constexpr uint32_t ID_SUM = make_idesc<F16>(128, 64 * DB, 0, 1);
+    const auto step_y = [](uint64_t desc, int i) { return desc + (uint64_t)(((i >> 2) * 8192 + (i & 3) * 32) >> 4); };
+    const auto scores = [&](int n) {
+      const int s = n % kStages, slot = n & 1;
+      if (!(ok = wait(&misc->full[s], (n / kStages) & 1))) return;
+      uint8_t* const y = smem + L::Y + s * 2 * L::TILE;
+      if (p.masks.dirty[(int64_t)b * (p.masks.Nkp >> 6) + row_of(n) / kWalk]) {
+        clear_rows<DB, kWalk>(y, p.masks, b, p.Nk, row_of(n), lane);
+        clear_rows<DB, kWalk>(y + L::TILE, p.masks, b, p.Nk, row_of(n), lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint64_t dx0 = make_desc_sw128(smem_u32(smem), 16, 1024), dx1 = make_desc_sw128(smem_u32(smem + L::OWN), 16, 1024);
+        const uint64_t dy0 = make_desc_sw128(smem_u32(y), 16, 1024), dy1 = make_desc_sw128(smem_u32(y + L::TILE), 16, 1024);
+#pragma unroll
+        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128, kmaj_step(dx0, i), step_y(dy0, i), ID_S, i > 0);
+#pragma unroll
+        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128 + 64, kmaj_step(dx1, i), step_y(dy1, i), ID_S, i > 0);
+        tc_commit(&misc->s_full[slot]);
+      }
+      __syncwarp();
+    };
+    if (total > 0) {
+      ok = wait(&misc->own_full, 0);
+      if (ok) scores(0);
+      if (ok && total > 1) scores(1);
+      for (int n = 0; ok && n < total; ++n) {
+        const int s = n % kStages, slot = n & 1;
+        if (!(ok = wait(&misc->w_ready[slot], (n >> 1) & 1))) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint32_t y = smem_u32(smem + L::Y + s * 2 * L::TILE);
+          const uint64_t dy0 = make_desc_sw128(y, 8192, 1024), dy1 = make_desc_sw128(y + L::TILE, 8192, 1024);
+          if (KEYS) {
+#pragma unroll
+            for (int i = 0; i < kWalk / 16; ++i) mma_ts(tmem + T_P, tmem + slot * 128 + i * 8, mnmaj_step(dy1, i), ID_SUM, i > 0 || n > 0);
+          }
+#pragma unroll
+          for (int i = 0; i < kWalk / 16; ++i) mma_ts(tmem + T_DS, tmem + slot * 128 + 64 + i * 8, mnmaj_step(dy0, i), ID_SUM, i > 0 || n > 0);
+          tc_commit(&misc->empty[s]);
+          if (n + 1 == total) tc_commit(&misc->done);
+        }
+        __syncwarp();
+        if (n + 2 < total) scores(n + 2);  // (behind the products that read P and dS where it goes: products run in order)
+      }
+    }
+  } else {
+    const int slot = warp >> 2, row = x0 + (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + slot * 128, td = ts + 64;
+    float lse = INFINITY, delta = 0.0f;
+    int2 keys = make_int2(0, 0);
+    if (!KEYS) {
+      const int64_t at = ((int64_t)b * p.H + head) * p.masks.Nqp + row;
+      lse = p.lse[at];
+      delta = p.delta[at];
+      keys = p.masks.range[(int64_t)b * p.masks.Nqp + row];
+    }
+    ScoreScale sc = score_scale(p, KEYS ? head * group : head);
+#pragma unroll 1
+    for (int n = slot; n < total; n += 2) {
+      const int y0 = row_of(n), s_ = n % kStages;
+      if (KEYS && BIAS) sc = score_scale(p, head_of(n));
+      // (its completion follows from that of the copies, so the statistics are there too; the wait on `full` makes them visible)
+      if (KEYS && !(ok = wait(&misc->full[s_], (n / kStages) & 1))) break;
+      if (!(ok = wait(&misc->s_full[slot], (n >> 1) & 1))) break;
+      tc_fence_after_sync();
+      const Stats& st = misc->stats[s_];
+      const bool all = KEYS ? st.keys[0].y >= x0 + 128 && st.keys[kWalk - 1].x <= x0
+                            : __all_sync(0xffffffffu, keys.x <= y0 && keys.y >= y0 + kWalk) != 0;
+      const float d0 = (float)(row - y0);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], d[32];
+        tmem_ld32(ts + c * 32, s);
+        tmem_ld32(td + c * 32, d);
+        tmem_wait_ld();
+        tmem_fence_regs(s);
+        tmem_fence_regs(d);
+        float wp[2], wd[2];
+        uint32_t pw[16], dw[16];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const int col = c * 32 + k;
+          const float l = KEYS ? st.lse[col] : lse, dl = KEYS ? st.delta[col] : delta;
+          float x = __uint_as_float(s[k]), r = 0.0f;
+          if (CAP) {
+            r = cap_weight(x, sc);
+            x = capped(r, sc);
+            if (BIAS) x = fmaf(-sc.slope, fabsf(d0 - (float)col), x);
+            x -= l;
+          } else if (BIAS) {
+            x = fmaf(-sc.slope, fabsf(d0 - (float)col), x * sc.plain) - l;
+          } else {
+            x = fmaf(x, sc.plain, -l);
+          }
+          float w = ex2_approx(x);
+          float g = w * (__uint_as_float(d[k]) - dl);
+          if (CAP) g *= 4.0f * r * (1.0f - r);
+          if (!all) {
+            const int2 see = KEYS ? st.keys[col] : keys;
+            const int key = KEYS ? row : y0 + col;
+            const bool on = key >= see.x && key < see.y;
+            w = on ? w : 0.0f;
+            g = on ? g : 0.0f;
+          }
+          wp[k & 1] = w;
+          wd[k & 1] = g;
+          if (k & 1) {
+            pw[k >> 1] = pack2<F16>(wp[0], wp[1]);
+            dw[k >> 1] = pack2<F16>(wd[0], wd[1]);
+          }
+        }
+        // (the halves' reads come in the order of their writes: columns 16 c of what was read is all read by now)
+        if (KEYS) tmem_st16(ts + c * 16, pw);
+        tmem_st16(td + c * 16, dw);
+      }
+      tmem_wait_st();
+      tc_fence_before_sync();
+      warp_arrive(&misc->w_ready[slot], lane);
+    }
+    if (ok && total > 0) ok = wait(&misc->done, 0);
+    if (ok) {
+      tc_fence_after_sync();
+      const int rows = KEYS ? p.Nk : p.Nq;
+      const int64_t at = (((int64_t)b * rows + row) * heads + head) * p.D;
+      const auto put = [&](void* out, uint32_t t, int c, float f) {
+        uint32_t r[32];
+        if (total > 0) {
+          tmem_read<32>(tl + t + c * 32, r);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0u;
+        }
+        if (row < rows) store_columns<F16>(reinterpret_cast<uint16_t*>(out) + at, c * 32, p.D, r, f);
+      };
+      if (KEYS) {  // a group each
+#pragma unroll
+        for (int c = 0; c < 2 * DB; ++c)
+          if (slot == 0) put(p.dk, T_DS, c, p.scale);
+          else put(p.dv, T_P, c, 1.0f);
+      } else {  // half the columns each
+#pragma unroll
+        for (int c = 0; c < DB; ++c) put(p.dq, T_DS, slot * DB + c, p.scale);
+      }
+    }
+  }
+  if (!ok) {
+    misc->abort_flag = 1;
+    atomicOr(p.err, 1);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+}
+
+template <bool F16, bool KEYS>
+int launch(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream) {
+  constexpr int DB = FLARE_ATTN_DB;
+  const auto map = [&](CUtensorMap* m, int which, uint32_t rows) {
+    switch (which) {
+      case 0: return head_map(m, a.q, a.B, a.Nq, a.H, a.D, a.q_stride_b, a.q_stride_n, a.q_stride_h, rows);
+      case 1: return head_map(m, a.dy, a.B, a.Nq, a.H, a.D, a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, rows);
+      case 2: return head_map(m, a.k, a.B, a.Nk, a.J, a.D, a.k_stride_b, a.k_stride_n, a.k_stride_h, rows);
+      default: return head_map(m, a.v, a.B, a.Nk, a.J, a.D, a.v_stride_b, a.v_stride_n, a.v_stride_h, rows);
+    }
+  };
+  CUtensorMap x0, x1, y0, y1;
+  const int own = KEYS ? 2 : 0;
+  if (!map(&x0, own, 128) || !map(&x1, own + 1, 128) || !map(&y0, 2 - own, kWalk) || !map(&y1, 3 - own, kWalk)) return FLARE_ERR_CUDA;
+  const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
+  auto* const kernel = cap ? (bias ? attention_backward_kernel<DB, F16, true, true, KEYS> : attention_backward_kernel<DB, F16, true, false, KEYS>)
+                           : (bias ? attention_backward_kernel<DB, F16, false, true, KEYS> : attention_backward_kernel<DB, F16, false, false, KEYS>);
+  FLARE_CUDA_CHECK(allow_smem(kernel));
+  const int64_t blocks = (int64_t)((KEYS ? a.Nk : a.Nq) + 127) / 128 * a.B * (KEYS ? a.J : a.H);
+  if (blocks > 0x7fffffff) return FLARE_ERR_UNSUPPORTED;
+  LaunchTimer timer(KEYS ? "attention_backward_kernel (keys)" : "attention_backward_kernel (queries)", stream);
+  FLARE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)blocks), dim3(kThreads), Layout<DB>::BYTES, stream, x0, x1, y0, y1, p));
+  return FLARE_OK;
+}
+
+}  // namespace
+
+template <int DB>
+int launch_backward_db(const flare_attention_args_t& a, const AttnParams& p, bool keys, cudaStream_t stream);
+template <>
+int launch_backward_db<FLARE_ATTN_DB>(const flare_attention_args_t& a, const AttnParams& p, bool keys, cudaStream_t stream) {
+  if (a.dtype == FLARE_F16) return keys ? launch<true, true>(a, p, stream) : launch<true, false>(a, p, stream);
+  return keys ? launch<false, true>(a, p, stream) : launch<false, false>(a, p, stream);
+}
+
+#else
+
+template <int DB>
+int launch_backward_db(const flare_attention_args_t& a, const AttnParams& p, bool keys, cudaStream_t stream);
+template <>
+int launch_backward_db<1>(const flare_attention_args_t& a, const AttnParams& p, bool keys, cudaStream_t stream);
+template <>
+int launch_backward_db<2>(const flare_attention_args_t& a, const AttnParams& p, bool keys, cudaStream_t stream);
+
+int launch_backward_tc(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream) {
+  for (const bool keys : {true, false})
+    if (const int rc = a.D <= 64 ? launch_backward_db<1>(a, p, keys, stream) : launch_backward_db<2>(a, p, keys, stream)) return rc;
+  return FLARE_OK;
+}
+
+#endif
+
+}  // namespace attn
+}  // namespace flare

@@ -1,0 +1,337 @@
+// Attention forward on tcgen05: y = softmax(scores) V in one pass over the keys.
+//
+// One CTA per head and 256 queries, as two groups of 128 (a thread is a query is a lane of tensor memory).  Per tile of 128 keys and
+// group: S = Q K^T into tensor memory, the group's threads read their rows, take the running maximum and lay P = exp2(S - m) down
+// over S as packed 16-bit values, O += P V takes its A operand from there.  The groups take turns on the tensor cores: while
+// one works on its exponentials the other's products run.  O stays in tensor memory; it is rescaled only where the maximum has grown by
+// more than 2^8 since the frame was set (exact: the frame cancels in O / l; P up to 2^8 is still far from the end of fp16).
+// Sums are of the unrounded weights, in fp32; P is rounded once, to the type of V, which is what the products take.
+//
+// Tensor memory: S / P of the groups at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, K and V two stages each.
+// Bound by the tensor cores and the exponentials alike (128 x 128 x 2 D products of 512 cycles against 128 x 128 / 16 exponentials).
+#include "attention_tc.cuh"
+
+namespace flare {
+namespace attn {
+
+#ifdef FLARE_ATTN_DB
+
+namespace {
+
+constexpr int kThreads = 320;  // two groups of four warps, products, copies
+constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr float kGrowth = 8.0f;
+
+struct Misc {
+  uint64_t q_full[2], k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_ready[2], o_done[2];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+template <int DB>
+struct Layout {
+  static constexpr int STAGES = DB == 1 ? 4 : 2, TILE = DB * 16384;
+  static constexpr int K = 2 * TILE, V = K + STAGES * TILE, MISC = V + STAGES * TILE, BYTES = MISC + (int)sizeof(Misc) + 1024;
+};
+
+template <int DB, bool F16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
+  using L = Layout<DB>;
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  Misc* const misc = reinterpret_cast<Misc*>(smem + L::MISC);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&misc->q_full[g], 1);
+      mbar_init(&misc->s_full[g], 1);
+      mbar_init(&misc->p_ready[g], 4);
+      mbar_init(&misc->o_done[g], 1);
+    }
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(&misc->k_full[i], 1);
+      mbar_init(&misc->k_empty[i], 1);
+      mbar_init(&misc->v_full[i], 1);
+      mbar_init(&misc->v_empty[i], 1);
+    }
+    misc->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc(&misc->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = misc->tmem_base;
+  pdl_wait();
+
+  const int lanes = p.B * p.H, block = gridDim.x / lanes - 1 - blockIdx.x / lanes;  // (causal: the longest first)
+  const int b = blockIdx.x % lanes / p.H, h = blockIdx.x % p.H, kv = h / (p.H / p.J), q0 = block * 256;
+  // tiles of keys of each group
+  int first[2], last[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int tile = block * 2 + g;
+    const int2 s = tile * 128 < p.masks.Nqp ? p.masks.query_span[b * (p.masks.Nqp >> 7) + tile] : make_int2(0, 0);
+    first[g] = s.x >> 7;
+    last[g] = s.y > s.x ? (s.y + 127) >> 7 : first[g];
+  }
+  const bool have0 = last[0] > first[0], have1 = last[1] > first[1];
+  const int j0 = have0 ? (have1 ? min(first[0], first[1]) : first[0]) : first[1];
+  const int j1 = have0 ? (have1 ? max(last[0], last[1]) : last[0]) : last[1];
+  const auto in = [&](int g, int j) { return j >= first[g] && j < last[g]; };
+  bool ok = true;
+  const auto wait_one = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, &misc->abort_flag, 8); };
+  // (whole warps give up together)
+  const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_one(bar, parity)) != 0; };
+
+  if (warp == kWarpTma) {
+    if (elect_one()) {
+      for (int g = 0; g < 2; ++g)
+        if (last[g] > first[g]) {
+          mbar_arrive_expect_tx(&misc->q_full[g], L::TILE);
+          for (int d = 0; d < DB; ++d) tma_load_4d(smem + g * L::TILE + d * 16384, &tm_q, &misc->q_full[g], d * 64, h, q0 + g * 128, b);
+        }
+      int n = 0;
+      for (int j = j0; ok && j < j1; ++j) {
+        if (!in(0, j) && !in(1, j)) continue;
+        const int s = n % L::STAGES;
+        const uint32_t phase = (n / L::STAGES) & 1;
+        if (!(ok = wait_one(&misc->k_empty[s], phase ^ 1))) break;
+        mbar_arrive_expect_tx(&misc->k_full[s], L::TILE);
+        for (int d = 0; d < DB; ++d)
+          tma_load_4d(smem + L::K + s * L::TILE + d * 16384, &tm_k, &misc->k_full[s], d * 64, kv, j * 128, b);
+        if (!(ok = wait_one(&misc->v_empty[s], phase ^ 1))) break;
+        mbar_arrive_expect_tx(&misc->v_full[s], L::TILE);
+        for (int d = 0; d < DB; ++d)
+          tma_load_4d(smem + L::V + s * L::TILE + d * 16384, &tm_v, &misc->v_full[s], d * 64, kv, j * 128, b);
+        ++n;
+      }
+    }
+  } else if (warp == kWarpMma) {
+    constexpr uint32_t ID_S = make_idesc<F16>(128, 128, 0, 0);      // Q, K: K-major
+    constexpr uint32_t ID_O = make_idesc<F16>(128, 64 * DB, 0, 1);  // P (tensor memory), V: MN-major
+    int n = 0, count[2] = {0, 0};
+    const auto scores = [&](int g, int tile) {  // of the n-th tile in the ring
+      const int s = tile % L::STAGES;
+      if (!(ok = wait(&misc->k_full[s], (tile / L::STAGES) & 1))) return;
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const uint64_t dq = make_desc_sw128(smem_u32(smem + g * L::TILE), 16, 1024);
+        const uint64_t dk = make_desc_sw128(smem_u32(smem + L::K + s * L::TILE), 16, 1024);
+#pragma unroll
+        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + g * 128, kmaj_step(dq, i), kmaj_step(dk, i), ID_S, i > 0);
+        tc_commit(&misc->s_full[g]);
+      }
+      __syncwarp();
+    };
+    for (int j = j0; ok && j < j1; ++j) {
+      if (!in(0, j) && !in(1, j)) continue;
+      const int s = n % L::STAGES;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (ok && in(g, j) && j == first[g] && (ok = wait(&misc->q_full[g], 0))) scores(g, n);
+      if (!ok) break;
+      if (elect_one()) tc_commit(&misc->k_empty[s]);  // (the scores of this tile have all been issued)
+      __syncwarp();
+      if (!(ok = wait(&misc->v_full[s], (n / L::STAGES) & 1))) break;
+      const uint8_t* const dirty = p.masks.dirty + (int64_t)b * (p.masks.Nkp >> 6) + j * 2;
+      if (dirty[0] | dirty[1]) {
+        clear_rows<DB, 128>(smem + L::V + s * L::TILE, p.masks, b, p.Nk, j * 128, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (!ok || !in(g, j)) continue;
+        if (!(ok = wait(&misc->p_ready[g], count[g] & 1))) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t dv = make_desc_sw128(smem_u32(smem + L::V + s * L::TILE), 16384, 1024);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mma_ts(tmem + 256 + g * 128, tmem + g * 128 + i * 8, mnmaj_step(dv, i), ID_O, i > 0 || count[g] > 0);
+          if (j + 1 == last[g]) tc_commit(&misc->o_done[g]);
+        }
+        __syncwarp();
+        ++count[g];
+        if (j + 1 < last[g]) scores(g, n + 1);  // (behind the product that reads P where S goes: products run in order)
+      }
+      if (!ok) break;
+      if (elect_one()) tc_commit(&misc->v_empty[s]);
+      __syncwarp();
+      ++n;
+    }
+  } else {
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane, i = q0 + g * 128 + row;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + g * 128, to = tl + 256 + g * 128;
+    const bool inside = i < p.masks.Nqp;
+    const int2 keys = inside ? p.masks.range[(int64_t)b * p.masks.Nqp + i] : make_int2(0, 0);
+    const int position = i + (p.masks.cached != nullptr ? p.masks.cached[b] : 0);
+    const ScoreScale sc = score_scale(p, h);
+    float m = -INFINITY, sum = 0.0f;
+    const int tiles = last[g] - first[g];
+#pragma unroll 1
+    for (int n = 0; n < tiles; ++n) {
+      const int key0 = (first[g] + n) * 128;
+      if (!(ok = wait(&misc->s_full[g], n & 1))) break;
+      tc_fence_after_sync();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s[c]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_fence_regs(s[c]);
+      if (CAP || BIAS) {
+        const float d0 = (float)(position - key0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float x = __uint_as_float(s[c][k]);
+            x = CAP ? capped(cap_weight(x, sc), sc) : x * sc.plain;
+            if (BIAS) x = fmaf(-sc.slope, fabsf(d0 - (float)(c * 32 + k)), x);
+            s[c][k] = __float_as_uint(x);
+          }
+      }
+      if (!__all_sync(0xffffffffu, keys.x <= key0 && keys.y >= key0 + 128)) {
+        const int from = keys.x - key0, to_ = keys.y - key0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0xff800000u;  // -inf
+      }
+      float top = -INFINITY;
+      {
+        float t4[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          t4[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+          for (int k = 1; k + 1 < 32; k += 2) t4[c] = fmax3(t4[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+          t4[c] = fmaxf(t4[c], __uint_as_float(s[c][31]));
+        }
+        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+      }
+      const float unit = CAP || BIAS ? 1.0f : sc.plain;
+      top *= unit;
+      const bool grow = top > m + kGrowth || (m == -INFINITY && top > m);
+      if (n == 0) {
+        if (grow) m = top;
+      } else if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? ex2_approx(m - top) : 1.0f;
+        if (grow) m = top;
+        sum *= f;
+#pragma unroll
+        for (int c = 0; c < 2 * DB; ++c) {
+          uint32_t o[32];
+          tmem_read<32>(to + c * 32, o);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          tmem_st32(to + c * 32, o);
+        }
+      }
+      const float frame = m == -INFINITY ? 0.0f : m;
+      const uint64_t unit2 = f2_pack(unit, unit), frame2 = f2_pack(-frame, -frame);
+      uint64_t sum2[2] = {0, 0};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const uint64_t x = f2_pack(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
+          float lo, hi;
+          f2_unpack(CAP || BIAS ? f2_add(x, frame2) : f2_fma(x, unit2, frame2), lo, hi);
+          lo = ex2_approx(lo);
+          hi = ex2_approx(hi);
+          sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(lo, hi));
+          w[k] = pack2<F16>(lo, hi);
+        }
+        tmem_st16(ts + c * 16, w);
+      }
+      float a0, a1, a2, a3;
+      f2_unpack(sum2[0], a0, a1);
+      f2_unpack(sum2[1], a2, a3);
+      sum += (a0 + a1) + (a2 + a3);
+      tmem_wait_st();
+      tc_fence_before_sync();
+      warp_arrive(&misc->p_ready[g], lane);
+    }
+    if (ok && tiles > 0 && !(ok = wait(&misc->o_done[g], 0))) sum = 0.0f;
+    if (ok) {
+      tc_fence_after_sync();
+      const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
+      uint16_t* const y = reinterpret_cast<uint16_t*>(p.y) + (((int64_t)b * p.Nq + i) * p.H + h) * p.D;
+#pragma unroll
+      for (int c = 0; c < 2 * DB; ++c) {
+        uint32_t o[32];
+        if (tiles > 0) {
+          tmem_read<32>(to + c * 32, o);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
+        }
+        if (i < p.Nq) store_columns<F16>(y, c * 32, p.D, o, inv);
+      }
+      // (a query without keys: +inf, so that every weight the backward forms is 0)
+      if (p.lse != nullptr && inside) p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum == 0.0f ? INFINITY : m + __log2f(sum);
+    }
+  }
+  if (!ok) {
+    misc->abort_flag = 1;
+    atomicOr(p.err, 1);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kWarpMma) tmem_dealloc(tmem, 512);
+}
+
+template <bool F16>
+int launch(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream) {
+  constexpr int DB = FLARE_ATTN_DB;
+  CUtensorMap q, k, v;
+  if (!head_map(&q, a.q, a.B, a.Nq, a.H, a.D, a.q_stride_b, a.q_stride_n, a.q_stride_h, 128) ||
+      !head_map(&k, a.k, a.B, a.Nk, a.J, a.D, a.k_stride_b, a.k_stride_n, a.k_stride_h, 128) ||
+      !head_map(&v, a.v, a.B, a.Nk, a.J, a.D, a.v_stride_b, a.v_stride_n, a.v_stride_h, 128))
+    return FLARE_ERR_CUDA;
+  const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
+  auto* const kernel = cap ? (bias ? attention_forward_kernel<DB, F16, true, true> : attention_forward_kernel<DB, F16, true, false>)
+                           : (bias ? attention_forward_kernel<DB, F16, false, true> : attention_forward_kernel<DB, F16, false, false>);
+  FLARE_CUDA_CHECK(allow_smem(kernel));
+  const int64_t blocks = (int64_t)((a.Nq + 255) / 256) * a.B * a.H;
+  if (blocks > 0x7fffffff) return FLARE_ERR_UNSUPPORTED;
+  LaunchTimer timer("attention_forward_kernel", stream);
+  FLARE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)blocks), dim3(kThreads), Layout<DB>::BYTES, stream, q, k, v, p));
+  return FLARE_OK;
+}
+
+}  // namespace
+
+template <int DB>
+int launch_forward_db(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream);
+template <>
+int launch_forward_db<FLARE_ATTN_DB>(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream) {
+  return a.dtype == FLARE_F16 ? launch<true>(a, p, stream) : launch<false>(a, p, stream);
+}
+
+#else
+
+template <int DB>
+int launch_forward_db(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream);
+template <>
+int launch_forward_db<1>(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream);
+template <>
+int launch_forward_db<2>(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream);
+
+int launch_forward_tc(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream) {
+  return a.D <= 64 ? launch_forward_db<1>(a, p, stream) : launch_forward_db<2>(a, p, stream);
+}
+
+#endif
+
+}  // namespace attn
+}  // namespace flare

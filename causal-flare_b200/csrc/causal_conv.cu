@@ -428,7 +428,13 @@ int flare_conv_decode(const flare_conv_args_t* args, flare_stream_t stream) {
 }
 
 size_t flare_mixers_abi_sizeof(int which) {
-  return which == 0 ? sizeof(flare_conv_args_t) : which == 1 ? sizeof(flare_scan_args_t) : 0;
+  switch (which) {
+    case 0: return sizeof(flare_conv_args_t);
+    case 1: return sizeof(flare_scan_args_t);
+    case 2: return sizeof(flare_attention_args_t);
+    case 3: return sizeof(flare_cache_args_t);
+    default: return 0;
+  }
 }
 
 }  // extern "C"

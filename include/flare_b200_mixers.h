@@ -1,6 +1,6 @@
 /*
  * flare_b200_mixers.h - the causal token mixers of libflare_b200.so beside FLARE: the short causal convolution and the
- * selective state space scan, for whole sequences (with gradients), prompts and single tokens.
+ * selective state space scan and softmax attention, for whole sequences (with gradients), prompts and single tokens.
  *
  * Conventions are those of flare_b200.h: device pointers, sizes, an int status; launches on the given stream; no call
  * allocates or synchronises; workspaces come from the caller (sizes from *_workspace_bytes, 256-byte aligned).
@@ -104,7 +104,81 @@ int flare_scan_backward(const flare_scan_args_t* args, flare_stream_t stream);
  * read and updated in place; state_in is ignored. */
 int flare_scan_decode(const flare_scan_args_t* args, flare_stream_t stream);
 
-/* sizeof(flare_conv_args_t / flare_scan_args_t) for which = 0 / 1 (other values: 0) */
+/*
+ * Causal attention of H query heads over J key / value heads (H a multiple of J, head h reads h / (H / J)) of width D (a
+ * multiple of 8, at most 128), bf16 or fp16.  The score of the query at position i for the key at position j is
+ *   cap tanh(scale <q, k> / cap) - slopes[h] |i - j|          (cap = 0: scale <q, k>; slopes NULL: no bias)
+ * and token i sees the keys j <= i of its document, with `window` > 0 only j > i - window; where `prefix` [B, N] (bytes,
+ * non-zero: true) holds for the first tokens of a document, all tokens of the document see those.  Without a key in
+ * sight y and all gradients are 0.
+ *
+ * Whole sequences (cached = NULL): Nk = Nq.  Prompts behind a cache (`cached` [B] int32: tokens that it holds): k and v are the
+ * caches [B, Nk, J, D] with the new tokens in place (flare_attention_append), the Nq queries of row b lie at positions
+ * cached[b] + i; lengths [B] (or NULL) as above; documents exclude `cached`, and there is no backward.
+ */
+typedef struct flare_attention_args {
+  const void* q;            /* [B, Nq, H, D] */
+  const void* k;            /* [B, Nk, J, D] */
+  const void* v;            /* [B, Nk, J, D] */
+  void* y;                  /* [B, Nq, H, D] contiguous */
+  float* lse;               /* [B, H, Nq rounded up to 128]: log2 of the softmax denominators, for the backward; may be NULL */
+  const int32_t* documents; /* [B, Nq] contiguous or NULL */
+  const uint8_t* prefix;    /* [B, Nq] contiguous or NULL */
+  const int32_t* cached;    /* [B] or NULL */
+  const int32_t* lengths;   /* [B] or NULL */
+  const float* slopes;      /* [H] or NULL */
+  const void* dy;           /* backward: [B, Nq, H, D] */
+  void* dq;                 /* [B, Nq, H, D] contiguous */
+  void* dk;                 /* [B, Nk, J, D] contiguous, like dv */
+  void* dv;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t B, Nq, Nk, H, J, D;
+  int64_t q_stride_b, q_stride_n, q_stride_h, k_stride_b, k_stride_n, k_stride_h, v_stride_b, v_stride_n, v_stride_h;
+  int64_t dy_stride_b, dy_stride_n, dy_stride_h; /* all strides multiples of 8 elements and positive, pointers 16-byte aligned */
+  float scale, cap;
+  int32_t window; /* 0: none */
+  int32_t dtype;
+} flare_attention_args_t;
+
+size_t flare_attention_forward_workspace_bytes(const flare_attention_args_t* args);
+int flare_attention_forward(const flare_attention_args_t* args, flare_stream_t stream);
+/* y and lse as the forward of the same problem left them */
+size_t flare_attention_backward_workspace_bytes(const flare_attention_args_t* args);
+int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t stream);
+
+/*
+ * Caches: k_cache, v_cache [B, L, J, D] (contiguous rows of D, strides in elements), written in place.
+ * append: new_k[b, t] goes to position cached[b] + t for t < lengths[b] (NULL: N); positions outside [0, L) are left out.
+ * decode: one token per row, q, y [B, H, D], new_k, new_v [B, J, D].  The row's keys are the first cached[b] of its cache and the
+ * new one, which is written to position cached[b].  A row whose position lies outside [0, L) is idle: y = 0, nothing is written.
+ */
+typedef struct flare_cache_args {
+  const void* q;
+  const void* new_k;
+  const void* new_v;
+  void* k_cache;
+  void* v_cache;
+  void* y;                /* [B, H, D] contiguous */
+  const int32_t* cached;  /* [B]; append: NULL: 0 */
+  const int32_t* lengths; /* [B] or NULL; append only */
+  const float* slopes;    /* [H] or NULL */
+  void* workspace;        /* decode */
+  size_t workspace_bytes;
+  int32_t B, N, H, J, D, L;
+  int64_t q_stride_b, q_stride_h;
+  int64_t new_k_stride_b, new_k_stride_n, new_k_stride_h, new_v_stride_b, new_v_stride_n, new_v_stride_h;
+  int64_t k_stride_b, k_stride_n, k_stride_h, v_stride_b, v_stride_n, v_stride_h; /* of the caches; multiples of 8, like the others */
+  float scale, cap;
+  int32_t window;
+  int32_t dtype;
+} flare_cache_args_t;
+
+int flare_attention_append(const flare_cache_args_t* args, flare_stream_t stream);
+size_t flare_attention_decode_workspace_bytes(const flare_cache_args_t* args);
+int flare_attention_decode(const flare_cache_args_t* args, flare_stream_t stream);
+
+/* sizeof(flare_conv_args_t / flare_scan_args_t / flare_attention_args_t / flare_cache_args_t) for which = 0..3 (other values: 0) */
 size_t flare_mixers_abi_sizeof(int which);
 
 #ifdef __cplusplus

@@ -69,3 +69,68 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, sof
             y = y * z[:, t] * torch.sigmoid(z[:, t])
         ys.append(torch.where(on[:, t, None], y, torch.zeros_like(y)))
     return torch.stack(ys, 1), h
+
+
+def in_sight(N, documents=None, prefix=None, window=None):
+    """[B, N, N] truth values: does token i see token j?  B is 1 without documents and prefix."""
+    B = 1 if documents is None and prefix is None else (documents if documents is not None else prefix).shape[0]
+    device = next((t.device for t in (documents, prefix) if t is not None), "cpu")
+    see = torch.zeros(B, N, N, dtype=torch.bool)
+    run = torch.zeros(B, N, dtype=torch.long) if documents is None else runs(documents)[0].cpu()
+    on = torch.ones(B, N, dtype=torch.bool) if documents is None else (documents >= 0).cpu()
+    led = torch.zeros(B, N, dtype=torch.bool)
+    for b in range(B):
+        for j in range(N if prefix is not None else 0):
+            led[b, j] = prefix[b, j] and (j == 0 or run[b, j] != run[b, j - 1] or led[b, j - 1])
+    i, j = torch.arange(N)[:, None], torch.arange(N)[None]
+    for b in range(B):
+        see[b] = ((j <= i) | led[b][None]) & (run[b][:, None] == run[b][None]) & on[b][:, None] & on[b][None]
+        if window is not None:
+            see[b] &= j > i - window
+    return see.to(device)
+
+
+class Attention:
+    """Softmax attention of q [B, N, H, D] over k, v [B, M, J, D] where ``see`` [B or 1, N, M] holds; positions of the queries: first
+    [B] + 0..N-1.  With ``dy`` the gradients, in closed form.  ``eps``: half a step of the type that weights and outputs are rounded to; the
+    ``*_off`` are then bounds on how far a kernel that rounds P, dS and its outputs once, and computes in fp32 otherwise, may be off.  A
+    value below the type's normal numbers is off by up to half its smallest step, ``tiny``, instead (2^-25 in fp16, where a weight dS
+    of 2^-20 keeps four bits: the sum dk = scale sum dS q of n such terms may then be off by scale n 2^-25 |q|)."""
+
+    def __init__(self, q, k, v, see, scale, cap=None, slopes=None, first=None, dy=None, eps=0.0):
+        tiny = 2.0 ** -25 if eps == 2.0 ** -11 else 0.0
+        B, N, H, D = q.shape
+        M, J = k.shape[1], k.shape[2]
+        qh = q.transpose(1, 2)
+        kh, vh = (t.transpose(1, 2).repeat_interleave(H // J, 1) for t in (k, v))
+        s = scale * qh @ kh.transpose(2, 3)
+        t = torch.zeros_like(s)
+        if cap is not None:
+            t = torch.tanh(s / cap)
+            s = cap * t
+        if slopes is not None:
+            at = torch.arange(N, device=q.device)[None] + (0 if first is None else first[:, None])
+            s = s - slopes[None, :, None, None] * (at[..., None] - torch.arange(M, device=q.device)).abs()[:, None]
+        see = see[:, None].expand(B, H, N, M)
+        some = see.any(-1, keepdim=True)
+        p = torch.softmax(torch.where(some, s.masked_fill(~see, -torch.inf), torch.zeros_like(s)), -1) * some
+        y = p @ vh
+        # fp32: scores and exponents, a few units of 2^-22 of the largest score in sight
+        f = 2.0 ** -21 * (1 + (s.abs() * see).amax((-1, -2), keepdim=True))
+        rounded = lambda x: torch.maximum(eps * x.abs(), torch.full_like(x, tiny)) * see  # noqa: E731
+        y_off = (rounded(p) + f * p) @ vh.abs() + eps * y.abs()
+        back = lambda x: x.transpose(1, 2)  # noqa: E731
+        fold = lambda x: back(x).reshape(B, M, J, H // J, D).sum(3)  # noqa: E731
+        self.y, self.y_off = back(y), back(y_off)
+        if dy is None:
+            return
+        g = dy.transpose(1, 2)
+        dp = g @ vh.transpose(2, 3)
+        slope = 1 - t * t
+        raw = p * (dp - (g * y).sum(-1, keepdim=True)) * some
+        ds = raw * slope
+        ds_off = rounded(ds) + (ds.abs() + raw.abs()) * f + p * ((g.abs() * y_off).sum(-1, keepdim=True) + f * (g.abs() @ vh.abs().transpose(2, 3)))
+        self.dq, self.dk, self.dv = back(scale * ds @ kh), fold(scale * ds.transpose(2, 3) @ qh), fold(p.transpose(2, 3) @ g)
+        self.dq_off = back(scale * ds_off @ kh.abs()) + eps * self.dq.abs()
+        self.dk_off = fold(scale * ds_off.transpose(2, 3) @ qh.abs()) + eps * self.dk.abs()
+        self.dv_off = fold((rounded(p) + f * p).transpose(2, 3) @ g.abs()) + eps * self.dv.abs()
