@@ -310,17 +310,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool F16>
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-  if constexpr (F16) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 // One token.  Bound by memory: every key and value in sight is read once, by one block for up to 16 query heads that share
 // them.  A warp takes 16 keys at a time, straight from memory into the operands of m16n8k16 products: heads are the rows, so the
 // scores come out as the A operand that the product with V takes.  A thread's 16-byte piece of a key covers the contraction in an
@@ -328,6 +317,7 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
 // for the SMs, whose sums a second kernel joins; the warps of a block join theirs in shared memory.
 template <int DB, bool F16>
 __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeParams p) {
+  using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
   pdl_begin();
   const flare_cache_args_t& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
@@ -438,8 +428,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
         s[n][e] = exp2f(s[n][e] - frame[e >> 1]);
         sum[e >> 1] += s[n][e];
       }
-    const uint32_t w[4] = {pack_pair<F16>(s[0][0], s[0][1]), pack_pair<F16>(s[0][2], s[0][3]), pack_pair<F16>(s[1][0], s[1][1]),
-                           pack_pair<F16>(s[1][2], s[1][3])};
+    const uint32_t w[4] = {pack_pair<T>(s[0][0], s[0][1]), pack_pair<T>(s[0][2], s[0][3]), pack_pair<T>(s[1][0], s[1][1]),
+                           pack_pair<T>(s[1][2], s[1][3])};
 #pragma unroll
     for (int g = 0; g < DB; ++g) {
       const uint32_t v0[4] = {vr[0][g].x, vr[0][g].y, vr[0][g].z, vr[0][g].w}, v1[4] = {vr[1][g].x, vr[1][g].y, vr[1][g].z, vr[1][g].w};

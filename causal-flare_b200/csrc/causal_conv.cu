@@ -11,6 +11,7 @@ namespace flare {
 namespace {
 
 using namespace mixer;
+using namespace sm100;
 
 constexpr int kWarps = 4;
 
@@ -25,23 +26,22 @@ struct ConvParams {
 __device__ __forceinline__ float weight_at(const flare_conv_args_t& a, int64_t i) { return load1(a.weight, a.weight_dtype, i); }
 
 // What a walk carries from token to token: the ids in front of it and how many of them belong to its document.
-template <int W>
+template <int W, bool DOCS>
 struct Reach {
-  const int32_t* ids;  // of the row, or null
+  const int32_t* ids;  // of the row
   int last, reach;
   __device__ __forceinline__ void start(const int32_t* row, int t) {
     ids = row;
-    reach = W - 1;
-    last = 0;
-    if (ids == nullptr) return;
     reach = 0;
+    last = -1;
+    if (!DOCS) return;
     last = t > 0 ? ids[t - 1] : -1;
     for (int j = 2; j < W && t - j >= 0 && ids[t - j] == last; ++j) ++reach;
   }
   // the number of tokens in front of t that its taps may see; the id of t in `id`
   __device__ __forceinline__ int step(int t, int& id) {
     id = 0;
-    if (ids == nullptr) return W - 1;
+    if (!DOCS) return W - 1;
     id = ids[t];
     reach = t > 0 && id == last ? min(reach + 1, W - 1) : 0;
     last = id;
@@ -49,13 +49,39 @@ struct Reach {
   }
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void load_weights(const flare_conv_args_t& a, int c, int count, float (&w)[W][8], float (&bias)[8]) {
+// eight channels as four pairs: the packed operations halve what is issued
+struct Pairs {
+  uint64_t v[4];
+};
+__device__ __forceinline__ Pairs zero_pairs() { return Pairs{{0, 0, 0, 0}}; }
+template <typename T>
+__device__ __forceinline__ Pairs to_pairs(const Raw8<T>& r) {
+  float f[8];
+  unpack8(r, f);
+  Pairs p;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) p.v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+  return p;
+}
+__device__ __forceinline__ void from_pairs(const Pairs& p, float (&f)[8]) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = i < count ? weight_at(a, (int64_t)(c + i) * W + j) : 0.0f;
-    bias[i] = i < count && a.bias != nullptr ? load1(a.bias, a.weight_dtype, c + i) : 0.0f;
+  for (int i = 0; i < 4; ++i) f2_unpack(p.v[i], f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ void fma_pairs(const Pairs& a, const Pairs& b, Pairs& c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c.v[i] = f2_fma(a.v[i], b.v[i], c.v[i]);
+}
+
+template <int W>
+__device__ __forceinline__ void load_weights(const flare_conv_args_t& a, int c, int count, Pairs (&w)[W], Pairs& bias) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      w[j].v[i] = f2_pack(2 * i < count ? weight_at(a, (int64_t)(c + 2 * i) * W + j) : 0.0f,
+                          2 * i + 1 < count ? weight_at(a, (int64_t)(c + 2 * i + 1) * W + j) : 0.0f);
+    bias.v[i] = f2_pack(2 * i < count && a.bias != nullptr ? load1(a.bias, a.weight_dtype, c + 2 * i) : 0.0f,
+                        2 * i + 1 < count && a.bias != nullptr ? load1(a.bias, a.weight_dtype, c + 2 * i + 1) : 0.0f);
   }
 }
 
@@ -66,28 +92,26 @@ __device__ __forceinline__ Raw8<T> row_at(const flare_conv_args_t& a, const T* x
   return load_raw8<T>(state + (int64_t)(W - 1 + t) * a.C, state != nullptr && t >= 1 - W ? count : 0, wide);
 }
 
-// x is summed newest tap last, bias first: v = bias + w[0] x[t-W+1] + ... + w[W-1] x[t]
+// x is summed newest tap first, bias in front: v = bias + w[W-1] x[t] + ... + w[0] x[t-W+1]; past[j]: token t - j
 template <int W>
-__device__ __forceinline__ void taps(const float (&w)[W][8], const float (&bias)[8], const float (&past)[W][8], int reach, float (&v)[8]) {
+__device__ __forceinline__ Pairs taps(const Pairs (&w)[W], const Pairs& bias, const Pairs (&past)[W], int reach) {
+  Pairs v = bias;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = bias[i];
-#pragma unroll
-  for (int j = W - 1; j >= 0; --j)
-    if (j <= reach) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf(w[W - 1 - j][i], past[j][i], v[i]);
-    }
+  for (int j = 0; j < W; ++j)
+    if (j <= reach) fma_pairs(w[W - 1 - j], past[j], v);
+  return v;
 }
 
-template <typename T, int W>
+// (WIDE: every thread has eight channels and 16-byte pieces)
+template <typename T, int W, bool DOCS, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps) conv_forward_kernel(const ConvParams p) {
   pdl_begin();
   const flare_conv_args_t& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.blocks_n, nb = blockIdx.x % p.blocks_n;
-  const int c = (blockIdx.y * 32 + lane) * 8, count = min(8, a.C - c);
-  if (count <= 0) return;
-  const bool wide = p.wide != 0;
+  const int c = (blockIdx.y * 32 + lane) * 8;
+  if (c >= a.C) return;
+  const int count = WIDE ? 8 : min(8, a.C - c);
   const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)b * a.x_stride_b + c;
   const T* state = a.state_in != nullptr ? reinterpret_cast<const T*>(a.state_in) + (int64_t)b * (W - 1) * a.C + c : nullptr;
   T* y = reinterpret_cast<T*>(a.y) + (int64_t)b * a.N * a.C + c;
@@ -97,42 +121,45 @@ __global__ void __launch_bounds__(32 * kWarps) conv_forward_kernel(const ConvPar
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
       float v[8];
-      unpack8(row_at<T, W>(a, x, state, len - (W - 1) + j, len, count, wide), v);
-      store8<T>(out + (int64_t)j * a.C, v, count, wide);
+      unpack8(row_at<T, W>(a, x, state, len - (W - 1) + j, len, count, WIDE), v);
+      store8<T>(out + (int64_t)j * a.C, v, count, WIDE);
     }
   }
   const int t0 = (nb * kWarps + warp) * p.run, t1 = min(a.N, t0 + p.run);
   if (t0 >= t1) return;
-  float w[W][8], bias[8], past[W][8];
-  load_weights<T, W>(a, c, count, w, bias);
-  Reach<W> docs;
-  docs.start(a.documents != nullptr ? a.documents + (int64_t)b * a.N : nullptr, t0);
-#pragma unroll
-  for (int j = 1; j < W; ++j) unpack8(row_at<T, W>(a, x, state, t0 - j, a.N, count, wide), past[j - 1]);
   constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
-  for (int t = t0; t < t1; t += kAhead) {
-    Raw8<T> rows[kAhead];
+  Raw8<T> rows[kAhead];
+  const auto fetch = [&](int t) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) rows[k] = load_raw8<T>(x + (int64_t)(t + k) * a.x_stride_n, t + k < t1 ? count : 0, wide);
+    for (int k = 0; k < kAhead; ++k) rows[k] = load_raw8<T>(x + (int64_t)(t + k) * a.x_stride_n, t + k < t1 ? count : 0, WIDE);
+  };
+  fetch(t0);
+  Pairs w[W], bias, past[W];
+  load_weights<W>(a, c, count, w, bias);
+  Reach<W, DOCS> docs;
+  docs.start(DOCS ? a.documents + (int64_t)b * a.N : nullptr, t0);
+#pragma unroll
+  for (int j = 1; j < W; ++j) past[j - 1] = to_pairs(row_at<T, W>(a, x, state, t0 - j, a.N, count, WIDE));
+  for (int t = t0; t < t1; t += kAhead) {
+    if (t > t0) fetch(t);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (t + k >= t1) break;
 #pragma unroll
-      for (int j = W - 1; j > 0; --j)
+      for (int j = W - 1; j > 0; --j) past[j] = past[j - 1];
+      past[0] = to_pairs(rows[k]);
+      if (t + k < t1) {
+        int id;
+        const int reach = docs.step(t + k, id);
+        float v[8];
+        from_pairs(taps<W>(w, bias, past, reach), v);
+        const bool on = (!DOCS || id >= 0) && t + k < len;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) past[j][i] = past[j - 1][i];
-      unpack8(rows[k], past[0]);
-      int id;
-      const int reach = docs.step(t + k, id);
-      float v[8];
-      taps<W>(w, bias, past, reach, v);
-      const bool on = id >= 0 && t + k < len;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (a.activation == FLARE_SILU) v[i] *= sigmoid(v[i]);
-        if (!on) v[i] = 0.0f;
+        for (int i = 0; i < 8; ++i) {
+          if (a.activation == FLARE_SILU) v[i] *= sigmoid(v[i]);
+          if (!on) v[i] = 0.0f;
+        }
+        store8<T>(y + (int64_t)(t + k) * a.C, v, count, WIDE);
       }
-      store8<T>(y + (int64_t)(t + k) * a.C, v, count, wide);
     }
   }
 }
@@ -140,33 +167,29 @@ __global__ void __launch_bounds__(32 * kWarps) conv_forward_kernel(const ConvPar
 // g[t] = dy[t] act'(pre[t]); dx[t] = sum_j w[W-1-j] g[t+j]; dw[W-1-j] = sum_t g[t] x[t-j]; dbias = sum g.
 // A run computes the g of the W - 1 tokens behind it as well (their rows are read twice), and adds only its own tokens' to
 // the weights' gradients: one partial sum per block, added up in order afterwards.
-template <typename T, int W>
+template <typename T, int W, bool DOCS, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps) conv_backward_kernel(const ConvParams p) {
   pdl_begin();
   const flare_conv_args_t& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.blocks_n, nb = blockIdx.x % p.blocks_n;
-  const int c = (blockIdx.y * 32 + lane) * 8, count = max(0, min(8, a.C - c));
-  const bool wide = p.wide != 0;
+  const int c = (blockIdx.y * 32 + lane) * 8, count = c >= a.C ? 0 : WIDE ? 8 : min(8, a.C - c);
   const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)b * a.x_stride_b + c;
   const T* dy = reinterpret_cast<const T*>(a.dy) + (int64_t)b * a.dy_stride_b + c;
   T* dx = reinterpret_cast<T*>(a.dx) + (int64_t)b * a.N * a.C + c;
   const int t0 = (nb * kWarps + warp) * p.run, t1 = min(a.N, t0 + p.run), t2 = min(a.N, t1 + W - 1);
-  float dw[W + 1][8];  // (the last row: bias)
+  Pairs dw[W + 1];  // (the last one: bias)
 #pragma unroll
-  for (int j = 0; j <= W; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
+  for (int j = 0; j <= W; ++j) dw[j] = zero_pairs();
   if (t0 < t1 && count > 0) {
-    float w[W][8], bias[8], past[W][8], acc[W][8];  // acc[j]: gradient of token t - j, as far as it is known
-    load_weights<T, W>(a, c, count, w, bias);
-    Reach<W> docs;
-    docs.start(a.documents != nullptr ? a.documents + (int64_t)b * a.N : nullptr, t0);
+    Pairs w[W], bias, past[W], acc[W];  // acc[j]: gradient of token t - j, as far as it is known
+    load_weights<W>(a, c, count, w, bias);
+    Reach<W, DOCS> docs;
+    docs.start(DOCS ? a.documents + (int64_t)b * a.N : nullptr, t0);
 #pragma unroll
     for (int j = 1; j < W; ++j) {
-      unpack8(row_at<T, W>(a, x, nullptr, t0 - j, a.N, count, wide), past[j - 1]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[j - 1][i] = 0.0f;
+      past[j - 1] = to_pairs(row_at<T, W>(a, x, nullptr, t0 - j, a.N, count, WIDE));
+      acc[j - 1] = zero_pairs();
     }
     constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
     const int end = t1 + W - 1;  // the last run's gradients leave W - 1 steps behind its last token
@@ -175,55 +198,51 @@ __global__ void __launch_bounds__(32 * kWarps) conv_backward_kernel(const ConvPa
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int n = t + k < t2 ? count : 0;
-        rows[k] = load_raw8<T>(x + (int64_t)(t + k) * a.x_stride_n, n, wide);
-        drows[k] = load_raw8<T>(dy + (int64_t)(t + k) * a.dy_stride_n, n, wide);
+        rows[k] = load_raw8<T>(x + (int64_t)(t + k) * a.x_stride_n, n, WIDE);
+        drows[k] = load_raw8<T>(dy + (int64_t)(t + k) * a.dy_stride_n, n, WIDE);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (t + k >= end) break;
 #pragma unroll
-        for (int j = W - 1; j > 0; --j)
+        for (int j = W - 1; j > 0; --j) {
+          past[j] = past[j - 1];
+          acc[j] = acc[j - 1];
+        }
+        past[0] = to_pairs(rows[k]);
+        acc[0] = zero_pairs();
+        int id = -1, reach = 0;
+        if (t + k < t2) reach = docs.step(t + k, id);
+        if (id >= 0) {
+          Pairs g = to_pairs(drows[k]);
+          if (a.activation == FLARE_SILU) {
+            float v[8], d[8];
+            from_pairs(taps<W>(w, bias, past, reach), v);
+            from_pairs(g, d);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            past[j][i] = past[j - 1][i];
-            acc[j][i] = acc[j - 1][i];
-          }
-        unpack8(rows[k], past[0]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[0][i] = 0.0f;
-        if (t + k < t2) {
-          int id;
-          const int reach = docs.step(t + k, id);
-          if (id >= 0) {
-            float g[8];
-            unpack8(drows[k], g);
-            if (a.activation == FLARE_SILU) {
-              float v[8];
-              taps<W>(w, bias, past, reach, v);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float r = sigmoid(v[i]);
-                g[i] *= r * fmaf(v[i], 1.0f - r, 1.0f);
-              }
+            for (int i = 0; i < 8; ++i) {
+              const float r = sigmoid(v[i]);
+              d[i] *= r * fmaf(v[i], 1.0f - r, 1.0f);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) g.v[i] = f2_pack(d[2 * i], d[2 * i + 1]);
+          }
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            if (j <= reach) fma_pairs(w[W - 1 - j], g, acc[j]);
+          if (t + k < t1) {
 #pragma unroll
             for (int j = 0; j < W; ++j)
-              if (j <= reach) {
+              if (j <= reach) fma_pairs(g, past[j], dw[W - 1 - j]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[j][i] = fmaf(w[W - 1 - j][i], g[i], acc[j][i]);
-                if (t + k < t1) {
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) dw[W - 1 - j][i] = fmaf(g[i], past[j][i], dw[W - 1 - j][i]);
-                }
-              }
-            if (t + k < t1) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) dw[W][i] += g[i];
-            }
+            for (int i = 0; i < 4; ++i) dw[W].v[i] = f2_add(dw[W].v[i], g.v[i]);
           }
         }
         const int done = t + k - (W - 1);
-        if (done >= t0 && done < t1) store8<T>(dx + (int64_t)done * a.C, acc[W - 1], count, wide);
+        if (done >= t0 && done < t1) {
+          float v[8];
+          from_pairs(acc[W - 1], v);
+          store8<T>(dx + (int64_t)done * a.C, v, count, WIDE);
+        }
       }
     }
   }
@@ -231,24 +250,28 @@ __global__ void __launch_bounds__(32 * kWarps) conv_backward_kernel(const ConvPa
   __shared__ float sums[kWarps - 1][32][8 * (W + 1) + 1];
   if (warp > 0) {
 #pragma unroll
-    for (int j = 0; j <= W; ++j)
+    for (int j = 0; j <= W; ++j) {
+      float v[8];
+      from_pairs(dw[j], v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sums[warp - 1][lane][j * 8 + i] = dw[j][i];
+      for (int i = 0; i < 8; ++i) sums[warp - 1][lane][j * 8 + i] = v[i];
+    }
   }
   __syncthreads();
   if (warp > 0) return;
   float* out = p.partial + (int64_t)blockIdx.x * a.C * (W + 1);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < count) {
+  for (int j = 0; j <= W; ++j) {
+    float v[8];
+    from_pairs(dw[j], v);
 #pragma unroll
-      for (int j = 0; j <= W; ++j) {
-        float v = dw[j][i];
+    for (int i = 0; i < 8; ++i)
+      if (i < count) {
 #pragma unroll
-        for (int q = 0; q < kWarps - 1; ++q) v += sums[q][lane][j * 8 + i];
-        out[j < W ? (int64_t)(c + i) * W + j : (int64_t)a.C * W + c + i] = v;
+        for (int q = 0; q < kWarps - 1; ++q) v[i] += sums[q][lane][j * 8 + i];
+        out[j < W ? (int64_t)(c + i) * W + j : (int64_t)a.C * W + c + i] = v[i];
       }
-    }
+  }
 }
 
 // One token: the state's rows move up by one, the token's is the last.
@@ -267,17 +290,21 @@ __global__ void __launch_bounds__(128) conv_decode_kernel(const ConvParams p) {
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) rows[j] = load_raw8<T>(state + (int64_t)j * a.C, count, wide);
   rows[W - 1] = load_raw8<T>(reinterpret_cast<const T*>(a.x) + b * a.x_stride_b + c, count, wide);
-  float w[W][8], bias[8], past[W][8], v[8];
-  load_weights<T, W>(a, c, count, w, bias);
+  Pairs w[W], bias, past[W];
+  float v[8];
+  load_weights<W>(a, c, count, w, bias);
 #pragma unroll
-  for (int j = 0; j < W; ++j) unpack8(rows[W - 1 - j], past[j]);
-  taps<W>(w, bias, past, W - 1, v);
+  for (int j = 0; j < W; ++j) past[j] = to_pairs(rows[W - 1 - j]);
+  from_pairs(taps<W>(w, bias, past, W - 1), v);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (a.activation == FLARE_SILU) v[i] *= sigmoid(v[i]);
   store8<T>(reinterpret_cast<T*>(a.y) + b * a.C + c, v, count, wide);
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) store8<T>(state + (int64_t)j * a.C, past[W - 2 - j], count, wide);
+  for (int j = 0; j < W - 1; ++j) {
+    from_pairs(past[W - 2 - j], v);
+    store8<T>(state + (int64_t)j * a.C, v, count, wide);
+  }
 }
 
 // Runs of 64 tokens where that leaves eight warps for every SM, of 8 where it does not: the W - 1 rows read again weigh less than idle SMs.
@@ -371,7 +398,11 @@ int flare_conv_forward(const flare_conv_args_t* args, flare_stream_t stream) {
   const dim3 grid((unsigned)(a.B * (int64_t)p.blocks_n), (unsigned)((a.C + 255) / 256));
   return by_type(a.dtype, a.W, [&](auto t, auto w) -> int {
     LaunchTimer timer("conv_forward_kernel", stream);
-    FLARE_CUDA_CHECK(launch_pdl(conv_forward_kernel<decltype(t), decltype(w)::value>, grid, dim3(32 * kWarps), 0, stream, p));
+    using T = decltype(t);
+    constexpr int W = decltype(w)::value;
+    auto* const kernel = a.documents != nullptr ? (p.wide ? conv_forward_kernel<T, W, true, true> : conv_forward_kernel<T, W, true, false>)
+                                                : (p.wide ? conv_forward_kernel<T, W, false, true> : conv_forward_kernel<T, W, false, false>);
+    FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(32 * kWarps), 0, stream, p));
     return FLARE_OK;
   });
 }
@@ -398,7 +429,11 @@ int flare_conv_backward(const flare_conv_args_t* args, flare_stream_t stream) {
   const dim3 grid((unsigned)parts, (unsigned)((a.C + 255) / 256));
   const int rc = by_type(a.dtype, a.W, [&](auto t, auto w) -> int {
     LaunchTimer timer("conv_backward_kernel", stream);
-    FLARE_CUDA_CHECK(launch_pdl(conv_backward_kernel<decltype(t), decltype(w)::value>, grid, dim3(32 * kWarps), 0, stream, p));
+    using T = decltype(t);
+    constexpr int W = decltype(w)::value;
+    auto* const kernel = a.documents != nullptr ? (p.wide ? conv_backward_kernel<T, W, true, true> : conv_backward_kernel<T, W, true, false>)
+                                                : (p.wide ? conv_backward_kernel<T, W, false, true> : conv_backward_kernel<T, W, false, false>);
+    FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(32 * kWarps), 0, stream, p));
     return FLARE_OK;
   });
   if (rc) return rc;

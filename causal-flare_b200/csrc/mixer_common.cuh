@@ -4,6 +4,9 @@
 
 #include "../../include/flare_b200_mixers.h"
 #include "flare_common.cuh"
+#include "sm100_ptx.cuh"
+
+#include <type_traits>
 
 namespace flare {
 namespace mixer {
@@ -25,38 +28,83 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  return std::is_same<T, __half>::value ? sm100::pack_f16(lo, hi) : sm100::pack_bf16(lo, hi);
+}
+
 // Eight elements as they lie in memory, so that loads can be in flight while the eight before are worked on.
 template <typename T>
-struct alignas(16) Raw8 {
-  T v[8];
+struct Raw8 {
+  static constexpr int WORDS = sizeof(T) * 8 / 4;
+  uint32_t w[WORDS];
 };
+
+__device__ __forceinline__ uint32_t word_of(__nv_bfloat16 lo, __nv_bfloat16 hi) {
+  return (uint32_t)__bfloat16_as_ushort(lo) | (uint32_t)__bfloat16_as_ushort(hi) << 16;
+}
+__device__ __forceinline__ uint32_t word_of(__half lo, __half hi) {
+  return (uint32_t)__half_as_ushort(lo) | (uint32_t)__half_as_ushort(hi) << 16;
+}
 
 // `count` elements (the rest 0) from p; `wide`: p is 16-byte aligned and all eight lie inside the tensor.
 template <typename T>
 __device__ __forceinline__ Raw8<T> load_raw8(const T* p, int count, bool wide) {
   Raw8<T> r;
-  if (wide && count >= 8) {
+  if (wide) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) reinterpret_cast<uint4*>(r.v)[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < Raw8<T>::WORDS / 4; ++i) {
+      const uint4 v = count >= 8 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+      r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+    }
   } else {
+    const T zero = from_float<T>(0.0f);
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = i < count ? p[i] : from_float<T>(0.0f);
+      for (int i = 0; i < 8; ++i) r.w[i] = __float_as_uint(i < count ? (float)p[i] : 0.0f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = word_of(2 * i < count ? p[2 * i] : zero, 2 * i + 1 < count ? p[2 * i + 1] : zero);
+    }
   }
   return r;
 }
 template <typename T>
 __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&out)[8]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) out[i] = to_float<T>(r.v[i]);
+    for (int i = 0; i < 8; ++i) out[i] = __uint_as_float(r.w[i]);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[2 * i] = __uint_as_float(r.w[i] << 16);
+      out[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+      out[2 * i] = f.x;
+      out[2 * i + 1] = f.y;
+    }
+  }
 }
+// `wide`: all eight go out in 16-byte pieces (or, with count < 8, nothing does)
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8], int count, bool wide) {
-  if (wide && count >= 8) {
-    Raw8<T> r;
+  if (wide) {
+    if (count < 8) return;
+    uint32_t w[Raw8<T>::WORDS];
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = from_float<T>(x[i]);
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(x[i]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(r.v)[i];
+      for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(x[2 * i], x[2 * i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::WORDS / 4; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
