@@ -33,12 +33,14 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return std::is_same<T, __half>::value ? sm100::pack_f16(lo, hi) : sm100::pack_bf16(lo, hi);
 }
 
-// Eight elements as they lie in memory, so that loads can be in flight while the eight before are worked on.
-template <typename T>
-struct Raw8 {
-  static constexpr int WORDS = sizeof(T) * 8 / 4;
+// V elements (8 unless said otherwise) as they lie in memory, so that loads can be in flight while others are worked on.
+template <typename T, int V = 8>
+struct Raw {
+  static constexpr int WORDS = sizeof(T) * V / 4;
   uint32_t w[WORDS];
 };
+template <typename T>
+using Raw8 = Raw<T, 8>;
 
 __device__ __forceinline__ uint32_t word_of(__nv_bfloat16 lo, __nv_bfloat16 hi) {
   return (uint32_t)__bfloat16_as_ushort(lo) | (uint32_t)__bfloat16_as_ushort(hi) << 16;
@@ -47,70 +49,87 @@ __device__ __forceinline__ uint32_t word_of(__half lo, __half hi) {
   return (uint32_t)__half_as_ushort(lo) | (uint32_t)__half_as_ushort(hi) << 16;
 }
 
-// `count` elements (the rest 0) from p; `wide`: p is 16-byte aligned and all eight lie inside the tensor.
-template <typename T>
-__device__ __forceinline__ Raw8<T> load_raw8(const T* p, int count, bool wide) {
-  Raw8<T> r;
+// `count` elements (the rest 0) from p; `wide`: p is aligned to 16 bytes (or to the V elements, if those are fewer), and `count` is V or 0.
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p, int count, bool wide) {
+  Raw<T, V> r;
   if (wide) {
+    if constexpr (Raw<T, V>::WORDS == 2) {
+      const uint2 v = count >= V ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+      r.w[0] = v.x; r.w[1] = v.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < Raw8<T>::WORDS / 4; ++i) {
-      const uint4 v = count >= 8 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
-      r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+      for (int i = 0; i < Raw<T, V>::WORDS / 4; ++i) {
+        const uint4 v = count >= V ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+        r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+      }
     }
   } else {
     const T zero = from_float<T>(0.0f);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.w[i] = __float_as_uint(i < count ? (float)p[i] : 0.0f);
+      for (int i = 0; i < V; ++i) r.w[i] = __float_as_uint(i < count ? (float)p[i] : 0.0f);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r.w[i] = word_of(2 * i < count ? p[2 * i] : zero, 2 * i + 1 < count ? p[2 * i + 1] : zero);
+      for (int i = 0; i < V / 2; ++i) r.w[i] = word_of(2 * i < count ? p[2 * i] : zero, 2 * i + 1 < count ? p[2 * i + 1] : zero);
     }
   }
   return r;
 }
 template <typename T>
-__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&out)[8]) {
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p, int count, bool wide) { return load_raw<T, 8>(p, count, wide); }
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&out)[V]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = __uint_as_float(r.w[i]);
+    for (int i = 0; i < V; ++i) out[i] = __uint_as_float(r.w[i]);
   } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V / 2; ++i) {
       out[2 * i] = __uint_as_float(r.w[i] << 16);
       out[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V / 2; ++i) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
       out[2 * i] = f.x;
       out[2 * i + 1] = f.y;
     }
   }
 }
-// `wide`: all eight go out in 16-byte pieces (or, with count < 8, nothing does)
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8], int count, bool wide) {
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&out)[8]) { unpack<T, 8>(r, out); }
+
+// `wide`: all V go out in wide pieces (or, with count < V, nothing does)
+template <typename T, int V>
+__device__ __forceinline__ void store_all(T* p, const float (&x)[V], int count, bool wide) {
   if (wide) {
-    if (count < 8) return;
-    uint32_t w[Raw8<T>::WORDS];
+    if (count < V) return;
+    uint32_t w[Raw<T, V>::WORDS];
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(x[i]);
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(x[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(x[2 * i], x[2 * i + 1]);
+      for (int i = 0; i < V / 2; ++i) w[i] = pack_pair<T>(x[2 * i], x[2 * i + 1]);
     }
+    if constexpr (Raw<T, V>::WORDS == 2) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < Raw8<T>::WORDS / 4; ++i)
-      reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      for (int i = 0; i < Raw<T, V>::WORDS / 4; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < V; ++i)
       if (i < count) p[i] = from_float<T>(x[i]);
   }
 }
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8], int count, bool wide) { store_all<T, 8>(p, x, count, wide); }
 
 // 1 / (1 + exp(-x)): both functions within a few units in the last place, exp(-x) = inf gives 0
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }

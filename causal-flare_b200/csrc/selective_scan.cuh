@@ -7,18 +7,20 @@
 namespace flare {
 namespace scan {
 
-constexpr int kChannels = 64;  // of a block
-constexpr int kLanes = 4;      // threads of a channel, S / 4 states each
-constexpr int kThreads = kChannels * kLanes;
+constexpr int kTile = 32;  // tokens of a tile, and between two kept states
 
-// tokens between two kept states, and of a tile: 512 state projections of b and of c at most
-__host__ __device__ constexpr int tile_tokens(int S) { return S <= 16 ? 32 : 16; }
+// How a block works: threads of a channel (each with S / lanes states), threads
+struct Shape {
+  int lanes, threads;
+  int channels() const { return threads / lanes; }
+};
+Shape shape_of(int S, bool backward);
 
 struct ScanParams {
   flare_scan_args_t a;
   int wide;       // rows of x, dt, z, y, dy and their gradients in 16-byte pieces
   int channels;   // of a group
-  int blocks_c;   // blocks along a group's channels
+  int blocks_c;   // blocks along a group's channels (of the kernels at hand: forward and backward differ)
   int segments, seg_tokens;  // tokens of a row are cut into segments of whole tiles
   // of every segment: what it leaves behind from zero, then (after the join) what it starts from; the sum of its deltas, -1: a
   // document begins in it
