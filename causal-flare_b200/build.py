@@ -1,4 +1,4 @@
-"""Build libflare_b200.so (sm_100a) from csrc/ with nvcc and the native host layer with g++.  Objects are cached by content hash."""
+"""Build libflare_b200.so (sm_100a) from csrc/ with nvcc and the native host layers with g++.  Objects are cached by content hash."""
 
 from __future__ import annotations
 
@@ -14,7 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build", "obj")
 LIB = os.path.join(HERE, "libflare_b200.so")
-HOST = os.path.join(HERE, "causal_flare", "_host.so")  # native host layer of the Python package (host_ext.cpp)
+# native host layers of the Python package
+HOSTS = [(src, os.path.join(HERE, "causal_flare", name)) for src, name in (("host_ext.cpp", "_host.so"), ("mixers_ext.cpp", "_mixers_host.so"))]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -108,31 +109,33 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
-    _build_host()
+    with cf.ThreadPoolExecutor(len(HOSTS)) as pool:
+        list(pool.map(lambda h: _build_host(*h), HOSTS))
     return LIB
 
 
-def _build_host() -> None:
-    """The native host layer: plain C++ against torch's headers (no CUDA code in it)."""
+def _build_host(src: str, out: str) -> None:
+    """A native host layer: plain C++ against torch's headers (no CUDA code in it)."""
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths
 
-    stamp = os.path.join(OBJ, "host_ext.sha")
-    dig = _digest("host_ext.cpp", [torch.__version__, sys.version])  # (an extension module of this interpreter)
-    if os.path.exists(HOST) and os.path.exists(stamp) and open(stamp).read() == dig:
+    stamp = os.path.join(OBJ, os.path.splitext(src)[0] + ".sha")
+    dig = _digest(src, [torch.__version__, sys.version])  # (an extension module of this interpreter)
+    if os.path.exists(out) and os.path.exists(stamp) and open(stamp).read() == dig:
         return
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_host",
+    module = os.path.splitext(os.path.basename(out))[0]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-DTORCH_EXTENSION_NAME={module}",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{p}" for p in (*include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include"))),
-           os.path.join(CSRC, "host_ext.cpp"), "-o", HOST,
+           os.path.join(CSRC, src), "-o", out,
            f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for host_ext.cpp:\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"g++ failed for {src}:\n{res.stdout}\n{res.stderr}")
     with open(stamp, "w") as f:
         f.write(dig)
 

@@ -88,6 +88,24 @@ def load() -> C.CDLL:
     return _bound
 
 
+_host = None
+
+
+def host():
+    """The native host layer (mixers_ext.cpp), bound to the loaded library: serves the plain calls of the operators."""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _mixers_host as native
+        except ImportError as e:
+            raise RuntimeError(f"the native host layer is missing ({e}). Build it with `python causal-flare_b200/build.py`.") from e
+        names = (*_CALLS, *_SIZES, "flare_mixers_abi_sizeof", "flare_status_string", "flare_last_cuda_error")
+        native.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in names})
+        _host = native
+    return _host
+
+
 def run(name: str, args, device, workspace: str | None = None) -> None:
     """Launch an entry point on the device's current stream, with a workspace of what `workspace` (a size query) asks for."""
     lib = load()

@@ -122,6 +122,10 @@ def flare_causal_attention(q, k, v, *, scale=None, cap=None, slopes=None, window
     ``scale`` defaults to D ** -0.5 (1 for D = 8, as in the FLARE operators); ``cap``, ``slopes`` [H] fp32, ``window``, ``documents`` and ``prefix`` as the module says.  Returns y
     [B, N, H, D].  Softmax statistics and sums are in fp32; its weights meet V in the inputs' type.  The gradients are the same bits
     in every call."""
+    if q.is_cuda:
+        y = _mixers.host().attention(q, k, v, scale, cap, slopes, window, documents, prefix)
+        if y is not None:
+            return y
     name = "flare_causal_attention"
     how = _attention_args(name, q, k, v, scale, cap, slopes, window, True)
     documents = whole_numbers(name, "documents", documents, q.shape[:2])
@@ -165,6 +169,10 @@ def flare_causal_attention_prefill(q, k, v, k_cache, v_cache, *, cached=None, le
     front.  ``lengths`` [B]: tokens of row b (None: N); what lies behind is padding: nothing is written for it and y is 0.  A token
     whose position lies outside the cache is treated the same way (a row whose ``cached`` does: all of it).  ``prefix`` marks tokens of
     the prompt's beginning that all new tokens see.  Returns y [B, N, H, D]; not differentiable."""
+    if q.is_cuda:
+        y = _mixers.host().attention_prefill(q, k, v, k_cache, v_cache, cached, lengths, scale, cap, slopes, window, prefix)
+        if y is not None:
+            return y
     name = "flare_causal_attention_prefill"
     how = _attention_args(name, q, k, v, scale, cap, slopes, window, True)
     _check_caches(name, q, k, k_cache, v_cache)
@@ -195,6 +203,10 @@ def flare_causal_attention_decode(q, k, v, k_cache, v_cache, cached, *, scale=No
     Its key and value are written to position cached[b] of the caches [B, L, J, D] and it sees them and the cached[b] in front; the
     caller counts ``cached`` up.  A row whose position lies outside the cache is idle: y is 0 and nothing is written (-1 for an empty
     slot of a batch).  Returns y in q's shape; not differentiable."""
+    if q.is_cuda:
+        y = _mixers.host().attention_decode(q, k, v, k_cache, v_cache, cached, scale, cap, slopes, window)
+        if y is not None:
+            return y
     name = "flare_causal_attention_decode"
     shape = q.shape
     q, k, v = (t[:, 0] if t.dim() == 4 and t.shape[1] == 1 else t for t in (q, k, v))

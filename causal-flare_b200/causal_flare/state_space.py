@@ -97,6 +97,10 @@ def flare_causal_conv(x, weight, bias=None, *, activation=None, documents=None):
 
     x [B, N, C]; weight [C, W] of 2 to 4 taps, the last one for the token itself; bias [C] in the weight's type.
     ``activation``: None or "silu".  Returns y [B, N, C] in x's type; sums are in fp32, weight gradients in the weight's type."""
+    if x.is_cuda:
+        y = _mixers.host().conv(x, weight, bias, activation, documents)
+        if y is not None:
+            return y
     name = "flare_causal_conv"
     code = _conv_args(name, x, weight, bias, activation, True)
     documents = whole_numbers(name, "documents", documents, x.shape[:2])
@@ -108,6 +112,10 @@ def flare_causal_conv_prefill(x, weight, bias=None, state=None, *, activation=No
     """Tokens on top of a carried state [B, W - 1, C] (the inputs in front of them, oldest first; None: zeros).
 
     Returns ``(y [B, N, C], state)`` with a fresh state in x's type; not differentiable."""
+    if x.is_cuda:
+        out = _mixers.host().conv_prefill(x, weight, bias, state, activation, lengths)
+        if out is not None:
+            return out
     name = "flare_causal_conv_prefill"
     code = _conv_args(name, x, weight, bias, activation, True)
     B, N, channels = x.shape
@@ -133,6 +141,10 @@ def flare_causal_conv_decode(x, weight, bias=None, state=None, *, activation=Non
     """One token: x [B, C] or [B, 1, C].  Returns ``(y in x's shape, state)``.
 
     The state is updated IN PLACE when it is contiguous (the returned one is then the same tensor); not differentiable."""
+    if x.is_cuda:
+        out = _mixers.host().conv_decode(x, weight, bias, state, activation)
+        if out is not None:
+            return out
     name = "flare_causal_conv_decode"
     shape = x.shape
     if x.dim() == 3 and x.shape[1] == 1:
@@ -265,6 +277,10 @@ def flare_selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, *, dt_sof
 
     x, dt, z [B, N, C]; A [C, S] with S of 8, 16 or 32; B, C [B, N, S], or [B, N, G, S] for G groups of channels; D, dt_bias
     [C].  A, D and dt_bias are fp32, the others share one type, which y [B, N, C] has too.  States and sums are in fp32."""
+    if x.is_cuda:
+        y = _mixers.host().scan(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus), documents)
+        if y is not None:
+            return y
     name = "flare_selective_scan"
     B, C = _scan_args(name, x, dt, A, B, C, D, z, dt_bias, True)
     documents = whole_numbers(name, "documents", documents, x.shape[:2])
@@ -288,6 +304,10 @@ def flare_selective_scan_prefill(x, dt, A, B, C, state=None, *, D=None, z=None, 
     """Tokens on top of a carried state [B, C, S] fp32 (None: zeros).
 
     Returns ``(y [B, N, C], state)`` with a fresh state; not differentiable."""
+    if x.is_cuda:
+        out = _mixers.host().scan_prefill(x, dt, A, B, C, state, D, z, dt_bias, bool(dt_softplus), lengths)
+        if out is not None:
+            return out
     name = "flare_selective_scan_prefill"
     B, C = _scan_args(name, x, dt, A, B, C, D, z, dt_bias, True)
     lengths = whole_numbers(name, "lengths", lengths, x.shape[:1])
@@ -308,6 +328,10 @@ def flare_selective_scan_decode(x, dt, A, B, C, state=None, *, D=None, z=None, d
 
     Returns ``(y in x's shape, state)``.  The state is updated IN PLACE when it is contiguous (the returned one is then the
     same tensor); not differentiable."""
+    if x.is_cuda:
+        out = _mixers.host().scan_decode(x, dt, A, B, C, state, D, z, dt_bias, bool(dt_softplus))
+        if out is not None:
+            return out
     name = "flare_selective_scan_decode"
     shape = x.shape
     if x.dim() == 3 and x.shape[1] == 1:
