@@ -7,8 +7,8 @@
 // dP = X1 Y1^T into tensor memory, rows of the own side on the lanes; the threads turn them into P and dS, laid down over S and dP
 // as packed 16-bit values, from where the products that are summed over the walk take their A operand (dV += P Y1,
 // dK or dQ += dS Y0): neither P nor dS passes through shared memory, and no gradient is added by two CTAs (a key head's dK and dV walk its
-// query heads one after the other).  The price is S and dP twice, 14 instead of 10 products of D operations for a pair.  Two groups of
-// four warps work on every other tile, so that one's exponentials run under the other's products.
+// query heads one after the other).  The price is S and dP twice, 14 instead of 10 products of D operations for a pair.  Two slots take every
+// other tile, with eight warps each (32 of the 64 columns a warp), so that one's exponentials run under the other's products.
 //
 // Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384.  P and dS are rounded once, to the type of the
 // operands they meet (fp16: what of dS lies below 2^-14 keeps an absolute 2^-25, as the gradients themselves do); everything in front
@@ -22,8 +22,8 @@ namespace attn {
 
 namespace {
 
-constexpr int kThreads = 320;
-constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr int kThreads = 576;  // four groups of four warps, products, copies
+constexpr int kWarpMma = 16, kWarpTma = 17;
 constexpr int kStages = 4, kWalk = 64;
 
 struct Stats {  // of a tile of queries (KEYS)
@@ -65,7 +65,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
     mbar_init(&misc->done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&misc->s_full[i], 1);
-      mbar_init(&misc->w_ready[i], 4);
+      mbar_init(&misc->w_ready[i], 8);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&misc->full[i], 1);
@@ -123,58 +123,49 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
       }
     }
   } else if (warp == kWarpMma) {
-    constexpr uint32_t ID_S = make_idesc<F16>(128, kWalk, 0, 0);
-    constexpr uint32_t ID_SUM = make_idesc<F16>(128, 64 * DB, 0, 1);
-    const auto step_y = [](uint64_t desc, int i) { return desc + (uint64_t)(((i >> 2) * 8192 + (i & 3) * 32) >> 4); };
-    const auto scores = [&](int n) {
-      const int s = n % kStages, slot = n & 1;
-      if (!(ok = wait(&misc->full[s], (n / kStages) & 1))) return;
-      uint8_t* const y = smem + L::Y + s * 2 * L::TILE;
-      if (p.masks.dirty[(int64_t)b * (p.masks.Nkp >> 6) + row_of(n) / kWalk]) {
-        clear_rows<DB, kWalk>(y, p.masks, b, p.Nk, row_of(n), lane);
-        clear_rows<DB, kWalk>(y + L::TILE, p.masks, b, p.Nk, row_of(n), lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      tc_fence_after_sync();
-      if (elect_one()) {
-        const uint64_t dx0 = make_desc_sw128(smem_u32(smem), 16, 1024), dx1 = make_desc_sw128(smem_u32(smem + L::OWN), 16, 1024);
-        const uint64_t dy0 = make_desc_sw128(smem_u32(y), 16, 1024), dy1 = make_desc_sw128(smem_u32(y + L::TILE), 16, 1024);
+    if (total > 0 && elect_one()) {  // (one thread all along: what it does between two products is on every tile's way)
+      constexpr uint32_t ID_S = make_idesc<F16>(128, kWalk, 0, 0);
+      constexpr uint32_t ID_SUM = make_idesc<F16>(128, 64 * DB, 0, 1);
+      const auto step_y = [](uint64_t desc, int i) { return desc + (uint64_t)(((i >> 2) * 8192 + (i & 3) * 32) >> 4); };
+      const uint64_t dx0 = make_desc_sw128(smem_u32(smem), 16, 1024), dx1 = make_desc_sw128(smem_u32(smem + L::OWN), 16, 1024);
+      const uint32_t y = smem_u32(smem + L::Y);
+      const uint64_t k0 = make_desc_sw128(y, 16, 1024), k1 = make_desc_sw128(y + L::TILE, 16, 1024);      // K-major
+      const uint64_t mn0 = make_desc_sw128(y, 8192, 1024), mn1 = make_desc_sw128(y + L::TILE, 8192, 1024);  // MN-major
+      const auto scores = [&](int n) {
+        const int s = n % kStages, slot = n & 1;
+        if (!(ok = wait_one(&misc->full[s], (n / kStages) & 1))) return;
+        tc_fence_after_sync();
+        const uint64_t at = (uint64_t)((s * 2 * L::TILE) >> 4);
 #pragma unroll
-        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128, kmaj_step(dx0, i), step_y(dy0, i), ID_S, i > 0);
+        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128, kmaj_step(dx0, i), step_y(k0 + at, i), ID_S, i > 0);
 #pragma unroll
-        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128 + 64, kmaj_step(dx1, i), step_y(dy1, i), ID_S, i > 0);
+        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128 + 64, kmaj_step(dx1, i), step_y(k1 + at, i), ID_S, i > 0);
         tc_commit(&misc->s_full[slot]);
-      }
-      __syncwarp();
-    };
-    if (total > 0) {
-      ok = wait(&misc->own_full, 0);
+      };
+      ok = wait_one(&misc->own_full, 0);
       if (ok) scores(0);
       if (ok && total > 1) scores(1);
       for (int n = 0; ok && n < total; ++n) {
         const int s = n % kStages, slot = n & 1;
-        if (!(ok = wait(&misc->w_ready[slot], (n >> 1) & 1))) break;
+        if (!(ok = wait_one(&misc->w_ready[slot], (n >> 1) & 1))) break;
         tc_fence_after_sync();
-        if (elect_one()) {
-          const uint32_t y = smem_u32(smem + L::Y + s * 2 * L::TILE);
-          const uint64_t dy0 = make_desc_sw128(y, 8192, 1024), dy1 = make_desc_sw128(y + L::TILE, 8192, 1024);
-          if (KEYS) {
+        const uint64_t at = (uint64_t)((s * 2 * L::TILE) >> 4);
+        if (KEYS) {
 #pragma unroll
-            for (int i = 0; i < kWalk / 16; ++i) mma_ts(tmem + T_P, tmem + slot * 128 + i * 8, mnmaj_step(dy1, i), ID_SUM, i > 0 || n > 0);
-          }
-#pragma unroll
-          for (int i = 0; i < kWalk / 16; ++i) mma_ts(tmem + T_DS, tmem + slot * 128 + 64 + i * 8, mnmaj_step(dy0, i), ID_SUM, i > 0 || n > 0);
-          tc_commit(&misc->empty[s]);
-          if (n + 1 == total) tc_commit(&misc->done);
+          for (int i = 0; i < kWalk / 16; ++i)
+            mma_ts(tmem + T_P, tmem + slot * 128 + (i >> 1) * 32 + (i & 1) * 8, mnmaj_step(mn1 + at, i), ID_SUM, i > 0 || n > 0);
         }
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kWalk / 16; ++i)
+          mma_ts(tmem + T_DS, tmem + slot * 128 + 64 + (i >> 1) * 32 + (i & 1) * 8, mnmaj_step(mn0 + at, i), ID_SUM, i > 0 || n > 0);
+        tc_commit(&misc->empty[s]);
+        if (n + 1 == total) tc_commit(&misc->done);
         if (n + 2 < total) scores(n + 2);  // (behind the products that read P and dS where it goes: products run in order)
       }
     }
   } else {
-    const int slot = warp >> 2, row = x0 + (warp & 3) * 32 + lane;
-    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + slot * 128, td = ts + 64;
+    const int slot = (warp >> 2) & 1, half = warp >> 3, row = x0 + (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + slot * 128 + half * 32, td = ts + 64;
     float lse = INFINITY, delta = 0.0f;
     int2 keys = make_int2(0, 0);
     if (!KEYS) {
@@ -184,63 +175,80 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
       keys = p.masks.range[(int64_t)b * p.masks.Nqp + row];
     }
     ScoreScale sc = score_scale(p, KEYS ? head * group : head);
+    const CapSeries series(sc.in);
+    DirtyTiles dirty(p.masks, b);
 #pragma unroll 1
     for (int n = slot; n < total; n += 2) {
       const int y0 = row_of(n), s_ = n % kStages;
       if (KEYS && BIAS) sc = score_scale(p, head_of(n));
-      // (its completion follows from that of the copies, so the statistics are there too; the wait on `full` makes them visible)
-      if (KEYS && !(ok = wait(&misc->full[s_], (n / kStages) & 1))) break;
+      // (the tile has been there since before its scores; the wait on `full` makes its statistics visible to this thread)
+      const bool unclean = dirty(y0 / kWalk);
+      if ((KEYS || unclean) && !(ok = wait(&misc->full[s_], (n / kStages) & 1))) break;
       if (!(ok = wait(&misc->s_full[slot], (n >> 1) & 1))) break;
       tc_fence_after_sync();
+      if (unclean) {  // scores of rows that belong to nobody are masked, whatever they are; the products behind them take the rows themselves
+        const int r = half * 32 + (warp & 3) * 8 + (lane >> 2);
+        if ((lane & 3) < 2) clear_row<DB, kWalk>(smem + L::Y + (s_ * 2 + (lane & 1)) * L::TILE, p.masks, b, p.Nk, y0, r);
+        fence_proxy_async_smem();
+      }
       const Stats& st = misc->stats[s_];
       const bool all = KEYS ? st.keys[0].y >= x0 + 128 && st.keys[kWalk - 1].x <= x0
                             : __all_sync(0xffffffffu, keys.x <= y0 && keys.y >= y0 + kWalk) != 0;
       const float d0 = (float)(row - y0);
+      // 16 columns at a time, of this warp's half; packed, they take the first of the columns that they were read from
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], d[32];
-        tmem_ld32(ts + c * 32, s);
-        tmem_ld32(td + c * 32, d);
+        const int col0 = half * 32 + c * 16;
+        uint32_t s[16], d[16], pw[8], dw[8];
+        tmem_ld16(ts + c * 16, s);
+        tmem_ld16(td + c * 16, d);
         tmem_wait_ld();
-        tmem_fence_regs(s);
-        tmem_fence_regs(d);
-        float wp[2], wd[2];
-        uint32_t pw[16], dw[16];
+        tmem_fence_regs16(s);
+        tmem_fence_regs16(d);
+        const auto in_sight = [&](int col) {
+          const int2 see = KEYS ? st.keys[col] : keys;
+          const int key = KEYS ? row : y0 + col;
+          return key >= see.x && key < see.y;
+        };
+        if (CAP) {
+          if (!all) {  // (what lies out of sight does not choose the form)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const int col = c * 32 + k;
-          const float l = KEYS ? st.lse[col] : lse, dl = KEYS ? st.delta[col] : delta;
-          float x = __uint_as_float(s[k]), r = 0.0f;
-          if (CAP) {
-            r = cap_weight(x, sc);
-            x = capped(r, sc);
-            if (BIAS) x = fmaf(-sc.slope, fabsf(d0 - (float)col), x);
-            x -= l;
-          } else if (BIAS) {
-            x = fmaf(-sc.slope, fabsf(d0 - (float)col), x * sc.plain) - l;
-          } else {
-            x = fmaf(x, sc.plain, -l);
+            for (int k = 0; k < 16; ++k)
+              if (!in_sight(col0 + k)) s[k] = 0u;
           }
-          float w = ex2_approx(x);
-          float g = w * (__uint_as_float(d[k]) - dl);
-          if (CAP) g *= 4.0f * r * (1.0f - r);
-          if (!all) {
-            const int2 see = KEYS ? st.keys[col] : keys;
-            const int key = KEYS ? row : y0 + col;
-            const bool on = key >= see.x && key < see.y;
-            w = on ? w : 0.0f;
-            g = on ? g : 0.0f;
-          }
-          wp[k & 1] = w;
-          wd[k & 1] = g;
-          if (k & 1) {
-            pw[k >> 1] = pack2<F16>(wp[0], wp[1]);
-            dw[k >> 1] = pack2<F16>(wd[0], wd[1]);
-          }
+          cap_scores(s, series, sc.in);
         }
-        // (the halves' reads come in the order of their writes: columns 16 c of what was read is all read by now)
-        if (KEYS) tmem_st16(ts + c * 16, pw);
-        tmem_st16(td + c * 16, dw);
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          const int col = col0 + k;
+          const float2 l = KEYS ? *reinterpret_cast<const float2*>(&st.lse[col]) : make_float2(lse, lse);
+          const float2 dl = KEYS ? *reinterpret_cast<const float2*>(&st.delta[col]) : make_float2(delta, delta);
+          const uint64_t t = f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+          float b0 = -l.x, b1 = -l.y;
+          if (BIAS) {
+            b0 = fmaf(-sc.slope, fabsf(d0 - (float)col), b0);
+            b1 = fmaf(-sc.slope, fabsf(d0 - (float)(col + 1)), b1);
+          }
+          float w0, w1;
+          f2_unpack(f2_fma(t, twice(sc.unit), f2_pack(b0, b1)), w0, w1);
+          w0 = ex2_approx(w0);
+          w1 = ex2_approx(w1);
+          uint64_t g = f2_mul(f2_pack(w0, w1), f2_add(f2_pack(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), f2_pack(-dl.x, -dl.y)));
+          if (CAP) g = f2_mul(g, f2_fma(f2_mul(t, twice(-1.0f)), t, twice(1.0f)));
+          float g0, g1;
+          f2_unpack(g, g0, g1);
+          if (!all) {
+            const bool on0 = in_sight(col), on1 = in_sight(col + 1);
+            w0 = on0 ? w0 : 0.0f;
+            g0 = on0 ? g0 : 0.0f;
+            w1 = on1 ? w1 : 0.0f;
+            g1 = on1 ? g1 : 0.0f;
+          }
+          pw[k >> 1] = pack2<F16>(w0, w1);
+          dw[k >> 1] = pack2<F16>(g0, g1);
+        }
+        if (KEYS) tmem_st8(ts + c * 8, pw);
+        tmem_st8(td + c * 8, dw);
       }
       tmem_wait_st();
       tc_fence_before_sync();
@@ -261,14 +269,13 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
         }
         if (row < rows) store_columns<F16>(reinterpret_cast<uint16_t*>(out) + at, c * 32, p.D, r, f);
       };
-      if (KEYS) {  // a group each
+      if (KEYS) {  // a sum for the groups of a slot, half the columns each
 #pragma unroll
-        for (int c = 0; c < 2 * DB; ++c)
-          if (slot == 0) put(p.dk, T_DS, c, p.scale);
-          else put(p.dv, T_P, c, 1.0f);
-      } else {  // half the columns each
-#pragma unroll
-        for (int c = 0; c < DB; ++c) put(p.dq, T_DS, slot * DB + c, p.scale);
+        for (int c = 0; c < DB; ++c)
+          if (slot == 0) put(p.dk, T_DS, half * DB + c, p.scale);
+          else put(p.dv, T_P, half * DB + c, 1.0f);
+      } else if (slot * 2 + half < 2 * DB) {  // 32 columns each
+        put(p.dq, T_DS, slot * 2 + half, p.scale);
       }
     }
   }

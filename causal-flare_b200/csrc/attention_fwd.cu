@@ -1,14 +1,17 @@
 // Attention forward on tcgen05: y = softmax(scores) V in one pass over the keys.
 //
-// One CTA per head and 256 queries, as two groups of 128 (a thread is a query is a lane of tensor memory).  Per tile of 128 keys and
+// One CTA per head and 256 queries, as two groups of 128 (a thread is a query is a lane of tensor memory).  Per tile of 64 keys and
 // group: S = Q K^T into tensor memory, the group's threads read their rows, take the running maximum and lay P = exp2(S - m) down
-// over S as packed 16-bit values, O += P V takes its A operand from there.  The groups take turns on the tensor cores: while
-// one works on its exponentials the other's products run.  O stays in tensor memory; it is rescaled only where the maximum has grown by
+// over S as packed 16-bit values, O += P V takes its A operand from there.  S has two buffers per group, so that a group finds its next
+// scores when it is done with a tile; with one buffer of 128 keys it waited
+// for its own two products and their hand-overs every time: 5 100 cycles for 128 keys, of which its own work took 3 000.
+// O stays in tensor memory; it is rescaled only where the maximum has grown by
 // more than 2^8 since the frame was set (exact: the frame cancels in O / l; P up to 2^8 is still far from the end of fp16).
 // Sums are of the unrounded weights, in fp32; P is rounded once, to the type of V, which is what the products take.
 //
-// Tensor memory: S / P of the groups at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, K and V two stages each.
-// Bound by the tensor cores and the exponentials alike (128 x 128 x 2 D products of 512 cycles against 128 x 128 / 16 exponentials).
+// Tensor memory: S / P of the groups, two buffers each, at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, K and V four
+// stages of 16 KB each.  Floors per 64 keys and both groups, in cycles: products 1 024 (M = 128, N = 64 from shared memory: 1 280),
+// exponentials 1 024.
 #include "attention_tc.cuh"
 
 namespace flare {
@@ -22,16 +25,18 @@ constexpr int kThreads = 320;  // two groups of four warps, products, copies
 constexpr int kWarpMma = 8, kWarpTma = 9;
 constexpr float kGrowth = 8.0f;
 
+constexpr int kKeys = 64, kStages = 4;
+
 struct Misc {
-  uint64_t q_full[2], k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_ready[2], o_done[2];
+  uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2][2], p_ready[2][2], o_free[2], o_done[2];
   uint32_t tmem_base;
   volatile int abort_flag;
 };
 
 template <int DB>
 struct Layout {
-  static constexpr int STAGES = DB == 1 ? 4 : 2, TILE = DB * 16384;
-  static constexpr int K = 2 * TILE, V = K + STAGES * TILE, MISC = V + STAGES * TILE, BYTES = MISC + (int)sizeof(Misc) + 1024;
+  static constexpr int Q = DB * 16384, TILE = DB * 8192;
+  static constexpr int K = 2 * Q, V = K + kStages * TILE, MISC = V + kStages * TILE, BYTES = MISC + (int)sizeof(Misc) + 1024;
 };
 
 template <int DB, bool F16, bool CAP, bool BIAS>
@@ -46,11 +51,14 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
   if (tid == 0) {
     for (int g = 0; g < 2; ++g) {
       mbar_init(&misc->q_full[g], 1);
-      mbar_init(&misc->s_full[g], 1);
-      mbar_init(&misc->p_ready[g], 4);
+      mbar_init(&misc->o_free[g], 1);
       mbar_init(&misc->o_done[g], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&misc->s_full[g][i], 1);
+        mbar_init(&misc->p_ready[g][i], 4);
+      }
     }
-    for (int i = 0; i < L::STAGES; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&misc->k_full[i], 1);
       mbar_init(&misc->k_empty[i], 1);
       mbar_init(&misc->v_full[i], 1);
@@ -77,8 +85,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
   for (int g = 0; g < 2; ++g) {
     const int tile = block * 2 + g;
     const int2 s = tile * 128 < p.masks.Nqp ? p.masks.query_span[b * (p.masks.Nqp >> 7) + tile] : make_int2(0, 0);
-    first[g] = s.x >> 7;
-    last[g] = s.y > s.x ? (s.y + 127) >> 7 : first[g];
+    first[g] = s.x / kKeys;
+    last[g] = s.y > s.x ? (s.y + kKeys - 1) / kKeys : first[g];
   }
   const bool have0 = last[0] > first[0], have1 = last[1] > first[1];
   const int j0 = have0 ? (have1 ? min(first[0], first[1]) : first[0]) : first[1];
@@ -93,77 +101,73 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
     if (elect_one()) {
       for (int g = 0; g < 2; ++g)
         if (last[g] > first[g]) {
-          mbar_arrive_expect_tx(&misc->q_full[g], L::TILE);
-          for (int d = 0; d < DB; ++d) tma_load_4d(smem + g * L::TILE + d * 16384, &tm_q, &misc->q_full[g], d * 64, h, q0 + g * 128, b);
+          mbar_arrive_expect_tx(&misc->q_full[g], L::Q);
+          for (int d = 0; d < DB; ++d) tma_load_4d(smem + g * L::Q + d * 16384, &tm_q, &misc->q_full[g], d * 64, h, q0 + g * 128, b);
         }
       int n = 0;
       for (int j = j0; ok && j < j1; ++j) {
         if (!in(0, j) && !in(1, j)) continue;
-        const int s = n % L::STAGES;
-        const uint32_t phase = (n / L::STAGES) & 1;
+        const int s = n % kStages;
+        const uint32_t phase = (n / kStages) & 1;
         if (!(ok = wait_one(&misc->k_empty[s], phase ^ 1))) break;
         mbar_arrive_expect_tx(&misc->k_full[s], L::TILE);
         for (int d = 0; d < DB; ++d)
-          tma_load_4d(smem + L::K + s * L::TILE + d * 16384, &tm_k, &misc->k_full[s], d * 64, kv, j * 128, b);
+          tma_load_4d(smem + L::K + s * L::TILE + d * 8192, &tm_k, &misc->k_full[s], d * 64, kv, j * kKeys, b);
         if (!(ok = wait_one(&misc->v_empty[s], phase ^ 1))) break;
         mbar_arrive_expect_tx(&misc->v_full[s], L::TILE);
         for (int d = 0; d < DB; ++d)
-          tma_load_4d(smem + L::V + s * L::TILE + d * 16384, &tm_v, &misc->v_full[s], d * 64, kv, j * 128, b);
+          tma_load_4d(smem + L::V + s * L::TILE + d * 8192, &tm_v, &misc->v_full[s], d * 64, kv, j * kKeys, b);
         ++n;
       }
     }
   } else if (warp == kWarpMma) {
-    constexpr uint32_t ID_S = make_idesc<F16>(128, 128, 0, 0);      // Q, K: K-major
-    constexpr uint32_t ID_O = make_idesc<F16>(128, 64 * DB, 0, 1);  // P (tensor memory), V: MN-major
-    int n = 0, count[2] = {0, 0};
-    const auto scores = [&](int g, int tile) {  // of the n-th tile in the ring
-      const int s = tile % L::STAGES;
-      if (!(ok = wait(&misc->k_full[s], (tile / L::STAGES) & 1))) return;
-      tc_fence_after_sync();
-      if (elect_one()) {
-        const uint64_t dq = make_desc_sw128(smem_u32(smem + g * L::TILE), 16, 1024);
-        const uint64_t dk = make_desc_sw128(smem_u32(smem + L::K + s * L::TILE), 16, 1024);
-#pragma unroll
-        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + g * 128, kmaj_step(dq, i), kmaj_step(dk, i), ID_S, i > 0);
-        tc_commit(&misc->s_full[g]);
-      }
-      __syncwarp();
-    };
-    for (int j = j0; ok && j < j1; ++j) {
-      if (!in(0, j) && !in(1, j)) continue;
-      const int s = n % L::STAGES;
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (ok && in(g, j) && j == first[g] && (ok = wait(&misc->q_full[g], 0))) scores(g, n);
-      if (!ok) break;
-      if (elect_one()) tc_commit(&misc->k_empty[s]);  // (the scores of this tile have all been issued)
-      __syncwarp();
-      if (!(ok = wait(&misc->v_full[s], (n / L::STAGES) & 1))) break;
-      const uint8_t* const dirty = p.masks.dirty + (int64_t)b * (p.masks.Nkp >> 6) + j * 2;
-      if (dirty[0] | dirty[1]) {
-        clear_rows<DB, 128>(smem + L::V + s * L::TILE, p.masks, b, p.Nk, j * 128, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (!ok || !in(g, j)) continue;
-        if (!(ok = wait(&misc->p_ready[g], count[g] & 1))) break;
+    if (elect_one()) {  // (one thread all along: what it does between two products is on every tile's way)
+      constexpr uint32_t ID_S = make_idesc<F16>(128, kKeys, 0, 0);    // Q, K: K-major
+      constexpr uint32_t ID_O = make_idesc<F16>(128, 64 * DB, 0, 1);  // P (tensor memory), V: MN-major
+      const uint64_t dq[2] = {make_desc_sw128(smem_u32(smem), 16, 1024), make_desc_sw128(smem_u32(smem + L::Q), 16, 1024)};
+      const uint64_t dk0 = make_desc_sw128(smem_u32(smem + L::K), 16, 1024), dv0 = make_desc_sw128(smem_u32(smem + L::V), 8192, 1024);
+      int n = 0, count[2] = {0, 0};  // tiles in the ring, tiles of a group behind it
+      const auto scores = [&](int g, int ahead) {  // of the group's next tile but `ahead`, which is the ring's tile n + ahead
+        const int s = (n + ahead) % kStages, buffer = (count[g] + ahead) & 1;
+        if (!(ok = wait_one(&misc->k_full[s], ((n + ahead) / kStages) & 1))) return;
         tc_fence_after_sync();
-        if (elect_one()) {
-          const uint64_t dv = make_desc_sw128(smem_u32(smem + L::V + s * L::TILE), 16384, 1024);
+        const uint64_t dk = dk0 + (uint64_t)((s * L::TILE) >> 4);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mma_ts(tmem + 256 + g * 128, tmem + g * 128 + i * 8, mnmaj_step(dv, i), ID_O, i > 0 || count[g] > 0);
+        for (int i = 0; i < 4 * DB; ++i)
+          mma_ss(tmem + g * 128 + buffer * 64, kmaj_step(dq[g], i), dk + (uint64_t)(((i >> 2) * 8192 + (i & 3) * 32) >> 4), ID_S, i > 0);
+        tc_commit(&misc->s_full[g][buffer]);
+      };
+      for (int j = j0; ok && j < j1; ++j) {
+        if (!in(0, j) && !in(1, j)) continue;
+        const int s = n % kStages;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (ok && in(g, j) && j == first[g] && (ok = wait_one(&misc->q_full[g], 0))) {
+            scores(g, 0);
+            if (ok && j + 1 < last[g]) scores(g, 1);
+          }
+        if (!ok) break;
+        tc_commit(&misc->k_empty[s]);  // (the scores of this tile have all been issued)
+        if (!(ok = wait_one(&misc->v_full[s], (n / kStages) & 1))) break;
+        const uint64_t dv = dv0 + (uint64_t)((s * L::TILE) >> 4);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (!ok || !in(g, j)) continue;
+          const int buffer = count[g] & 1;
+          if (!(ok = wait_one(&misc->p_ready[g][buffer], (count[g] >> 1) & 1))) break;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_ts(tmem + 256 + g * 128, tmem + g * 128 + buffer * 64 + i * 8, mnmaj_step(dv, i), ID_O, i > 0 || count[g] > 0);
+          tc_commit(&misc->o_free[g]);
           if (j + 1 == last[g]) tc_commit(&misc->o_done[g]);
+          if (j + 2 < last[g]) scores(g, 2);  // (behind the product that reads P where S goes: products run in order)
+          ++count[g];
         }
-        __syncwarp();
-        ++count[g];
-        if (j + 1 < last[g]) scores(g, n + 1);  // (behind the product that reads P where S goes: products run in order)
+        if (!ok) break;
+        tc_commit(&misc->v_empty[s]);
+        ++n;
       }
-      if (!ok) break;
-      if (elect_one()) tc_commit(&misc->v_empty[s]);
-      __syncwarp();
-      ++n;
     }
   } else {
     const int g = warp >> 2, row = (warp & 3) * 32 + lane, i = q0 + g * 128 + row;
@@ -172,61 +176,80 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
     const int2 keys = inside ? p.masks.range[(int64_t)b * p.masks.Nqp + i] : make_int2(0, 0);
     const int position = i + (p.masks.cached != nullptr ? p.masks.cached[b] : 0);
     const ScoreScale sc = score_scale(p, h);
+    const CapSeries series(sc.in);
+    DirtyTiles dirty(p.masks, b);
     float m = -INFINITY, sum = 0.0f;
     const int tiles = last[g] - first[g];
+    // the ring's number of this group's first tile: tiles that nobody walks (between the groups' keys) are not in the ring
+    const int ring0 = g == 0 || !have0 ? 0 : first[1] > last[0] ? last[0] - first[0] : first[1] - j0;
 #pragma unroll 1
     for (int n = 0; n < tiles; ++n) {
-      const int key0 = (first[g] + n) * 128;
-      if (!(ok = wait(&misc->s_full[g], n & 1))) break;
+      const int key0 = (first[g] + n) * kKeys;
+      const uint32_t tp = ts + (n & 1) * 64;
+      if (!(ok = wait(&misc->s_full[g][n & 1], (n >> 1) & 1))) break;
       tc_fence_after_sync();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s[c]);
+      uint32_t s[2][32];
+      tmem_ld32(tp, s[0]);
+      tmem_ld32(tp + 32, s[1]);
+      if (dirty(first[g] + n)) {  // (both groups may clear the same rows: zeros over zeros)
+        const int stage = (ring0 + n) % kStages;
+        if (!(ok = wait(&misc->v_full[stage], ((ring0 + n) / kStages) & 1))) break;
+        if (row < kKeys) clear_row<DB, kKeys>(smem + L::V + stage * L::TILE, p.masks, b, p.Nk, key0, row);
+        fence_proxy_async_smem();
+      }
       tmem_wait_ld();
+      tmem_fence_regs(s[0]);
+      tmem_fence_regs(s[1]);
+      const bool full = __all_sync(0xffffffffu, keys.x <= key0 && keys.y >= key0 + kKeys) != 0;
+      const int from = keys.x - key0, to_ = keys.y - key0;
+      if (CAP) {
+        if (!full) {  // (what lies out of sight does not choose the form)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_fence_regs(s[c]);
-      if (CAP || BIAS) {
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0u;
+        }
+        cap_scores(s[0], series, sc.in);
+        cap_scores(s[1], series, sc.in);
+      }
+      if (BIAS) {
         const float d0 = (float)(position - key0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            float x = __uint_as_float(s[c][k]);
-            x = CAP ? capped(cap_weight(x, sc), sc) : x * sc.plain;
-            if (BIAS) x = fmaf(-sc.slope, fabsf(d0 - (float)(c * 32 + k)), x);
-            s[c][k] = __float_as_uint(x);
-          }
+          for (int k = 0; k < 32; ++k)
+            s[c][k] = __float_as_uint(fmaf(-sc.slope, fabsf(d0 - (float)(c * 32 + k)), __uint_as_float(s[c][k]) * sc.unit));
       }
-      if (!__all_sync(0xffffffffu, keys.x <= key0 && keys.y >= key0 + 128)) {
-        const int from = keys.x - key0, to_ = keys.y - key0;
+      if (!full) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int k = 0; k < 32; ++k)
             if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0xff800000u;  // -inf
       }
-      float top = -INFINITY;
-      {
-        float t4[4];
+      float t4[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          t4[c] = __uint_as_float(s[c][0]);
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t* const v = s[c >> 1] + (c & 1) * 16;
+        t4[c] = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 #pragma unroll
-          for (int k = 1; k + 1 < 32; k += 2) t4[c] = fmax3(t4[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-          t4[c] = fmaxf(t4[c], __uint_as_float(s[c][31]));
-        }
-        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+        for (int k = 2; k < 16; k += 2) t4[c] = fmax3(t4[c], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
       }
-      const float unit = CAP || BIAS ? 1.0f : sc.plain;
-      top *= unit;
+      const float unit = BIAS ? 1.0f : sc.unit;
+      const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * unit;
       const bool grow = top > m + kGrowth || (m == -INFINITY && top > m);
       if (n == 0) {
         if (grow) m = top;
       } else if (__any_sync(0xffffffffu, grow)) {
+        // O is at rest once the product of the tile before is done.  (That of the one before it is: these scores were issued behind it,
+        // so the barrier is in this phase or through with it.)
+        if (!(ok = wait(&misc->o_free[g], (n - 1) & 1))) break;
+        tc_fence_after_sync();
         const float f = grow ? ex2_approx(m - top) : 1.0f;
         if (grow) m = top;
         sum *= f;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2 * DB; ++c) {
           uint32_t o[32];
           tmem_read<32>(to + c * 32, o);
@@ -236,30 +259,30 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
         }
       }
       const float frame = m == -INFINITY ? 0.0f : m;
-      const uint64_t unit2 = f2_pack(unit, unit), frame2 = f2_pack(-frame, -frame);
+      const uint64_t unit2 = twice(unit), frame2 = twice(-frame);
       uint64_t sum2[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const uint64_t x = f2_pack(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
           float lo, hi;
-          f2_unpack(CAP || BIAS ? f2_add(x, frame2) : f2_fma(x, unit2, frame2), lo, hi);
+          f2_unpack(BIAS ? f2_add(x, frame2) : f2_fma(x, unit2, frame2), lo, hi);
           lo = ex2_approx(lo);
           hi = ex2_approx(hi);
           sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(lo, hi));
           w[k] = pack2<F16>(lo, hi);
         }
-        tmem_st16(ts + c * 16, w);
+        tmem_st16(tp + c * 16, w);
       }
+      tmem_wait_st();
+      tc_fence_before_sync();
+      warp_arrive(&misc->p_ready[g][n & 1], lane);
       float a0, a1, a2, a3;
       f2_unpack(sum2[0], a0, a1);
       f2_unpack(sum2[1], a2, a3);
       sum += (a0 + a1) + (a2 + a3);
-      tmem_wait_st();
-      tc_fence_before_sync();
-      warp_arrive(&misc->p_ready[g], lane);
     }
     if (ok && tiles > 0 && !(ok = wait(&misc->o_done[g], 0))) sum = 0.0f;
     if (ok) {
@@ -295,8 +318,8 @@ int launch(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t st
   constexpr int DB = FLARE_ATTN_DB;
   CUtensorMap q, k, v;
   if (!head_map(&q, a.q, a.B, a.Nq, a.H, a.D, a.q_stride_b, a.q_stride_n, a.q_stride_h, 128) ||
-      !head_map(&k, a.k, a.B, a.Nk, a.J, a.D, a.k_stride_b, a.k_stride_n, a.k_stride_h, 128) ||
-      !head_map(&v, a.v, a.B, a.Nk, a.J, a.D, a.v_stride_b, a.v_stride_n, a.v_stride_h, 128))
+      !head_map(&k, a.k, a.B, a.Nk, a.J, a.D, a.k_stride_b, a.k_stride_n, a.k_stride_h, kKeys) ||
+      !head_map(&v, a.v, a.B, a.Nk, a.J, a.D, a.v_stride_b, a.v_stride_n, a.v_stride_h, kKeys))
     return FLARE_ERR_CUDA;
   const bool cap = p.cap > 0.0f, bias = p.slopes != nullptr;
   auto* const kernel = cap ? (bias ? attention_forward_kernel<DB, F16, true, true> : attention_forward_kernel<DB, F16, true, false>)

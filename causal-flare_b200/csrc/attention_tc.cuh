@@ -9,25 +9,62 @@ namespace attn {
 
 using namespace tc;
 
-// Scores in units of log 2.  CAP: cap tanh(s / cap) = cap (1 - 2 r) with r = 1 / (exp(2 s / cap) + 1); the absolute error is a few
-// 2^-24 of cap whatever s is (tanh.approx would be off by 2^-11 of it, hundredths of a nat).
+// Scores, in units of log 2 once they are multiplied by `unit`.  CAP: cap tanh(x), x = scale <q, k> / cap.  The special-function
+// unit would give tanh as 1 - 2 / (exp(2 x) + 1), two results of it per score where the softmax itself takes one (tanh.approx is off by 2^-11 of
+// cap, hundredths of a nat); for |x| <= 1 / 2, where caps leave all but a few scores, an odd polynomial does it on the FMA pipe: the
+// least largest error of x p(x^2) with five coefficients there is 3.1e-9 (a weighted least-squares fit, repeated until its
+// error is level), with fp32 arithmetic 3.6e-8.  A warp that meets a larger |x| takes the exponential form.
 struct ScoreScale {
-  float plain;     // scale log2 e
-  float cap_in;    // 2 log2 e scale / cap
-  float cap_out;   // cap log2 e
-  float slope;     // of the head, log2 e times
+  float unit;   // scale log2 e, or cap log2 e
+  float in;     // scale / cap
+  float slope;  // of the head, log2 e times
 };
 __device__ __forceinline__ ScoreScale score_scale(const AttnParams& p, int h) {
   ScoreScale s;
-  s.plain = p.scale * kLog2e;
-  s.cap_in = p.cap > 0.0f ? 2.0f * kLog2e * p.scale / p.cap : 0.0f;
-  s.cap_out = p.cap * kLog2e;
+  s.unit = (p.cap > 0.0f ? p.cap : p.scale) * kLog2e;
+  s.in = p.cap > 0.0f ? p.scale / p.cap : 0.0f;
   s.slope = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.0f;
   return s;
 }
-// r of the capped score
-__device__ __forceinline__ float cap_weight(float s, const ScoreScale& c) { return rcp_approx(ex2_approx(s * c.cap_in) + 1.0f); }
-__device__ __forceinline__ float capped(float r, const ScoreScale& c) { return fmaf(-2.0f * c.cap_out, r, c.cap_out); }
+__device__ __forceinline__ uint64_t twice(float x) { return f2_pack(x, x); }
+// the polynomial's coefficients, for raw products
+struct CapSeries {
+  uint64_t c[5];
+  __device__ __forceinline__ explicit CapSeries(float in) {
+    const float q = in * in;
+    c[0] = twice(0.9999999403953552f * in);
+    c[1] = twice(-0.3333277702331543f * in * q);
+    c[2] = twice(0.13320569694042206f * in * q * q);
+    c[3] = twice(-0.05276204273104668f * in * q * q * q);
+    c[4] = twice(0.016737382858991623f * in * q * q * q * q);
+  }
+};
+__device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.0f, rcp_approx(ex2_approx(x * (2.0f * kLog2e)) + 1.0f), 1.0f); }
+
+// raw products, in place: tanh of the capped score.  Whole warp.
+template <int N>
+__device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const CapSeries& series, float in) {
+  float most = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; k += 2) most = fmax3(most, fabsf(__uint_as_float(s[k])), fabsf(__uint_as_float(s[k + 1])));
+  if (__all_sync(0xffffffffu, most * in <= 0.5f)) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      const uint64_t x = f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), q = f2_mul(x, x);
+      uint64_t t = f2_fma(q, series.c[4], series.c[3]);
+      t = f2_fma(q, t, series.c[2]);
+      t = f2_fma(q, t, series.c[1]);
+      t = f2_fma(q, t, series.c[0]);
+      float lo, hi;
+      f2_unpack(f2_mul(x, t), lo, hi);
+      s[k] = __float_as_uint(lo);
+      s[k + 1] = __float_as_uint(hi);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = __float_as_uint(tanh_any(__uint_as_float(s[k]) * in));
+  }
+}
 
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -46,19 +83,32 @@ inline bool head_map(CUtensorMap* map, const void* base, int B, int N, int heads
   return make_map_bf16(map, base, 4, dims, strides, box);
 }
 
-// Clears the rows of a staged tile ([DB][ROWS][64 elements]) whose keys belong to nobody: their weights are 0, but 0 times what
-// may lie there need not be.  Whole warp; the caller orders the async proxy behind it.
+// Clears a row of a staged tile ([DB][ROWS][64 elements]) if its token belongs to nobody: its weights are 0, but 0 times what
+// may lie there need not be.  The caller orders the async proxy behind it.
 template <int DB, int ROWS>
-__device__ __forceinline__ void clear_rows(uint8_t* tile, const Masks& m, int b, int64_t per_row, int first, int lane) {
-#pragma unroll 1
-  for (int r = lane; r < ROWS; r += 32)
-    if (!m.owned(b, per_row, first + r)) {
+__device__ __forceinline__ void clear_row(uint8_t* tile, const Masks& m, int b, int64_t per_row, int first, int r) {
+  if (m.owned(b, per_row, first + r)) return;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + (d * ROWS + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-    }
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + (d * ROWS + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
+
+// Which of a row's tiles of 64 tokens hold some that belong to nobody: 32 tiles at a time, a bit each.  Whole warps.
+struct DirtyTiles {
+  const uint8_t* flags;
+  int count, base;
+  unsigned bits;
+  __device__ __forceinline__ DirtyTiles(const Masks& m, int b) : flags(m.dirty + (int64_t)b * (m.Nkp >> 6)), count(m.Nkp >> 6), base(-32), bits(0) {}
+  __device__ __forceinline__ bool operator()(int tile) {
+    if ((unsigned)(tile - base) >= 32u) {
+      base = tile;
+      const int at = tile + (threadIdx.x & 31);
+      bits = __ballot_sync(0xffffffffu, at < count && flags[at] != 0);
+    }
+    return bits >> (tile - base) & 1;
+  }
+};
 
 // 32 columns of fp32 times `f`, rounded, to a row of an output (columns from D on left out; D is a multiple of 8)
 template <bool F16>
