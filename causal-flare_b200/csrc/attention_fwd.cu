@@ -9,9 +9,11 @@
 // more than 2^8 since the frame was set (exact: the frame cancels in O / l; P up to 2^8 is still far from the end of fp16).
 // Sums are of the unrounded weights, in fp32; P is rounded once, to the type of V, which is what the products take.
 //
-// Tensor memory: S / P of the groups, two buffers each, at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, K and V four
-// stages of 16 KB each.  Floors per 64 keys and both groups, in cycles: products 1 024 (M = 128, N = 64 from shared memory: 1 280),
+// Tensor memory: S / P of the groups, two buffers each, at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, the
+// first two tiles of K, four stages of a tile of V and one of K.  Floors per 64 keys and both groups, in cycles: products 1 024 (M = 128, N = 64 from shared memory: 1 280),
 // exponentials 1 024.
+#include <limits.h>
+
 #include "attention_tc.cuh"
 
 namespace flare {
@@ -25,10 +27,10 @@ constexpr int kThreads = 320;  // two groups of four warps, products, copies
 constexpr int kWarpMma = 8, kWarpTma = 9;
 constexpr float kGrowth = 8.0f;
 
-constexpr int kKeys = 64, kStages = 4;
+constexpr int kKeys = 64, kStages = 4, kAhead = 2;
 
 struct Misc {
-  uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2][2], p_ready[2][2], o_free[2], o_done[2];
+  uint64_t q_full[2], head_full[kAhead], full[kStages], empty[kStages], s_full[2][2], p_ready[2][2], o_free[2], o_done[2];
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -36,7 +38,9 @@ struct Misc {
 template <int DB>
 struct Layout {
   static constexpr int Q = DB * 16384, TILE = DB * 8192;
-  static constexpr int K = 2 * Q, V = K + kStages * TILE, MISC = V + kStages * TILE, BYTES = MISC + (int)sizeof(Misc) + 1024;
+  // keys of the first tiles, then stages: the values of tile n and the keys of tile n + 2, which are needed at the same time
+  static constexpr int HEAD = 2 * Q, RING = HEAD + kAhead * TILE, STAGE = 2 * TILE, MISC = RING + kStages * STAGE, BYTES = MISC + (int)sizeof(Misc) + 1024;
+  static_assert(BYTES <= kMaxDynamicSmem, "shared memory");
 };
 
 template <int DB, bool F16, bool CAP, bool BIAS>
@@ -59,11 +63,10 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
       }
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&misc->k_full[i], 1);
-      mbar_init(&misc->k_empty[i], 1);
-      mbar_init(&misc->v_full[i], 1);
-      mbar_init(&misc->v_empty[i], 1);
+      mbar_init(&misc->full[i], 1);
+      mbar_init(&misc->empty[i], 1);
     }
+    for (int i = 0; i < kAhead; ++i) mbar_init(&misc->head_full[i], 1);
     misc->abort_flag = 0;
     fence_barrier_init();
   }
@@ -79,19 +82,16 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
 
   const int lanes = p.B * p.H, block = gridDim.x / lanes - 1 - blockIdx.x / lanes;  // (causal: the longest first)
   const int b = blockIdx.x % lanes / p.H, h = blockIdx.x % p.H, kv = h / (p.H / p.J), q0 = block * 256;
-  // tiles of keys of each group
-  int first[2], last[2];
+  // tiles of keys of each group: both begin with the first that one of them sees
+  int last[2], j0 = INT_MAX;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     const int tile = block * 2 + g;
     const int2 s = tile * 128 < p.masks.Nqp ? p.masks.query_span[b * (p.masks.Nqp >> 7) + tile] : make_int2(0, 0);
-    first[g] = s.x / kKeys;
-    last[g] = s.y > s.x ? (s.y + kKeys - 1) / kKeys : first[g];
+    last[g] = s.y > s.x ? (s.y + kKeys - 1) / kKeys : 0;
+    if (s.y > s.x) j0 = min(j0, s.x / kKeys);
   }
-  const bool have0 = last[0] > first[0], have1 = last[1] > first[1];
-  const int j0 = have0 ? (have1 ? min(first[0], first[1]) : first[0]) : first[1];
-  const int j1 = have0 ? (have1 ? max(last[0], last[1]) : last[0]) : last[1];
-  const auto in = [&](int g, int j) { return j >= first[g] && j < last[g]; };
+  const int tiles[2] = {max(0, last[0] - j0), max(0, last[1] - j0)}, total = max(tiles[0], tiles[1]);
   bool ok = true;
   const auto wait_one = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, &misc->abort_flag, 8); };
   // (whole warps give up together)
@@ -99,25 +99,26 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
 
   if (warp == kWarpTma) {
     if (elect_one()) {
+      const auto load = [&](const CUtensorMap* map, uint8_t* to, uint64_t* bar, int n) {
+        for (int d = 0; d < DB; ++d) tma_load_4d(to + d * 8192, map, bar, d * 64, kv, (j0 + n) * kKeys, b);
+      };
       for (int g = 0; g < 2; ++g)
-        if (last[g] > first[g]) {
+        if (tiles[g] > 0) {
           mbar_arrive_expect_tx(&misc->q_full[g], L::Q);
           for (int d = 0; d < DB; ++d) tma_load_4d(smem + g * L::Q + d * 16384, &tm_q, &misc->q_full[g], d * 64, h, q0 + g * 128, b);
         }
-      int n = 0;
-      for (int j = j0; ok && j < j1; ++j) {
-        if (!in(0, j) && !in(1, j)) continue;
+      for (int n = 0; n < min(kAhead, total); ++n) {
+        mbar_arrive_expect_tx(&misc->head_full[n], L::TILE);
+        load(&tm_k, smem + L::HEAD + n * L::TILE, &misc->head_full[n], n);
+      }
+      for (int n = 0; n < total; ++n) {
         const int s = n % kStages;
-        const uint32_t phase = (n / kStages) & 1;
-        if (!(ok = wait_one(&misc->k_empty[s], phase ^ 1))) break;
-        mbar_arrive_expect_tx(&misc->k_full[s], L::TILE);
-        for (int d = 0; d < DB; ++d)
-          tma_load_4d(smem + L::K + s * L::TILE + d * 8192, &tm_k, &misc->k_full[s], d * 64, kv, j * kKeys, b);
-        if (!(ok = wait_one(&misc->v_empty[s], phase ^ 1))) break;
-        mbar_arrive_expect_tx(&misc->v_full[s], L::TILE);
-        for (int d = 0; d < DB; ++d)
-          tma_load_4d(smem + L::V + s * L::TILE + d * 8192, &tm_v, &misc->v_full[s], d * 64, kv, j * kKeys, b);
-        ++n;
+        if (!(ok = wait_one(&misc->empty[s], ((n / kStages) & 1) ^ 1))) break;
+        uint8_t* const stage = smem + L::RING + s * L::STAGE;
+        const bool more = n + kAhead < total;
+        mbar_arrive_expect_tx(&misc->full[s], more ? 2 * L::TILE : L::TILE);
+        load(&tm_v, stage, &misc->full[s], n);
+        if (more) load(&tm_k, stage + L::TILE, &misc->full[s], n + kAhead);
       }
     }
   } else if (warp == kWarpMma) {
@@ -125,48 +126,42 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
       constexpr uint32_t ID_S = make_idesc<F16>(128, kKeys, 0, 0);    // Q, K: K-major
       constexpr uint32_t ID_O = make_idesc<F16>(128, 64 * DB, 0, 1);  // P (tensor memory), V: MN-major
       const uint64_t dq[2] = {make_desc_sw128(smem_u32(smem), 16, 1024), make_desc_sw128(smem_u32(smem + L::Q), 16, 1024)};
-      const uint64_t dk0 = make_desc_sw128(smem_u32(smem + L::K), 16, 1024), dv0 = make_desc_sw128(smem_u32(smem + L::V), 8192, 1024);
-      int n = 0, count[2] = {0, 0};  // tiles in the ring, tiles of a group behind it
-      const auto scores = [&](int g, int ahead) {  // of the group's next tile but `ahead`, which is the ring's tile n + ahead
-        const int s = (n + ahead) % kStages, buffer = (count[g] + ahead) & 1;
-        if (!(ok = wait_one(&misc->k_full[s], ((n + ahead) / kStages) & 1))) return;
-        tc_fence_after_sync();
-        const uint64_t dk = dk0 + (uint64_t)((s * L::TILE) >> 4);
+      const uint64_t dk0 = make_desc_sw128(smem_u32(smem), 16, 1024), dv0 = make_desc_sw128(smem_u32(smem + L::RING), 8192, 1024);
+      const auto scores = [&](int g, int buffer, int at) {  // of the keys that lie at byte `at`
+        const uint64_t dk = dk0 + (uint64_t)(at >> 4);
 #pragma unroll
         for (int i = 0; i < 4 * DB; ++i)
           mma_ss(tmem + g * 128 + buffer * 64, kmaj_step(dq[g], i), dk + (uint64_t)(((i >> 2) * 8192 + (i & 3) * 32) >> 4), ID_S, i > 0);
         tc_commit(&misc->s_full[g][buffer]);
       };
-      for (int j = j0; ok && j < j1; ++j) {
-        if (!in(0, j) && !in(1, j)) continue;
-        const int s = n % kStages;
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        if (ok && n < total) ok = wait_one(&misc->head_full[n], 0);
 #pragma unroll
         for (int g = 0; g < 2; ++g)
-          if (ok && in(g, j) && j == first[g] && (ok = wait_one(&misc->q_full[g], 0))) {
-            scores(g, 0);
-            if (ok && j + 1 < last[g]) scores(g, 1);
+          if (ok && n < tiles[g] && (ok = wait_one(&misc->q_full[g], 0))) {
+            tc_fence_after_sync();
+            scores(g, n, L::HEAD + n * L::TILE);
           }
-        if (!ok) break;
-        tc_commit(&misc->k_empty[s]);  // (the scores of this tile have all been issued)
-        if (!(ok = wait_one(&misc->v_full[s], (n / kStages) & 1))) break;
-        const uint64_t dv = dv0 + (uint64_t)((s * L::TILE) >> 4);
+      }
+#pragma unroll 1
+      for (int n = 0; ok && n < total; ++n) {
+        const int s = n % kStages, buffer = n & 1;
+        if (!(ok = wait_one(&misc->full[s], (n / kStages) & 1))) break;
+        const uint64_t dv = dv0 + (uint64_t)((s * L::STAGE) >> 4);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          if (!ok || !in(g, j)) continue;
-          const int buffer = count[g] & 1;
-          if (!(ok = wait_one(&misc->p_ready[g][buffer], (count[g] >> 1) & 1))) break;
+          if (n >= tiles[g]) continue;
+          if (!(ok = wait_one(&misc->p_ready[g][buffer], (n >> 1) & 1))) break;
           tc_fence_after_sync();
 #pragma unroll
           for (int i = 0; i < kKeys / 16; ++i)
-            mma_ts(tmem + 256 + g * 128, tmem + g * 128 + buffer * 64 + i * 8, mnmaj_step(dv, i), ID_O, i > 0 || count[g] > 0);
+            mma_ts(tmem + 256 + g * 128, tmem + g * 128 + buffer * 64 + i * 8, mnmaj_step(dv, i), ID_O, i > 0 || n > 0);
           tc_commit(&misc->o_free[g]);
-          if (j + 1 == last[g]) tc_commit(&misc->o_done[g]);
-          if (j + 2 < last[g]) scores(g, 2);  // (behind the product that reads P where S goes: products run in order)
-          ++count[g];
+          if (n + 1 == tiles[g]) tc_commit(&misc->o_done[g]);
+          if (n + kAhead < tiles[g]) scores(g, buffer, L::RING + s * L::STAGE + L::TILE);  // (behind the product that reads P where S goes: products run in order)
         }
-        if (!ok) break;
-        tc_commit(&misc->v_empty[s]);
-        ++n;
+        if (ok) tc_commit(&misc->empty[s]);
       }
     }
   } else {
@@ -179,22 +174,19 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
     const CapSeries series(sc.in);
     DirtyTiles dirty(p.masks, b);
     float m = -INFINITY, sum = 0.0f;
-    const int tiles = last[g] - first[g];
-    // the ring's number of this group's first tile: tiles that nobody walks (between the groups' keys) are not in the ring
-    const int ring0 = g == 0 || !have0 ? 0 : first[1] > last[0] ? last[0] - first[0] : first[1] - j0;
 #pragma unroll 1
-    for (int n = 0; n < tiles; ++n) {
-      const int key0 = (first[g] + n) * kKeys;
+    for (int n = 0; n < tiles[g]; ++n) {
+      const int key0 = (j0 + n) * kKeys;
       const uint32_t tp = ts + (n & 1) * 64;
       if (!(ok = wait(&misc->s_full[g][n & 1], (n >> 1) & 1))) break;
       tc_fence_after_sync();
       uint32_t s[2][32];
       tmem_ld32(tp, s[0]);
       tmem_ld32(tp + 32, s[1]);
-      if (dirty(first[g] + n)) {  // (both groups may clear the same rows: zeros over zeros)
-        const int stage = (ring0 + n) % kStages;
-        if (!(ok = wait(&misc->v_full[stage], ((ring0 + n) / kStages) & 1))) break;
-        if (row < kKeys) clear_row<DB, kKeys>(smem + L::V + stage * L::TILE, p.masks, b, p.Nk, key0, row);
+      if (dirty(j0 + n)) {  // (both groups may clear the same rows: zeros over zeros)
+        const int stage = n % kStages;
+        if (!(ok = wait(&misc->full[stage], (n / kStages) & 1))) break;
+        if (row < kKeys) clear_row<DB, kKeys>(smem + L::RING + stage * L::STAGE, p.masks, b, p.Nk, key0, row);
         fence_proxy_async_smem();
       }
       tmem_wait_ld();
@@ -284,7 +276,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
       f2_unpack(sum2[1], a2, a3);
       sum += (a0 + a1) + (a2 + a3);
     }
-    if (ok && tiles > 0 && !(ok = wait(&misc->o_done[g], 0))) sum = 0.0f;
+    if (ok && tiles[g] > 0) ok = wait(&misc->o_done[g], 0);
     if (ok) {
       tc_fence_after_sync();
       const float inv = sum > 0.0f ? 1.0f / sum : sum != sum ? sum : 0.0f;
@@ -292,7 +284,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
 #pragma unroll
       for (int c = 0; c < 2 * DB; ++c) {
         uint32_t o[32];
-        if (tiles > 0) {
+        if (tiles[g] > 0) {
           tmem_read<32>(to + c * 32, o);
         } else {
 #pragma unroll

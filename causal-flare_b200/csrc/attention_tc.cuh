@@ -11,9 +11,9 @@ using namespace tc;
 
 // Scores, in units of log 2 once they are multiplied by `unit`.  CAP: cap tanh(x), x = scale <q, k> / cap.  The special-function
 // unit would give tanh as 1 - 2 / (exp(2 x) + 1), two results of it per score where the softmax itself takes one (tanh.approx is off by 2^-11 of
-// cap, hundredths of a nat); for |x| <= 1 / 2, where caps leave all but a few scores, an odd polynomial does it on the FMA pipe: the
-// least largest error of x p(x^2) with five coefficients there is 3.1e-9 (a weighted least-squares fit, repeated until its
-// error is level), with fp32 arithmetic 3.6e-8.  A warp that meets a larger |x| takes the exponential form.
+// cap, hundredths of a nat); for |x| <= 0.35, where caps leave nearly all scores, an odd polynomial does it on the FMA pipe: the
+// least largest error of x p(x^2) with four coefficients there is 5.9e-9 (a weighted least-squares fit, repeated until its
+// error is level), with fp32 arithmetic 3.9e-8.  A warp that meets a larger |x| takes the exponential form.
 struct ScoreScale {
   float unit;   // scale log2 e, or cap log2 e
   float in;     // scale / cap
@@ -29,14 +29,13 @@ __device__ __forceinline__ ScoreScale score_scale(const AttnParams& p, int h) {
 __device__ __forceinline__ uint64_t twice(float x) { return f2_pack(x, x); }
 // the polynomial's coefficients, for raw products
 struct CapSeries {
-  uint64_t c[5];
+  uint64_t c[4];
   __device__ __forceinline__ explicit CapSeries(float in) {
     const float q = in * in;
-    c[0] = twice(0.9999999403953552f * in);
-    c[1] = twice(-0.3333277702331543f * in * q);
-    c[2] = twice(0.13320569694042206f * in * q * q);
-    c[3] = twice(-0.05276204273104668f * in * q * q * q);
-    c[4] = twice(0.016737382858991623f * in * q * q * q * q);
+    c[0] = twice(0.9999998211860657f * in);
+    c[1] = twice(-0.3333165645599365f * in * q);
+    c[2] = twice(0.13283318281173706f * in * q * q);
+    c[3] = twice(-0.04837666451931f * in * q * q * q);
   }
 };
 __device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.0f, rcp_approx(ex2_approx(x * (2.0f * kLog2e)) + 1.0f), 1.0f); }
@@ -47,12 +46,11 @@ __device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const CapSeries& se
   float most = 0.0f;
 #pragma unroll
   for (int k = 0; k < N; k += 2) most = fmax3(most, fabsf(__uint_as_float(s[k])), fabsf(__uint_as_float(s[k + 1])));
-  if (__all_sync(0xffffffffu, most * in <= 0.5f)) {
+  if (__all_sync(0xffffffffu, most * in <= 0.35f)) {
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
       const uint64_t x = f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), q = f2_mul(x, x);
-      uint64_t t = f2_fma(q, series.c[4], series.c[3]);
-      t = f2_fma(q, t, series.c[2]);
+      uint64_t t = f2_fma(q, series.c[3], series.c[2]);
       t = f2_fma(q, t, series.c[1]);
       t = f2_fma(q, t, series.c[0]);
       float lo, hi;
