@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   }
 }
 
-// delta = <dy, y>, half a warp per row and head; 0 for queries without keys (their dy may hold anything)
+// -delta = -<dy, y>, half a warp per row and head; 0 for queries without keys (their dy may hold anything)
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const AttnParams p, const T* dy, int64_t sb, int64_t sn, int64_t sh, float* delta) {
   pdl_begin();
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const AttnParams p, const T*
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (live && lane == 0) delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum;
+  if (live && lane == 0) delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = -sum;
 }
 
 struct Layout {

@@ -28,7 +28,7 @@ struct AttnParams {
   Masks masks;
   const float* slopes;
   float* lse;          // forward: written, may be null; backward: read
-  const float* delta;  // backward: [B][H][Nqp] <dy, y>
+  const float* delta;  // backward: [B][H][Nqp] -<dy, y>
   void *y, *dq, *dk, *dv;
   int* err;
   int B, Nq, Nk, H, J, D;

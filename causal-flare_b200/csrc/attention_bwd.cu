@@ -10,7 +10,7 @@
 // query heads one after the other).  The price is S and dP twice, 14 instead of 10 products of D operations for a pair.  Two slots take every
 // other tile, with eight warps each (32 of the 64 columns a warp), so that one's exponentials run under the other's products.
 //
-// Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384.  P and dS are rounded once, to the type of the
+// Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P and dS are rounded once, to the type of the
 // operands they meet (fp16: what of dS lies below 2^-14 keeps an absolute 2^-25, as the gradients themselves do); everything in front
 // of that, and the sums, is fp32.
 #include "attention_tc.cuh"
@@ -26,13 +26,13 @@ constexpr int kThreads = 576;  // four groups of four warps, products, copies
 constexpr int kWarpMma = 16, kWarpTma = 17;
 constexpr int kStages = 4, kWalk = 64;
 
-struct Stats {  // of a tile of queries (KEYS)
+struct Stats {  // of a tile of queries (KEYS); lse and delta with their signs changed
   float lse[kWalk], delta[kWalk];
   int2 keys[kWalk];
 };
 struct Misc {
   alignas(16) Stats stats[kStages];
-  uint64_t own_full, full[kStages], empty[kStages], s_full[2], w_ready[2], done;
+  uint64_t own_full, own_ready, full[kStages], empty[kStages], s_full[2], w_ready[2], done;
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -55,13 +55,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __grid_constant__ CUtensorMap tm_x1,
                           const __grid_constant__ CUtensorMap tm_y0, const __grid_constant__ CUtensorMap tm_y1, const AttnParams p) {
   using L = Layout<DB>;
-  constexpr uint32_t T_DS = 256, T_P = 384;
+  constexpr uint32_t T_DS = 256, T_P = 384, T_X = 384;  // (queries: no sum of P products, their two own tiles instead)
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   Misc* const misc = reinterpret_cast<Misc*>(smem + L::MISC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     mbar_init(&misc->own_full, 1);
+    mbar_init(&misc->own_ready, 16);
     mbar_init(&misc->done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&misc->s_full[i], 1);
@@ -137,12 +138,19 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
         tc_fence_after_sync();
         const uint64_t at = (uint64_t)((s * 2 * L::TILE) >> 4);
 #pragma unroll
-        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128, kmaj_step(dx0, i), step_y(k0 + at, i), ID_S, i > 0);
+        for (int i = 0; i < 4 * DB; ++i) {
+          if (KEYS) mma_ss(tmem + slot * 128, kmaj_step(dx0, i), step_y(k0 + at, i), ID_S, i > 0);
+          else mma_ts(tmem + slot * 128, tmem + T_X + i * 8, step_y(k0 + at, i), ID_S, i > 0);
+        }
 #pragma unroll
-        for (int i = 0; i < 4 * DB; ++i) mma_ss(tmem + slot * 128 + 64, kmaj_step(dx1, i), step_y(k1 + at, i), ID_S, i > 0);
+        for (int i = 0; i < 4 * DB; ++i) {
+          if (KEYS) mma_ss(tmem + slot * 128 + 64, kmaj_step(dx1, i), step_y(k1 + at, i), ID_S, i > 0);
+          else mma_ts(tmem + slot * 128 + 64, tmem + T_X + 32 * DB + i * 8, step_y(k1 + at, i), ID_S, i > 0);
+        }
         tc_commit(&misc->s_full[slot]);
       };
-      ok = wait_one(&misc->own_full, 0);
+      ok = wait_one(KEYS ? &misc->own_full : &misc->own_ready, 0);
+      tc_fence_after_sync();
       if (ok) scores(0);
       if (ok && total > 1) scores(1);
       for (int n = 0; ok && n < total; ++n) {
@@ -166,7 +174,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
   } else {
     const int slot = (warp >> 2) & 1, half = warp >> 3, row = x0 + (warp & 3) * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + slot * 128 + half * 32, td = ts + 64;
-    float lse = INFINITY, delta = 0.0f;
+    float lse = -INFINITY, delta = 0.0f;  // (signs changed)
     int2 keys = make_int2(0, 0);
     if (!KEYS) {
       const int64_t at = ((int64_t)b * p.H + head) * p.masks.Nqp + row;
@@ -177,8 +185,31 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
     ScoreScale sc = score_scale(p, KEYS ? head * group : head);
     const CapSeries series(sc.in);
     DirtyTiles dirty(p.masks, b);
+    if (!KEYS && total > 0) {
+      // the own tiles move to tensor memory, from where products of 64 columns take them at the full rate: with both operands in shared
+      // memory they are bound by its bandwidth (128 + 64 rows of 32 bytes in 32 cycles).  A quarter of the columns a warp.
+      if ((ok = wait(&misc->own_full, 0))) {
+        const int r = (warp & 3) * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint8_t* const from = smem + t * L::OWN + (DB == 2 ? half * 16384 : 0);
+          const int part = DB == 2 ? slot : half * 2 + slot;  // of the row's 128 bytes there: a half, or a quarter
+          constexpr int PIECES = DB == 2 ? 4 : 2;
+          uint32_t w[PIECES * 4];
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from + swz_chunk_off(r, part * PIECES + c));
+            w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+          }
+          tmem_write<PIECES * 4>(tl + T_X + t * 32 * DB + (DB == 2 ? half * 32 : 0) + part * PIECES * 4, w);
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        warp_arrive(&misc->own_ready, lane);
+      }
+    }
 #pragma unroll 1
-    for (int n = slot; n < total; n += 2) {
+    for (int n = slot; ok && n < total; n += 2) {
       const int y0 = row_of(n), s_ = n % kStages;
       if (KEYS && BIAS) sc = score_scale(p, head_of(n));
       // (the tile has been there since before its scores; the wait on `full` makes its statistics visible to this thread)
@@ -196,60 +227,71 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
                             : __all_sync(0xffffffffu, keys.x <= y0 && keys.y >= y0 + kWalk) != 0;
       const float d0 = (float)(row - y0);
       // 16 columns at a time, of this warp's half; packed, they take the first of the columns that they were read from
+      const auto columns = [&](auto masked_) {  // (apart for tiles in full sight: a look at every pair keeps the pairs from overlapping)
+        constexpr bool MASKED = decltype(masked_)::value;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int col0 = half * 32 + c * 16;
-        uint32_t s[16], d[16], pw[8], dw[8];
-        tmem_ld16(ts + c * 16, s);
-        tmem_ld16(td + c * 16, d);
-        tmem_wait_ld();
-        tmem_fence_regs16(s);
-        tmem_fence_regs16(d);
-        const auto in_sight = [&](int col) {
-          const int2 see = KEYS ? st.keys[col] : keys;
-          const int key = KEYS ? row : y0 + col;
-          return key >= see.x && key < see.y;
-        };
-        if (CAP) {
-          if (!all) {  // (what lies out of sight does not choose the form)
+        for (int c = 0; c < 2; ++c) {
+          const int col0 = half * 32 + c * 16;
+          uint32_t s[16], d[16], pw[8], dw[8];
+          tmem_ld16(ts + c * 16, s);
+          tmem_ld16(td + c * 16, d);
+          tmem_wait_ld();
+          tmem_fence_regs16(s);
+          tmem_fence_regs16(d);
+          unsigned on = 0xffffu;
+          if (MASKED) {
+            on = 0;
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-              if (!in_sight(col0 + k)) s[k] = 0u;
+            for (int k = 0; k < 16; ++k) {
+              const int2 see = KEYS ? st.keys[col0 + k] : keys;
+              const int key = KEYS ? row : y0 + col0 + k;
+              on |= (unsigned)(key >= see.x && key < see.y) << k;
+            }
           }
-          cap_scores(s, series, sc.in);
+          if (CAP) {
+            if (MASKED) {  // (what lies out of sight does not choose the form)
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (!(on >> k & 1)) s[k] = 0u;
+            }
+            cap_scores(s, series, sc.in);
+          }
+#pragma unroll
+          for (int k4 = 0; k4 < 16; k4 += 4) {
+            ulonglong2 l4 = make_ulonglong2(twice(lse), twice(lse)), d4 = make_ulonglong2(twice(delta), twice(delta));
+            if (KEYS) {
+              l4 = *reinterpret_cast<const ulonglong2*>(&st.lse[col0 + k4]);
+              d4 = *reinterpret_cast<const ulonglong2*>(&st.delta[col0 + k4]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const int k = k4 + e, col = col0 + k;
+              const uint64_t t = f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+              uint64_t bias = e ? l4.y : l4.x;
+              if (BIAS) bias = f2_fma(twice(-sc.slope), f2_pack(fabsf(d0 - (float)col), fabsf(d0 - (float)(col + 1))), bias);
+              float w0, w1, g0, g1;
+              f2_unpack(f2_fma(t, twice(sc.unit), bias), w0, w1);
+              w0 = ex2_approx(w0);
+              w1 = ex2_approx(w1);
+              uint64_t g = f2_mul(f2_pack(w0, w1), f2_add(f2_pack(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), e ? d4.y : d4.x));
+              if (CAP) g = f2_mul(g, f2_fma(f2_mul(t, twice(-1.0f)), t, twice(1.0f)));
+              f2_unpack(g, g0, g1);
+              if (MASKED) {
+                w0 = on >> k & 1 ? w0 : 0.0f;
+                g0 = on >> k & 1 ? g0 : 0.0f;
+                w1 = on >> (k + 1) & 1 ? w1 : 0.0f;
+                g1 = on >> (k + 1) & 1 ? g1 : 0.0f;
+              }
+              pw[k >> 1] = pack2<F16>(w0, w1);
+              dw[k >> 1] = pack2<F16>(g0, g1);
+            }
+          }
+          if (KEYS) tmem_st8(ts + c * 8, pw);
+          tmem_st8(td + c * 8, dw);
         }
-#pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          const int col = col0 + k;
-          const float2 l = KEYS ? *reinterpret_cast<const float2*>(&st.lse[col]) : make_float2(lse, lse);
-          const float2 dl = KEYS ? *reinterpret_cast<const float2*>(&st.delta[col]) : make_float2(delta, delta);
-          const uint64_t t = f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-          float b0 = -l.x, b1 = -l.y;
-          if (BIAS) {
-            b0 = fmaf(-sc.slope, fabsf(d0 - (float)col), b0);
-            b1 = fmaf(-sc.slope, fabsf(d0 - (float)(col + 1)), b1);
-          }
-          float w0, w1;
-          f2_unpack(f2_fma(t, twice(sc.unit), f2_pack(b0, b1)), w0, w1);
-          w0 = ex2_approx(w0);
-          w1 = ex2_approx(w1);
-          uint64_t g = f2_mul(f2_pack(w0, w1), f2_add(f2_pack(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), f2_pack(-dl.x, -dl.y)));
-          if (CAP) g = f2_mul(g, f2_fma(f2_mul(t, twice(-1.0f)), t, twice(1.0f)));
-          float g0, g1;
-          f2_unpack(g, g0, g1);
-          if (!all) {
-            const bool on0 = in_sight(col), on1 = in_sight(col + 1);
-            w0 = on0 ? w0 : 0.0f;
-            g0 = on0 ? g0 : 0.0f;
-            w1 = on1 ? w1 : 0.0f;
-            g1 = on1 ? g1 : 0.0f;
-          }
-          pw[k >> 1] = pack2<F16>(w0, w1);
-          dw[k >> 1] = pack2<F16>(g0, g1);
-        }
-        if (KEYS) tmem_st8(ts + c * 8, pw);
-        tmem_st8(td + c * 8, dw);
-      }
+      };
+      if (all) columns(std::false_type());
+      else columns(std::true_type());
       tmem_wait_st();
       tc_fence_before_sync();
       warp_arrive(&misc->w_ready[slot], lane);

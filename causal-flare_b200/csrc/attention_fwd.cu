@@ -292,8 +292,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
         }
         if (i < p.Nq) store_columns<F16>(y, c * 32, p.D, o, inv);
       }
-      // (a query without keys: +inf, so that every weight the backward forms is 0)
-      if (p.lse != nullptr && inside) p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum == 0.0f ? INFINITY : m + __log2f(sum);
+      // with its sign changed, as the backward adds it (a query without keys: -inf, so that every weight formed with it is 0)
+      if (p.lse != nullptr && inside) p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum == 0.0f ? -INFINITY : -(m + __log2f(sum));
     }
   }
   if (!ok) {

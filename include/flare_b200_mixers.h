@@ -121,7 +121,7 @@ typedef struct flare_attention_args {
   const void* k;            /* [B, Nk, J, D] */
   const void* v;            /* [B, Nk, J, D] */
   void* y;                  /* [B, Nq, H, D] contiguous */
-  float* lse;               /* [B, H, Nq rounded up to 128]: log2 of the softmax denominators, for the backward; may be NULL */
+  float* lse;               /* [B, H, Nq rounded up to 128]: minus log2 of the softmax denominators, for the backward; may be NULL */
   const int32_t* documents; /* [B, Nq] contiguous or NULL */
   const uint8_t* prefix;    /* [B, Nq] contiguous or NULL */
   const int32_t* cached;    /* [B] or NULL */
