@@ -226,6 +226,8 @@ def _fill_scan(x, dt, A, B, C_, D, z, dt_bias, softplus, documents=None, lengths
     for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
         if t is not None:
             t = t.contiguous()
+            if name == "A" and t.data_ptr() % 16:
+                t = t.clone()
             held.append(t)
             setattr(a, name, t.data_ptr())
     a.documents, a.lengths = _lib.ptr(documents), _lib.ptr(lengths)

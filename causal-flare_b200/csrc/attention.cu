@@ -301,22 +301,35 @@ struct DecodeParams {
 
 constexpr int kDecodeWarps = 4, kHeads = 16;  // heads of a block: the rows of a product
 
-template <bool F16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// rows 8 to 15 of the product: none of them has a head (EIGHT), or they are there
+template <bool F16, bool EIGHT>
+__device__ __forceinline__ void mma16816(float (&d)[EIGHT ? 2 : 4], const uint32_t (&a)[EIGHT ? 2 : 4], uint32_t b0, uint32_t b1) {
+  if constexpr (EIGHT) {
+    float none0, none1;
+    if constexpr (F16)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
+                   : "+f"(d[0]), "+f"(d[1]), "=f"(none0), "=f"(none1) : "r"(a[0]), "r"(0), "r"(a[1]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
+                   : "+f"(d[0]), "+f"(d[1]), "=f"(none0), "=f"(none1) : "r"(a[0]), "r"(0), "r"(a[1]), "r"(b0), "r"(b1), "f"(0.0f));
+  } else {
+    if constexpr (F16)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                   : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                   : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
 }
+
 // One token.  Bound by memory: every key and value in sight is read once, by one block for up to 16 query heads that share
 // them.  A warp takes 16 keys at a time, straight from memory into the operands of m16n8k16 products: heads are the rows, so the
 // scores come out as the A operand that the product with V takes.  A thread's 16-byte piece of a key covers the contraction in an
 // order of its own (the queries are laid out in the same one); pairs of keys of V are formed by byte permutes.  Rows are cut into `splits` parts
 // for the SMs, whose sums a second kernel joins; the warps of a block join theirs in shared memory.
-template <int DB, bool F16>
+template <int DB, bool F16, bool EIGHT>
 __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeParams p) {
+  constexpr int HALVES = EIGHT ? 1 : 2;  // of the sixteen rows
   using T = typename std::conditional<F16, __half, __nv_bfloat16>::type;
   pdl_begin();
   const flare_cache_args_t& a = p.a;
@@ -325,7 +338,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
   const int h0 = j * group + (blockIdx.y % p.head_groups) * kHeads, heads = min(kHeads, (j + 1) * group - h0);
   const int position = a.cached[b];
   const bool idle = position < 0 || position >= a.L;
-  __shared__ float joined[kDecodeWarps][kHeads][64 * DB + 2];
+  __shared__ float joined[kDecodeWarps][8 * HALVES][64 * DB + 2];
   const uint16_t* const new_k = reinterpret_cast<const uint16_t*>(a.new_k) + b * a.new_k_stride_b + j * a.new_k_stride_h;
   const uint16_t* const new_v = reinterpret_cast<const uint16_t*>(a.new_v) + b * a.new_v_stride_b + j * a.new_v_stride_h;
   const uint16_t* const keys = reinterpret_cast<const uint16_t*>(a.k_cache) + b * a.k_stride_b + j * a.k_stride_h;
@@ -343,25 +356,25 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
   const int per = (chunks + p.splits - 1) / p.splits, begin = split * per, end = min(chunks, begin + per);
 
   // queries: k-step s of segment g (32 columns) takes columns 8 c + 4 s .. + 3
-  uint32_t q[2 * DB][2][4];
+  uint32_t q[2 * DB][2][2 * HALVES];
 #pragma unroll
   for (int g = 0; g < 2 * DB; ++g)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {  // rows r and r + 8
+    for (int half = 0; half < HALVES; ++half) {  // rows r and r + 8
       const int h = r + half * 8, d = g * 32 + c * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (h < heads && d < a.D) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + b * a.q_stride_b + (h0 + h) * a.q_stride_h + d);
-      q[g][0][half] = v.x; q[g][0][half + 2] = v.y;
-      q[g][1][half] = v.z; q[g][1][half + 2] = v.w;
+      q[g][0][half] = v.x; q[g][0][half + HALVES] = v.y;
+      q[g][1][half] = v.z; q[g][1][half + HALVES] = v.w;
     }
   const float plain = a.scale * kLog2e, cap_in = a.cap > 0.0f ? 2.0f * kLog2e * a.scale / a.cap : 0.0f, cap_out = a.cap * kLog2e;
-  float slope[2] = {0.0f, 0.0f};
+  float slope[HALVES] = {};
   if (a.slopes != nullptr)
-    for (int half = 0; half < 2; ++half)
+    for (int half = 0; half < HALVES; ++half)
       if (r + half * 8 < heads) slope[half] = a.slopes[h0 + r + half * 8] * kLog2e;
-  float o[DB * 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  float o[DB * 8][2 * HALVES] = {}, top[HALVES], sum[HALVES] = {};
 #pragma unroll
-  for (int n = 0; n < DB * 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+  for (int half = 0; half < HALVES; ++half) top[half] = -INFINITY;
 
   for (int chunk = begin + warp; chunk < end; chunk += kDecodeWarps) {
     const int key0 = first + chunk * 16;
@@ -386,22 +399,23 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
         vr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
       }
     }
-    float s[2][4];
+    float s[2][2 * HALVES] = {};
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
       for (int g = 0; g < 2 * DB; ++g) {
-        mma16816<F16>(s[n], q[g][0], kr[n][g].x, kr[n][g].y);
-        mma16816<F16>(s[n], q[g][1], kr[n][g].z, kr[n][g].w);
+        mma16816<F16, EIGHT>(s[n], q[g][0], kr[n][g].x, kr[n][g].y);
+        mma16816<F16, EIGHT>(s[n], q[g][1], kr[n][g].z, kr[n][g].w);
       }
     }
     // s[n][2 half + i]: head r + 8 half, key key0 + 8 n + 2 c + i
-    float most[2] = {-INFINITY, -INFINITY};
+    float most[HALVES];
+#pragma unroll
+    for (int half = 0; half < HALVES; ++half) most[half] = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2 * HALVES; ++e) {
         const int key = key0 + n * 8 + 2 * c + (e & 1);
         float x = s[n][e];
         if (a.cap > 0.0f) x = fmaf(-2.0f * cap_out, __fdividef(1.0f, exp2f(x * cap_in) + 1.0f), cap_out);
@@ -410,48 +424,51 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
         s[n][e] = key <= position ? x : -INFINITY;
         most[e >> 1] = fmaxf(most[e >> 1], s[n][e]);
       }
-    float scale[2];
+    float scale[HALVES], frame[HALVES];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < HALVES; ++half) {
       most[half] = fmaxf(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
       most[half] = fmaxf(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
       const float to = fmaxf(top[half], most[half]);
       scale[half] = top[half] == -INFINITY ? 0.0f : exp2f(top[half] - to);
       top[half] = to;
       sum[half] *= scale[half];
+      frame[half] = to == -INFINITY ? 0.0f : to;
     }
-    const float frame[2] = {top[0] == -INFINITY ? 0.0f : top[0], top[1] == -INFINITY ? 0.0f : top[1]};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2 * HALVES; ++e) {
         s[n][e] = exp2f(s[n][e] - frame[e >> 1]);
         sum[e >> 1] += s[n][e];
       }
-    const uint32_t w[4] = {pack_pair<T>(s[0][0], s[0][1]), pack_pair<T>(s[0][2], s[0][3]), pack_pair<T>(s[1][0], s[1][1]),
-                           pack_pair<T>(s[1][2], s[1][3])};
+    uint32_t w[2 * HALVES];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int half = 0; half < HALVES; ++half) w[n * HALVES + half] = pack_pair<T>(s[n][2 * half], s[n][2 * half + 1]);
 #pragma unroll
     for (int g = 0; g < DB; ++g) {
       const uint32_t v0[4] = {vr[0][g].x, vr[0][g].y, vr[0][g].z, vr[0][g].w}, v1[4] = {vr[1][g].x, vr[1][g].y, vr[1][g].z, vr[1][g].w};
       const uint32_t v2[4] = {vr[2][g].x, vr[2][g].y, vr[2][g].z, vr[2][g].w}, v3[4] = {vr[3][g].x, vr[3][g].y, vr[3][g].z, vr[3][g].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float(&acc)[4] = o[g * 8 + e];
-        acc[0] *= scale[0]; acc[1] *= scale[0];
-        acc[2] *= scale[1]; acc[3] *= scale[1];
+        float(&acc)[2 * HALVES] = o[g * 8 + e];
+#pragma unroll
+        for (int i = 0; i < 2 * HALVES; ++i) acc[i] *= scale[i >> 1];
         const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-        mma16816<F16>(acc, w, __byte_perm(v0[e >> 1], v1[e >> 1], sel), __byte_perm(v2[e >> 1], v3[e >> 1], sel));
+        mma16816<F16, EIGHT>(acc, w, __byte_perm(v0[e >> 1], v1[e >> 1], sel), __byte_perm(v2[e >> 1], v3[e >> 1], sel));
       }
     }
   }
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < HALVES; ++half) {
     sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 1);
     sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 2);
   }
   // o[g * 8 + e][2 half + i]: head r + 8 half, column 64 g + 8 (2 c + i) + e
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < HALVES; ++half) {
     float* const row = joined[warp][r + half * 8];
 #pragma unroll
     for (int n = 0; n < DB * 8; ++n)
@@ -617,8 +634,11 @@ int flare_attention_decode(const flare_cache_args_t* args, flare_stream_t stream
     p.part = reinterpret_cast<float*>(a.workspace);
   }
   if ((int64_t)a.J * p.head_groups > 65535) return FLARE_ERR_UNSUPPORTED;
-  auto* const kernel = a.D <= 64 ? (a.dtype == FLARE_F16 ? decode_kernel<1, true> : decode_kernel<1, false>)
-                                 : (a.dtype == FLARE_F16 ? decode_kernel<2, true> : decode_kernel<2, false>);
+  const bool f16 = a.dtype == FLARE_F16, eight = a.H / a.J <= 8;
+  auto* const kernel = a.D <= 64 ? (eight ? (f16 ? decode_kernel<1, true, true> : decode_kernel<1, false, true>)
+                                          : (f16 ? decode_kernel<1, true, false> : decode_kernel<1, false, false>))
+                                 : (eight ? (f16 ? decode_kernel<2, true, true> : decode_kernel<2, false, true>)
+                                          : (f16 ? decode_kernel<2, true, false> : decode_kernel<2, false, false>));
   {
     LaunchTimer timer("attention_decode_kernel", stream);
     FLARE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)p.splits, (unsigned)(a.J * p.head_groups), (unsigned)a.B), dim3(32 * kDecodeWarps), 0, stream, p));

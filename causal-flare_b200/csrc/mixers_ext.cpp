@@ -132,6 +132,7 @@ bool whole(const py::object& o, const Tensor& x, at::IntArrayRef sizes, Tensor* 
 }
 Tensor rows(const Tensor& t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor aligned(const Tensor& t) { return t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? reinterpret_cast<T*>(t.data_ptr()) : nullptr; }
@@ -321,7 +322,7 @@ struct ScanHeld {
   Tensor x, dt, A, B, C, D, z, bias;
 };
 ScanHeld fill_scan(flare_scan_args_t& a, const ScanInputs& s) {
-  ScanHeld h{rows(s.x), rows(s.dt), dense(s.A), rows(s.B), rows(s.C), dense(s.D), rows(s.z), dense(s.bias)};
+  ScanHeld h{rows(s.x), rows(s.dt), aligned(s.A), rows(s.B), rows(s.C), dense(s.D), rows(s.z), dense(s.bias)};
   memset(&a, 0, sizeof(a));
   const bool tokens = h.x.dim() == 3;
   a.x = h.x.data_ptr(); a.dt = h.dt.data_ptr(); a.z = ptr(h.z); a.b = h.B.data_ptr(); a.c = h.C.data_ptr();

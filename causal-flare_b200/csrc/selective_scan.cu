@@ -197,6 +197,7 @@ __device__ __forceinline__ void load_bc(const float (*p)[4], uint64_t (&b)[P], u
   }
 }
 
+__device__ __forceinline__ uint64_t twice(float x) { return f2_pack(x, x); }
 __device__ __forceinline__ uint64_t factor(uint64_t a2, uint64_t delta2) {
   float lo, hi;
   f2_unpack(f2_mul(a2, delta2), lo, hi);
@@ -611,56 +612,88 @@ __global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p
   }
 }
 
-// One token.  Bound by memory: every state is read and written once, 16 bytes of it by a thread.
+// One token.  Bound by memory: every state is read and written once.  Four threads share four channels (eight apart, so that a warp's
+// loads are contiguous): each prepares one of them (softplus, gate) and holds a quarter of the states of all four, for several rows of the
+// batch one after the other, whose A is read once.
 template <typename T, int NS>
-__global__ void __launch_bounds__(256) decode_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(256) decode_kernel(const ScanParams p, int rows) {
   pdl_begin();
-  constexpr int kLanes = 4, S = NS * kLanes;
+  constexpr int S = NS * 4, P = NS / 2;
   const flare_scan_args_t& a = p.a;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t channel = idx / kLanes;
-  if (channel >= (int64_t)a.B * a.C) return;  // (whole groups of four lanes)
-  const int64_t b = channel / a.C;
-  const int c = (int)(channel - b * a.C), sub = threadIdx.x & 3, group = c / p.channels;
-  float* state = a.state_out + channel * S + sub * NS;
-  uint64_t h[NS / 2], acc = 0;
-  load_pairs<NS / 2>(state, h);
-  const float x = to_float<T>(reinterpret_cast<const T*>(a.x)[b * a.x_stride_b + c]);
-  float delta = to_float<T>(reinterpret_cast<const T*>(a.dt)[b * a.dt_stride_b + c]) + (a.dt_bias != nullptr ? a.dt_bias[c] : 0.0f);
-  float slope;
-  if (a.dt_softplus) delta = softplus(delta, slope);
-  const uint64_t d2 = f2_pack(delta, delta), x2 = f2_pack(delta * x, delta * x);
-  const T* bp = reinterpret_cast<const T*>(a.b) + b * a.b_stride_b + group * a.b_stride_g + sub * NS;
-  const T* cp = reinterpret_cast<const T*>(a.c) + b * a.c_stride_b + group * a.c_stride_g + sub * NS;
-  const float* A = a.A + (int64_t)c * S + sub * NS;
+  const int lane = threadIdx.x & 31, quad = lane >> 2, sub = lane & 3;
+  const int base = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32;
+  if (base >= a.C) return;
+  const int mine = base + quad + 8 * sub;  // the channel that this thread prepares
+  const bool have = mine < a.C;
+  const float bias = have && a.dt_bias != nullptr ? a.dt_bias[mine] : 0.0f, D = have && a.D != nullptr ? a.D[mine] : 0.0f;
+  uint64_t A2[4][P];
 #pragma unroll
-  for (int i = 0; i < NS / 2; ++i) {
-    const uint64_t A2 = f2_pack(A[2 * i] * kLog2e, A[2 * i + 1] * kLog2e);
-    const uint64_t bv = f2_pack(to_float<T>(bp[2 * i]), to_float<T>(bp[2 * i + 1]));
-    const uint64_t cv = f2_pack(to_float<T>(cp[2 * i]), to_float<T>(cp[2 * i + 1]));
-    h[i] = f2_fma(factor(A2, d2), h[i], f2_mul(x2, bv));
-    acc = i ? f2_fma(h[i], cv, acc) : f2_mul(h[i], cv);
+  for (int k = 0; k < 4; ++k) {
+    const int c = min(base + quad + 8 * k, a.C - 1);
+    load_pairs<P>(a.A + (int64_t)c * S + sub * NS, A2[k]);
+#pragma unroll
+    for (int i = 0; i < P; ++i) A2[k][i] = f2_mul(A2[k][i], twice(kLog2e));
   }
-  store_pairs<NS / 2>(state, h);
-  float y = pair_sum(acc);
-  const unsigned mask = __activemask();
-  y += __shfl_xor_sync(mask, y, 1);
-  y += __shfl_xor_sync(mask, y, 2);
-  if (sub != 0) return;
-  if (a.D != nullptr) y = fmaf(a.D[c], x, y);
-  if (a.z != nullptr) {
-    const float z = to_float<T>(reinterpret_cast<const T*>(a.z)[b * a.z_stride_b + c]);
-    y *= z * sigmoid(z);
+  const int group = base / p.channels;
+  const bool one_group = min(base + 31, a.C - 1) / p.channels == group;
+  const int b_end = min(a.B, (int)(blockIdx.y + 1) * rows);
+#pragma unroll 1
+  for (int b = blockIdx.y * rows; b < b_end; ++b) {
+    float* const states = a.state_out + ((int64_t)b * a.C + base + quad) * S + sub * NS;
+    uint64_t h[4][P], bv[P], cv[P];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (base + quad + 8 * k < a.C) load_pairs<P>(states + 8 * k * S, h[k]);
+    float x = 0.0f, delta = 0.0f, z = 0.0f, slope;
+    if (have) {
+      x = to_float<T>(reinterpret_cast<const T*>(a.x)[b * a.x_stride_b + mine]);
+      delta = to_float<T>(reinterpret_cast<const T*>(a.dt)[b * a.dt_stride_b + mine]) + bias;
+      if (a.z != nullptr) z = to_float<T>(reinterpret_cast<const T*>(a.z)[b * a.z_stride_b + mine]);
+    }
+    const auto projections = [&](int g) {
+      const T* bp = reinterpret_cast<const T*>(a.b) + b * a.b_stride_b + g * a.b_stride_g + sub * NS;
+      const T* cp = reinterpret_cast<const T*>(a.c) + b * a.c_stride_b + g * a.c_stride_g + sub * NS;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        bv[i] = f2_pack(to_float<T>(bp[2 * i]), to_float<T>(bp[2 * i + 1]));
+        cv[i] = f2_pack(to_float<T>(cp[2 * i]), to_float<T>(cp[2 * i + 1]));
+      }
+    };
+    if (one_group) projections(group);
+    if (a.dt_softplus) delta = softplus(delta, slope);
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = base + quad + 8 * k;
+      const float dk = __shfl_sync(0xffffffffu, delta, quad * 4 + k), xk = __shfl_sync(0xffffffffu, x, quad * 4 + k);
+      y[k] = 0.0f;
+      if (c < a.C) {
+        if (!one_group) projections(c / p.channels);
+        uint64_t acc = 0;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          h[k][i] = f2_fma(factor(A2[k][i], twice(dk)), h[k][i], f2_mul(twice(dk * xk), bv[i]));
+          acc = i ? f2_fma(h[k][i], cv[i], acc) : f2_mul(h[k][i], cv[i]);
+        }
+        store_pairs<P>(states + 8 * k * S, h[k]);
+        y[k] = pair_sum(acc);
+      }
+    }
+    float out = fmaf(D, x, lane_sums<4>(y, sub));
+    if (a.z != nullptr) out *= z * sigmoid(z);
+    if (have) reinterpret_cast<T*>(a.y)[(int64_t)b * a.C + mine] = from_float<T>(out);
   }
-  reinterpret_cast<T*>(a.y)[channel] = from_float<T>(y);
 }
 
+// Rows of the batch that a thread takes: four, where that leaves two blocks for every SM
 template <typename T, int NS>
 int launch_decode(const ScanParams& p, cudaStream_t stream) {
-  const int64_t blocks = ((int64_t)p.a.B * p.a.C * 4 + 255) / 256;
-  if (blocks > 0x7fffffff) return FLARE_ERR_UNSUPPORTED;
+  const int64_t blocks = (p.a.C + 255) / 256;
+  int rows = 4;
+  while (rows > 1 && blocks * ((p.a.B + rows - 1) / rows) < 2 * (int64_t)sm_count()) rows /= 2;
+  while ((p.a.B + rows - 1) / rows > 65535) rows *= 2;
   LaunchTimer timer("scan_decode_kernel", stream);
-  FLARE_CUDA_CHECK(launch_pdl(decode_kernel<T, NS>, dim3((unsigned)blocks), dim3(256), 0, stream, p));
+  FLARE_CUDA_CHECK(launch_pdl(decode_kernel<T, NS>, dim3((unsigned)blocks, (unsigned)((p.a.B + rows - 1) / rows)), dim3(256), 0, stream, p, rows));
   return FLARE_OK;
 }
 
@@ -762,7 +795,7 @@ int check(const flare_scan_args_t* args) {
   if (a.dtype < 0 || a.dtype > 2) return FLARE_ERR_BAD_DTYPE;
   if (a.N > 0x7fffffff - 1024 || (int64_t)a.G * ((a.C / a.G + 31) / 32) > 65535) return FLARE_ERR_UNSUPPORTED;
   if (a.x == nullptr || a.dt == nullptr || a.A == nullptr || a.b == nullptr || a.c == nullptr) return FLARE_ERR_BAD_POINTER;
-  for (const void* q : {(const void*)a.state_in, (const void*)a.state_out, (const void*)a.keep})
+  for (const void* q : {(const void*)a.A, (const void*)a.state_in, (const void*)a.state_out, (const void*)a.keep})
     if (reinterpret_cast<uintptr_t>(q) & 15u) return FLARE_ERR_BAD_POINTER;
   return FLARE_OK;
 }

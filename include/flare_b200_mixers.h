@@ -67,7 +67,7 @@ typedef struct flare_scan_args {
   const void* z;            /* [B, N, C] or NULL: no gate */
   const void* b;            /* [B, N, G, S] */
   const void* c;            /* [B, N, G, S] */
-  const float* A;           /* [C, S] contiguous */
+  const float* A;           /* [C, S] contiguous, 16-byte aligned like the states */
   const float* D;           /* [C] or NULL */
   const float* dt_bias;     /* [C] or NULL */
   const int32_t* documents; /* [B, N] contiguous or NULL */

@@ -321,6 +321,24 @@ def test_strided_inputs(dtype):
         assert torch.equal(a, c)
 
 
+def test_weights_at_odd_addresses():
+    g = gen(14)
+    t = scan_inputs(g, 2, 40, 24, 16, 1, torch.float32)
+    w, b = randn(g, 24, 4), randn(g, 24)
+
+    def shifted(v):
+        s = torch.zeros(v.numel() + 1, device="cuda", dtype=v.dtype)
+        s[1:] = v.flatten()
+        return s[1:].view(v.shape)
+
+    moved = {k: (shifted(v) if k in ("A", "D", "dt_bias") else v) for k, v in t.items()}
+    assert torch.equal(cf.flare_selective_scan(**moved, dt_softplus=True), cf.flare_selective_scan(**t, dt_softplus=True))
+    one = lambda t: {k: (v[:, 0] if k in ("x", "dt", "z", "B", "C") else v) for k, v in t.items()}  # noqa: E731
+    for a, c in zip(cf.flare_selective_scan_decode(**one(moved), dt_softplus=True), cf.flare_selective_scan_decode(**one(t), dt_softplus=True)):
+        assert torch.equal(a, c)
+    assert torch.equal(cf.flare_causal_conv(t["x"], shifted(w), shifted(b)), cf.flare_causal_conv(t["x"], w, b))
+
+
 def test_same_bits_on_another_stream_and_from_a_graph():
     g = gen(13)
     t = scan_inputs(g, 1, 600, 64, 16, 1, torch.bfloat16)
