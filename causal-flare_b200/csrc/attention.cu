@@ -376,70 +376,114 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
 #pragma unroll
   for (int half = 0; half < HALVES; ++half) top[half] = -INFINITY;
 
+  // The keys of the chunk after this one are fetched as soon as this one's have met the queries, the values as soon as this one's
+  // have met the weights: both are on their way all the time, in the registers that they leave.
+  uint4 kr[2][2 * DB], vr[4][DB];
+  const int64_t last_row = position - 1;  // of the cache
+  const auto fetch_keys = [&](int chunk) {
+    const int key0 = first + chunk * 16;
+    if (key0 + 16 <= position && a.D == 64 * DB) {  // (whole chunks of the cache need no look at every piece)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint16_t* row = keys + (int64_t)(key0 + n * 8 + r) * a.k_stride_n + c * 8;
+#pragma unroll
+        for (int g = 0; g < 2 * DB; ++g) kr[n][g] = load_streaming(reinterpret_cast<const uint4*>(row + g * 32));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = key0 + n * 8 + r;
+        const uint16_t* row = key < position ? keys + min((int64_t)key, last_row) * a.k_stride_n : new_k;
+#pragma unroll
+        for (int g = 0; g < 2 * DB; ++g) {
+          const int d = g * 32 + c * 8;
+          kr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+  };
+  const auto fetch_values = [&](int chunk) {
+    const int key0 = first + chunk * 16;
+    if (key0 + 16 <= position && a.D == 64 * DB) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint16_t* row = values + (int64_t)(key0 + 2 * c + (n & 1) + (n >> 1) * 8) * a.v_stride_n + r * 8;
+#pragma unroll
+        for (int g = 0; g < DB; ++g) vr[n][g] = load_streaming(reinterpret_cast<const uint4*>(row + g * 64));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int key = key0 + 2 * c + (n & 1) + (n >> 1) * 8;
+        const uint16_t* row = key < position ? values + min((int64_t)key, last_row) * a.v_stride_n : new_v;
+#pragma unroll
+        for (int g = 0; g < DB; ++g) {
+          const int d = g * 64 + r * 8;
+          vr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+  };
+  if (begin + warp < end) {
+    fetch_keys(begin + warp);
+    fetch_values(begin + warp);
+  }
+#pragma unroll 1
   for (int chunk = begin + warp; chunk < end; chunk += kDecodeWarps) {
     const int key0 = first + chunk * 16;
-    uint4 kr[2][2 * DB], vr[4][DB];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int key = key0 + n * 8 + r;
-      const uint16_t* row = key < position ? keys + key * a.k_stride_n : new_k;
-#pragma unroll
-      for (int g = 0; g < 2 * DB; ++g) {
-        const int d = g * 32 + c * 8;
-        kr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int key = key0 + 2 * c + (n & 1) + (n >> 1) * 8;
-      const uint16_t* row = key < position ? values + key * a.v_stride_n : new_v;
-#pragma unroll
-      for (int g = 0; g < DB; ++g) {
-        const int d = g * 64 + r * 8;
-        vr[n][g] = key <= position && d < a.D ? load_streaming(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
-      }
-    }
     float s[2][2 * HALVES] = {};
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int g = 0; g < 2 * DB; ++g)
 #pragma unroll
-      for (int g = 0; g < 2 * DB; ++g) {
+      for (int n = 0; n < 2; ++n) {
         mma16816<F16, EIGHT>(s[n], q[g][0], kr[n][g].x, kr[n][g].y);
         mma16816<F16, EIGHT>(s[n], q[g][1], kr[n][g].z, kr[n][g].w);
       }
-    }
+    if (chunk + kDecodeWarps < end) fetch_keys(chunk + kDecodeWarps);
     // s[n][2 half + i]: head r + 8 half, key key0 + 8 n + 2 c + i
     float most[HALVES];
 #pragma unroll
     for (int half = 0; half < HALVES; ++half) most[half] = -INFINITY;
+    const bool whole = key0 + 15 <= position;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * HALVES; ++e) {
         const int key = key0 + n * 8 + 2 * c + (e & 1);
         float x = s[n][e];
-        if (a.cap > 0.0f) x = fmaf(-2.0f * cap_out, __fdividef(1.0f, exp2f(x * cap_in) + 1.0f), cap_out);
+        if (a.cap > 0.0f) x = fmaf(-2.0f * cap_out, sm100::rcp_approx(sm100::ex2_approx(x * cap_in) + 1.0f), cap_out);
         else x *= plain;
         x = fmaf(-slope[e >> 1], (float)(position - key), x);
-        s[n][e] = key <= position ? x : -INFINITY;
+        s[n][e] = whole || key <= position ? x : -INFINITY;
         most[e >> 1] = fmaxf(most[e >> 1], s[n][e]);
       }
-    float scale[HALVES], frame[HALVES];
+    // the frame moves only where the maximum has grown by more than 2^8 (it cancels in the quotient)
+    bool grow = false;
 #pragma unroll
     for (int half = 0; half < HALVES; ++half) {
       most[half] = fmaxf(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
       most[half] = fmaxf(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
-      const float to = fmaxf(top[half], most[half]);
-      scale[half] = top[half] == -INFINITY ? 0.0f : exp2f(top[half] - to);
-      top[half] = to;
-      sum[half] *= scale[half];
-      frame[half] = to == -INFINITY ? 0.0f : to;
+      grow |= most[half] > top[half] + 8.0f || (top[half] == -INFINITY && most[half] > top[half]);
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int half = 0; half < HALVES; ++half) {
+        const float to = fmaxf(top[half], most[half]);
+        const float scale = top[half] == -INFINITY ? 0.0f : exp2f(top[half] - to);
+        top[half] = to;
+        sum[half] *= scale;
+#pragma unroll
+        for (int n = 0; n < DB * 8; ++n) {
+          o[n][2 * half] *= scale;
+          o[n][2 * half + 1] *= scale;
+        }
+      }
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * HALVES; ++e) {
-        s[n][e] = exp2f(s[n][e] - frame[e >> 1]);
+        s[n][e] = sm100::ex2_approx(s[n][e] - (top[e >> 1] == -INFINITY ? 0.0f : top[e >> 1]));
         sum[e >> 1] += s[n][e];
       }
     uint32_t w[2 * HALVES];
@@ -453,13 +497,11 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
       const uint32_t v2[4] = {vr[2][g].x, vr[2][g].y, vr[2][g].z, vr[2][g].w}, v3[4] = {vr[3][g].x, vr[3][g].y, vr[3][g].z, vr[3][g].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float(&acc)[2 * HALVES] = o[g * 8 + e];
-#pragma unroll
-        for (int i = 0; i < 2 * HALVES; ++i) acc[i] *= scale[i >> 1];
         const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-        mma16816<F16, EIGHT>(acc, w, __byte_perm(v0[e >> 1], v1[e >> 1], sel), __byte_perm(v2[e >> 1], v3[e >> 1], sel));
+        mma16816<F16, EIGHT>(o[g * 8 + e], w, __byte_perm(v0[e >> 1], v1[e >> 1], sel), __byte_perm(v2[e >> 1], v3[e >> 1], sel));
       }
     }
+    if (chunk + kDecodeWarps < end) fetch_values(chunk + kDecodeWarps);
   }
 #pragma unroll
   for (int half = 0; half < HALVES; ++half) {
