@@ -34,21 +34,23 @@ using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int S_, int NS_, int THREADS_>
+template <int S_, int NS_, int THREADS_, int BLOCKS_ = 1, int SUB_ = 8>
 struct Config {
+  static constexpr int BLOCKS = BLOCKS_;  // of an SM, at least
+  static constexpr int SUB = SUB_;        // tokens that the backward recomputes at a time
   static constexpr int S = S_, NS = NS_, THREADS = THREADS_, P = NS / 2, LANES = S / NS, CH = THREADS / LANES, WARPS = THREADS / 32;
   static constexpr int V = kTile * CH / THREADS;   // neighbouring channels of a token that a thread stages
   static constexpr int PER = CH / V;               // threads of a token, staging
   static constexpr int BC = kTile * S / THREADS;   // elements of b and of c that a thread stages
   static constexpr int ROW = CH + 32 / LANES;      // rows of one value per channel: neither staging nor walking asks a bank twice
-  static constexpr int ROW2 = CH + CH / 16 * 2;    // rows of two, see padded()
+  static constexpr int ROW4 = CH + CH / 8;         // rows of four, see padded()
   static_assert(kTile * CH % THREADS == 0 && (V == 4 || V == 8) && kTile * S % THREADS == 0 && NS % 2 == 0, "tile");
 };
-__device__ __forceinline__ int padded(int c) { return c + 2 * (c >> 4); }
+__device__ __forceinline__ int padded(int c) { return c + (c >> 3); }
 
 template <typename K>
 struct Tile {
-  alignas(16) float2 dd[kTile][K::ROW2];       // delta, delta x
+  alignas(16) float4 dd[kTile][K::ROW4];       // delta, delta x, each twice: as the packed products take them
   alignas(16) float bc[kTile][K::S / 2][4];    // b, c of a pair of states
   int reset[kTile];
 };
@@ -63,7 +65,7 @@ struct BackwardSmem {
   float gy[kTile][K::ROW];
   float p1[kTile][K::ROW], p2[kTile][K::ROW], y[kTile][K::ROW];
   float bc[kTile][K::WARPS][2 * K::S];
-  alignas(16) float starts[kTile / 8][K::THREADS][K::NS];  // (each thread its own)
+  alignas(16) float starts[kTile / K::SUB][K::THREADS][K::NS];  // (each thread its own)
 };
 
 // softplus(u) = max(u, 0) + log(1 + t), t = exp(-|u|), and its slope 1 / (1 + exp(-u)).  log(1 + t) = 2 atanh(s) with s = t / (2 + t) <= 1 / 3: the
@@ -150,10 +152,9 @@ struct Rows {
       if (p.a.dt_softplus) delta[i] = softplus(delta[i], slope[i]);
       if (!on) delta[i] = 0.0f;
     }
-    float4* const row = reinterpret_cast<float4*>(&to.dd[at.token][padded(at.cg)]);
+    float4* const row = &to.dd[at.token][padded(at.cg)];
 #pragma unroll
-    for (int i = 0; i < K::V / 2; ++i)
-      row[i] = make_float4(delta[2 * i], delta[2 * i] * xf[2 * i], delta[2 * i + 1], delta[2 * i + 1] * xf[2 * i + 1]);
+    for (int i = 0; i < K::V; ++i) row[i] = make_float4(delta[i], delta[i], delta[i] * xf[i], delta[i] * xf[i]);
 #pragma unroll
     for (int i = 0; i < K::BC; ++i) {
       const int idx = threadIdx.x + i * K::THREADS, s = idx % K::S;
@@ -203,6 +204,11 @@ __device__ __forceinline__ uint64_t factor(uint64_t a2, uint64_t delta2) {
   f2_unpack(f2_mul(a2, delta2), lo, hi);
   return f2_pack(ex2_approx(lo), ex2_approx(hi));
 }
+__device__ __forceinline__ float low(uint64_t v) {
+  float lo, hi;
+  f2_unpack(v, lo, hi);
+  return lo;
+}
 __device__ __forceinline__ float pair_sum(uint64_t v) {
   float lo, hi;
   f2_unpack(v, lo, hi);
@@ -249,8 +255,8 @@ __device__ __forceinline__ int channel_sums(float (&v)[M], int lane) {
   return mine ? first : -1;
 }
 
-template <typename T, typename K, bool ENDS, bool WIDE>
-__global__ void __launch_bounds__(K::THREADS) forward_kernel(const ScanParams p) {
+template <typename T, typename K, bool ENDS, bool WIDE, bool DOCS>
+__global__ void __launch_bounds__(K::THREADS, K::BLOCKS) forward_kernel(const ScanParams p) {
   pdl_wait();
   extern __shared__ __align__(16) uint8_t smem[];
   ForwardSmem<K>& sm = *reinterpret_cast<ForwardSmem<K>*>(smem);
@@ -282,7 +288,6 @@ __global__ void __launch_bounds__(K::THREADS) forward_kernel(const ScanParams p)
   }
   const T* const zp = reinterpret_cast<const T*>(a.z);
   const int tiles = (a.N + kTile - 1) / kTile;
-  const bool docs = at.ids != nullptr;
   Rows<T, K, WIDE> rows;
   Raw<T, V> z;  // of the rows in `rows`
   const auto fetch = [&](int t0) {
@@ -317,16 +322,16 @@ __global__ void __launch_bounds__(K::THREADS) forward_kernel(const ScanParams p)
       float v[STEP];
 #pragma unroll
       for (int k = 0; k < STEP; ++k) {
-        if (docs && in.reset[t + k]) {
+        if (DOCS && in.reset[t + k]) {
 #pragma unroll
           for (int i = 0; i < P; ++i) h[i] = 0;
           if (ENDS) sum = -INFINITY;
         }
-        const float2 dd = in.dd[t + k][padded(at.ch)];
-        const uint64_t d2 = f2_pack(dd.x, dd.x), x2 = f2_pack(dd.y, dd.y);
+        const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t + k][padded(at.ch)]);
+        const uint64_t d2 = dd.x, x2 = dd.y;
         uint64_t b[P], c[P], acc = 0;
         load_bc<P>(&in.bc[t + k][at.sub * P], b, c);
-        if (ENDS) sum += dd.x;
+        if (ENDS) sum += low(d2);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           h[i] = f2_fma(factor(A2[i], d2), h[i], f2_mul(x2, b[i]));
@@ -373,15 +378,15 @@ __global__ void __launch_bounds__(K::THREADS) forward_kernel(const ScanParams p)
   }
 }
 
-template <typename T, typename K, bool ENDS, bool WIDE>
-__global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p) {
+template <typename T, typename K, bool ENDS, bool WIDE, bool DOCS>
+__global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const ScanParams p) {
   pdl_wait();
   extern __shared__ __align__(16) uint8_t smem[];
   BackwardSmem<K>& sm = *reinterpret_cast<BackwardSmem<K>*>(smem);
   const flare_scan_args_t& a = p.a;
   const Place<K> at(p);
   if (ENDS && at.seg == 0) return;
-  constexpr int S = K::S, P = K::P, NS = K::NS, V = K::V, LANES = K::LANES, SUB = 8;
+  constexpr int S = K::S, P = K::P, NS = K::NS, V = K::V, LANES = K::LANES, SUB = K::SUB;
   float bias[V], D[V], sum_d[V], sum_bias[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -403,7 +408,6 @@ __global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p
   if (!ENDS && p.segments > 1) load_pairs<P>(p.carry + carry_at, G);
   const T* const zp = reinterpret_cast<const T*>(a.z);
   const int tiles = (a.N + kTile - 1) / kTile;
-  const bool docs = at.ids != nullptr;
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
   Rows<T, K, WIDE> rows;
   Raw<T, V> dy, z;
@@ -444,15 +448,13 @@ __global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p
     if (ENDS) {
 #pragma unroll 4
       for (int t = kTile - 1; t >= 0; --t) {
-        const float2 dd = sm.in.dd[t][padded(at.ch)];
-        const float gys = sm.gy[t][at.ch];
-        const uint64_t d2 = f2_pack(dd.x, dd.x), gy = f2_pack(gys, gys);
+        const uint64_t d2 = *reinterpret_cast<const uint64_t*>(&sm.in.dd[t][padded(at.ch)]), gy = twice(sm.gy[t][at.ch]);
         uint64_t b[P], c[P];
         load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
-        sum += dd.x;
+        sum += low(d2);
 #pragma unroll
         for (int i = 0; i < P; ++i) G[i] = f2_mul(f2_fma(c[i], gy, G[i]), factor(A2[i], d2));
-        if (docs && sm.in.reset[t]) {
+        if (DOCS && sm.in.reset[t]) {
 #pragma unroll
           for (int i = 0; i < P; ++i) G[i] = 0;
           sum = -INFINITY;
@@ -460,12 +462,12 @@ __global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p
       }
     } else {
       const auto move = [&](int t, uint64_t (&f)[P], uint64_t (&before)[P]) {  // h over token t; its factors; what they multiply
-        if (docs && sm.in.reset[t]) {
+        if (DOCS && sm.in.reset[t]) {
 #pragma unroll
           for (int i = 0; i < P; ++i) h[i] = 0;
         }
-        const float2 dd = sm.in.dd[t][padded(at.ch)];
-        const uint64_t d2 = f2_pack(dd.x, dd.x), x2 = f2_pack(dd.y, dd.y);
+        const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch)]);
+        const uint64_t d2 = dd.x, x2 = dd.y;
         uint64_t b[P], c[P];
         load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
 #pragma unroll
@@ -498,9 +500,8 @@ __global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p
 #pragma unroll
           for (int k = LANES - 1; k >= 0; --k) {
             const int t = q * SUB + k0 + k;
-            const float2 dd = sm.in.dd[t][padded(at.ch)];
-            const float gys = sm.gy[t][at.ch];
-            const uint64_t d2 = f2_pack(dd.x, dd.x), x2 = f2_pack(dd.y, dd.y), gy = f2_pack(gys, gys);
+            const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch)]);
+            const uint64_t d2 = dd.x, x2 = dd.y, gy = twice(sm.gy[t][at.ch]);
             uint64_t b[P], c[P], s1 = 0, s2 = 0, s3 = 0;
             load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
             float v[2 * NS];
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(K::THREADS) backward_kernel(const ScanParams p
               f2_unpack(f2_mul(g, x2), v[2 * i], v[2 * i + 1]);
               f2_unpack(f2_mul(now, gy), v[NS + 2 * i], v[NS + 2 * i + 1]);
             }
-            if (docs && sm.in.reset[t]) {
+            if (DOCS && sm.in.reset[t]) {
 #pragma unroll
               for (int i = 0; i < P; ++i) G[i] = 0;
             }
@@ -701,13 +702,14 @@ template <typename T, typename K, bool BACKWARD>
 int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
   using Smem = typename std::conditional<BACKWARD, BackwardSmem<K>, ForwardSmem<K>>::type;
   static_assert(sizeof(Smem) <= (size_t)kMaxDynamicSmem, "shared memory");
-  void (*kernel)(ScanParams);
-  if constexpr (BACKWARD)
-    kernel = ends ? (p.wide ? backward_kernel<T, K, true, true> : backward_kernel<T, K, true, false>)
-                  : (p.wide ? backward_kernel<T, K, false, true> : backward_kernel<T, K, false, false>);
-  else
-    kernel = ends ? (p.wide ? forward_kernel<T, K, true, true> : forward_kernel<T, K, true, false>)
-                  : (p.wide ? forward_kernel<T, K, false, true> : forward_kernel<T, K, false, false>);
+  const auto pick = [&](auto ends_, auto wide, auto docs) -> void (*)(ScanParams) {
+    constexpr bool E = decltype(ends_)::value, W = decltype(wide)::value, DOCS = decltype(docs)::value;
+    if constexpr (BACKWARD) return backward_kernel<T, K, E, W, DOCS>;
+    else return forward_kernel<T, K, E, W, DOCS>;
+  };
+  const auto with_docs = [&](auto ends_, auto wide) { return p.a.documents != nullptr ? pick(ends_, wide, std::true_type()) : pick(ends_, wide, std::false_type()); };
+  const auto with_wide = [&](auto ends_) { return p.wide ? with_docs(ends_, std::true_type()) : with_docs(ends_, std::false_type()); };
+  auto* const kernel = ends ? with_wide(std::true_type()) : with_wide(std::false_type());
   const dim3 grid((unsigned)(p.a.B * (int64_t)p.segments), (unsigned)(p.a.G * p.blocks_c));
   FLARE_CUDA_CHECK(allow_smem(kernel));
   LaunchTimer timer(BACKWARD ? (ends ? "scan_backward_kernel (ends)" : "scan_backward_kernel") : (ends ? "scan_forward_kernel (ends)" : "scan_forward_kernel"),
@@ -726,11 +728,13 @@ int launch(Pass pass, const ScanParams& p, cudaStream_t stream) {
       return p.a.S == 8 ? launch_decode<T, 2>(p, stream) : p.a.S == 16 ? launch_decode<T, 4>(p, stream) : launch_decode<T, 8>(p, stream);
     case FORWARD:
     case FORWARD_ENDS:
-      if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256>, false>(ends, p, stream);
-      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 256>, false>(ends, p, stream);
-      return launch_walk<T, Config<32, 4, 256>, false>(ends, p, stream);
+      // (16 states in fours: B=8 N=2048 C=4096 594 us, B=1 N=8191 C=2048 241; in twos, with twice the threads: 705, 332)
+      if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256, 2>, false>(ends, p, stream);
+      if (p.a.S == 16) return launch_walk<T, Config<16, 4, 256, 2>, false>(ends, p, stream);
+      return launch_walk<T, Config<32, 4, 256, 2>, false>(ends, p, stream);
     default:
       if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256>, true>(ends, p, stream);
+      // (16 states in twos, B=4 N=4096 C=2048: 1 220 us; in fours 1 235 with the registers of one block on an SM, 2 000 where two share them)
       if (p.a.S == 16) return launch_walk<T, Config<16, 2, 512>, true>(ends, p, stream);
       return launch_walk<T, Config<32, 4, 256>, true>(ends, p, stream);
   }
@@ -750,7 +754,7 @@ using namespace mixer;
 // (the configurations of launch() below)
 }  // namespace
 
-Shape shape_of(int S, bool backward) { return S == 8 ? Shape{4, 256} : S == 16 ? Shape{8, backward ? 512 : 256} : Shape{8, 256}; }
+Shape shape_of(int S, bool backward) { return S == 8 ? Shape{4, 256} : S == 16 ? (backward ? Shape{8, 512} : Shape{4, 256}) : Shape{8, 256}; }
 
 namespace {
 
