@@ -7,12 +7,13 @@
 // dP = X1 Y1^T into tensor memory, rows of the own side on the lanes; the threads turn them into P and dS, laid down over S and dP
 // as packed 16-bit values, from where the products that are summed over the walk take their A operand (dV += P Y1,
 // dK or dQ += dS Y0): neither P nor dS passes through shared memory, and no gradient is added by two CTAs (a key head's dK and dV walk its
-// query heads one after the other).  The price is S and dP twice, 14 instead of 10 products of D operations for a pair.  Two slots take every
+// query heads one after the other).  The price is S and dP twice, and dS in two
+// parts 18 instead of 10 products of D operations for a pair.  Two slots take every
 // other tile, with eight warps each (32 of the 64 columns a warp), so that one's exponentials run under the other's products.
 //
-// Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P and dS are rounded once, to the type of the
-// operands they meet (fp16: what of dS lies below 2^-14 keeps an absolute 2^-25, as the gradients themselves do); everything in front
-// of that, and the sums, is fp32.
+// Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P is rounded once, to the type of the
+// operands it meets; dS goes to its product as a rounded value and what that lost, rounded again: rounded once it made dK and dQ 1.6 times as far
+// off as their own rounding does.  Everything in front of that, and the sums, is fp32.
 #include "attention_tc.cuh"
 
 namespace flare {
@@ -56,6 +57,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
                           const __grid_constant__ CUtensorMap tm_y0, const __grid_constant__ CUtensorMap tm_y1, const AttnParams p) {
   using L = Layout<DB>;
   constexpr uint32_t T_DS = 256, T_P = 384, T_X = 384;  // (queries: no sum of P products, their two own tiles instead)
+  constexpr uint32_t LOW = KEYS ? 16 : 0;  // of the 32 columns of a half's scores: where the lower part of dS goes
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   Misc* const misc = reinterpret_cast<Misc*>(smem + L::MISC);
@@ -166,6 +168,9 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
 #pragma unroll
         for (int i = 0; i < kWalk / 16; ++i)
           mma_ts(tmem + T_DS, tmem + slot * 128 + 64 + (i >> 1) * 32 + (i & 1) * 8, mnmaj_step(mn0 + at, i), ID_SUM, i > 0 || n > 0);
+#pragma unroll
+        for (int i = 0; i < kWalk / 16; ++i)
+          mma_ts(tmem + T_DS, tmem + slot * 128 + LOW + (i >> 1) * 32 + (i & 1) * 8, mnmaj_step(mn0 + at, i), ID_SUM, 1);
         tc_commit(&misc->empty[s]);
         if (n + 1 == total) tc_commit(&misc->done);
         if (n + 2 < total) scores(n + 2);  // (behind the products that read P and dS where it goes: products run in order)
@@ -229,6 +234,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
       // 16 columns at a time, of this warp's half; packed, they take the first of the columns that they were read from
       const auto columns = [&](auto masked_) {  // (apart for tiles in full sight: a look at every pair keeps the pairs from overlapping)
         constexpr bool MASKED = decltype(masked_)::value;
+        uint32_t low[2][8];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int col0 = half * 32 + c * 16;
@@ -284,11 +290,17 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
               }
               pw[k >> 1] = pack2<F16>(w0, w1);
               dw[k >> 1] = pack2<F16>(g0, g1);
+              float h0, h1;
+              unpack2<F16>(dw[k >> 1], h0, h1);
+              low[c][k >> 1] = pack2<F16>(g0 - h0, g1 - h1);
             }
           }
           if (KEYS) tmem_st8(ts + c * 8, pw);
           tmem_st8(td + c * 8, dw);
         }
+        // what dS lost in that rounding, behind P (which all scores of this half have been read from by now)
+        tmem_st8(ts + LOW, low[0]);
+        tmem_st8(ts + LOW + 8, low[1]);
       };
       if (all) columns(std::false_type());
       else columns(std::true_type());

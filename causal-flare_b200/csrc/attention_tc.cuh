@@ -69,6 +69,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return F16 ? pack_f16(lo, hi) : pack_bf16(lo, hi);
 }
 template <bool F16>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if (F16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  } else {
+    lo = bf16_lo(w);
+    hi = bf16_hi(w);
+  }
+}
+template <bool F16>
 constexpr uint32_t make_idesc(int M, int N, int a_mn, int b_mn) {
   return F16 ? make_idesc_f16(M, N, a_mn, b_mn) : make_idesc_bf16(M, N, a_mn, b_mn);
 }
