@@ -194,33 +194,62 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
       tmem_fence_regs(s[1]);
       const bool full = __all_sync(0xffffffffu, keys.x <= key0 && keys.y >= key0 + kKeys) != 0;
       const int from = keys.x - key0, to_ = keys.y - key0;
-      if (CAP) {
-        if (!full) {  // (what lies out of sight does not choose the form)
+      // Weights are formed in the frame so far, caps and biases on the way, the maximum behind them: only where it has grown too far (a
+      // few of the first tiles) are they formed once more.  So no exponential waits for the maximum, and caps, biases and exponentials,
+      // which have pipes of their own, are worked on side by side.  Not so the first tile, and what needs masks or the other form of caps.
+      const float unit = BIAS ? 1.0f : sc.unit, d0 = (float)(position - key0);
+      uint32_t w[2][16];
+      float part[4], t4[4];
+      const auto weights = [&](auto raw_) {  // raw: the scores are products still
+        constexpr bool RAW = decltype(raw_)::value;
+        const uint64_t frame2 = twice(m == -INFINITY ? 0.0f : -m), unit2 = twice(unit);
+        uint64_t sum2[2] = {0, 0};
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0u;
+          for (int k = 0; k < 16; ++k) {
+            const int col = c * 32 + 2 * k;
+            uint64_t x = f2_pack(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
+            float lo, hi;
+            if (RAW && (CAP || BIAS)) {
+              if (CAP) x = series(x);
+              if (BIAS) x = f2_fma(twice(-sc.slope), f2_pack(fabsf(d0 - (float)col), fabsf(d0 - (float)(col + 1))), f2_mul(x, twice(sc.unit)));
+              f2_unpack(x, lo, hi);
+              s[c][2 * k] = __float_as_uint(lo);
+              s[c][2 * k + 1] = __float_as_uint(hi);
+            }
+            f2_unpack(BIAS ? f2_add(x, frame2) : f2_fma(x, unit2, frame2), lo, hi);
+            lo = ex2_approx(lo);
+            hi = ex2_approx(hi);
+            sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(lo, hi));
+            w[c][k] = pack2<F16>(lo, hi);
+          }
+        f2_unpack(sum2[0], part[0], part[1]);
+        f2_unpack(sum2[1], part[2], part[3]);
+      };
+      const bool at_once = n > 0 && full && (!CAP || all_small(s[0], s[1], sc.in));
+      if (at_once) {
+        weights(std::true_type());
+      } else {
+        if (CAP) {
+          if (!full) {  // (what lies out of sight does not choose the form)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0u;
+          }
+          cap_scores(s[0], series, sc.in);
+          cap_scores(s[1], series, sc.in);
         }
-        cap_scores(s[0], series, sc.in);
-        cap_scores(s[1], series, sc.in);
-      }
-      if (BIAS) {
-        const float d0 = (float)(position - key0);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            s[c][k] = __float_as_uint(fmaf(-sc.slope, fabsf(d0 - (float)(c * 32 + k)), __uint_as_float(s[c][k]) * sc.unit));
-      }
-      if (!full) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
+          for (int k = 0; k < 32; ++k) {
+            if (BIAS) s[c][k] = __float_as_uint(fmaf(-sc.slope, fabsf(d0 - (float)(c * 32 + k)), __uint_as_float(s[c][k]) * sc.unit));
             if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0xff800000u;  // -inf
+          }
       }
-      float t4[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const uint32_t* const v = s[c >> 1] + (c & 1) * 16;
@@ -228,18 +257,14 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
 #pragma unroll
         for (int k = 2; k < 16; k += 2) t4[c] = fmax3(t4[c], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
       }
-      const float unit = BIAS ? 1.0f : sc.unit;
       const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * unit;
-      const bool grow = top > m + kGrowth || (m == -INFINITY && top > m);
-      if (n == 0) {
-        if (grow) m = top;
-      } else if (__any_sync(0xffffffffu, grow)) {
+      const bool grow = top > m + kGrowth || (m == -INFINITY && top > m), any = __any_sync(0xffffffffu, grow);
+      if (any && n > 0) {
         // O is at rest once the product of the tile before is done.  (That of the one before it is: these scores were issued behind it,
         // so the barrier is in this phase or through with it.)
         if (!(ok = wait(&misc->o_free[g], (n - 1) & 1))) break;
         tc_fence_after_sync();
         const float f = grow ? ex2_approx(m - top) : 1.0f;
-        if (grow) m = top;
         sum *= f;
 #pragma unroll 1
         for (int c = 0; c < 2 * DB; ++c) {
@@ -250,31 +275,14 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
           tmem_st32(to + c * 32, o);
         }
       }
-      const float frame = m == -INFINITY ? 0.0f : m;
-      const uint64_t unit2 = twice(unit), frame2 = twice(-frame);
-      uint64_t sum2[2] = {0, 0};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint64_t x = f2_pack(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1]));
-          float lo, hi;
-          f2_unpack(BIAS ? f2_add(x, frame2) : f2_fma(x, unit2, frame2), lo, hi);
-          lo = ex2_approx(lo);
-          hi = ex2_approx(hi);
-          sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(lo, hi));
-          w[k] = pack2<F16>(lo, hi);
-        }
-        tmem_st16(tp + c * 16, w);
-      }
+      if (grow) m = top;
+      if (any || !at_once) weights(std::false_type());
+      tmem_st16(tp, w[0]);
+      tmem_st16(tp + 16, w[1]);
       tmem_wait_st();
       tc_fence_before_sync();
       warp_arrive(&misc->p_ready[g][n & 1], lane);
-      float a0, a1, a2, a3;
-      f2_unpack(sum2[0], a0, a1);
-      f2_unpack(sum2[1], a2, a3);
-      sum += (a0 + a1) + (a2 + a3);
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
     }
     if (ok && tiles[g] > 0) ok = wait(&misc->o_done[g], 0);
     if (ok) {

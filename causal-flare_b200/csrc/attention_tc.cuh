@@ -37,24 +37,35 @@ struct CapSeries {
     c[2] = twice(0.13283318281173706f * in * q * q);
     c[3] = twice(-0.04837666451931f * in * q * q * q);
   }
+  __device__ __forceinline__ uint64_t operator()(uint64_t x) const {
+    const uint64_t q = f2_mul(x, x);
+    uint64_t t = f2_fma(q, c[3], c[2]);
+    t = f2_fma(q, t, c[1]);
+    return f2_mul(x, f2_fma(q, t, c[0]));
+  }
 };
 __device__ __forceinline__ float tanh_any(float x) { return fmaf(-2.0f, rcp_approx(ex2_approx(x * (2.0f * kLog2e)) + 1.0f), 1.0f); }
+
+template <int N>
+__device__ __forceinline__ float largest(const uint32_t (&s)[N]) {
+  float most = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; k += 2) most = fmax3(most, fabsf(__uint_as_float(s[k])), fabsf(__uint_as_float(s[k + 1])));
+  return most;
+}
+// may the whole warp's raw products take the polynomial?
+__device__ __forceinline__ bool all_small(const uint32_t (&a)[32], const uint32_t (&b)[32], float in) {
+  return __all_sync(0xffffffffu, fmaxf(largest(a), largest(b)) * in <= 0.35f) != 0;
+}
 
 // raw products, in place: tanh of the capped score.  Whole warp.
 template <int N>
 __device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const CapSeries& series, float in) {
-  float most = 0.0f;
-#pragma unroll
-  for (int k = 0; k < N; k += 2) most = fmax3(most, fabsf(__uint_as_float(s[k])), fabsf(__uint_as_float(s[k + 1])));
-  if (__all_sync(0xffffffffu, most * in <= 0.35f)) {
+  if (__all_sync(0xffffffffu, largest(s) * in <= 0.35f)) {
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
-      const uint64_t x = f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), q = f2_mul(x, x);
-      uint64_t t = f2_fma(q, series.c[3], series.c[2]);
-      t = f2_fma(q, t, series.c[1]);
-      t = f2_fma(q, t, series.c[0]);
       float lo, hi;
-      f2_unpack(f2_mul(x, t), lo, hi);
+      f2_unpack(series(f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1]))), lo, hi);
       s[k] = __float_as_uint(lo);
       s[k + 1] = __float_as_uint(hi);
     }
