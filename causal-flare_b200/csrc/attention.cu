@@ -141,26 +141,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     hi = __reduce_max_sync(0xffffffffu, hi);
     if (lane == 0) p.query_span[(int64_t)b * (Nqp / 128) + t] = hi > lo ? make_int2(lo, hi) : make_int2(0, 0);
   }
-  // tiles of 128 keys: the first query whose keys end behind the tile's first, and the first whose keys begin behind its last
-  for (int t = tid; t < p.m.Nkp / 128; t += kPlanThreads) {
-    int2 s = make_int2(0, 0);
-    if (p.m.cached == nullptr) {
-      int a = 0, z = p.Nq;
-      while (a < z) {
-        const int mid = (a + z) / 2;
-        if (range[mid].y > t * 128) z = mid;
-        else a = mid + 1;
-      }
-      s.x = a;
-      z = p.Nq;
-      while (a < z) {
-        const int mid = (a + z) / 2;
-        if (range[mid].x >= t * 128 + 128) z = mid;
-        else a = mid + 1;
-      }
-      s.y = a;
+  // tiles of 128 keys: the first query whose keys end behind the tile's first, and the first whose keys begin behind its last.  Both
+  // ends grow with the query, so every tile's two queries are where an end passes the tile: each query looks at the one before it.
+  int2* const key_span = p.key_span + (int64_t)b * (p.m.Nkp / 128);
+  for (int t = tid; t < p.m.Nkp / 128; t += kPlanThreads) key_span[t] = p.m.cached == nullptr ? make_int2(p.Nq, p.Nq) : make_int2(0, 0);
+  __syncthreads();
+  if (p.m.cached == nullptr) {
+    for (int i = tid; i < p.Nq; i += kPlanThreads) {
+      const int2 r = range[i], before = i > 0 ? range[i - 1] : make_int2(0, 0);
+      for (int t = (before.y + 127) / 128; t * 128 < r.y; ++t) key_span[t].x = i;
+      for (int t = before.x / 128; t * 128 + 128 <= r.x; ++t) key_span[t].y = i;
     }
-    p.key_span[(int64_t)b * (p.m.Nkp / 128) + t] = s;
   }
   for (int t = tid >> 5; t < p.m.Nkp / 64; t += kPlanThreads / 32) {
     bool bad = false;
@@ -174,26 +165,27 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   }
 }
 
-// -delta = -<dy, y>, half a warp per row and head; 0 for queries without keys (their dy may hold anything)
-template <typename T>
+// -delta = -<dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  Bound by memory.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) delta_kernel(const AttnParams p, const T* dy, int64_t sb, int64_t sn, int64_t sh, float* delta) {
   pdl_begin();
-  const int lane = threadIdx.x & 15;
-  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, total = (int64_t)p.B * p.masks.Nqp * p.H;
-  const bool live = idx < total;
-  const int64_t row = live ? idx / p.H : 0;
-  const int h = live ? (int)(idx - row * p.H) : 0, b = (int)(row / p.masks.Nqp), i = (int)(row - (int64_t)b * p.masks.Nqp);
-  const int2 r = p.masks.range[(int64_t)b * p.masks.Nqp + i];
+  const int lane = threadIdx.x % LANES, b = blockIdx.y;
+  const unsigned idx = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int i = (int)(idx / (unsigned)p.H), h = (int)(idx % (unsigned)p.H);
+  const bool live = i < p.masks.Nqp;
   float sum = 0.0f;
-  if (live && i < p.Nq && r.y > r.x && lane * 8 < p.D) {
-    float a[8], c[8];
-    unpack8(load_raw8<T>(dy + b * sb + i * sn + h * sh + lane * 8, 8, true), a);
-    unpack8(load_raw8<T>(reinterpret_cast<const T*>(p.y) + (((int64_t)b * p.Nq + i) * p.H + h) * p.D + lane * 8, 8, true), c);
+  if (live && i < p.Nq && lane * 8 < p.D) {
+    const int2 r = p.masks.range[(int64_t)b * p.masks.Nqp + i];
+    if (r.y > r.x) {
+      float a[8], c[8];
+      unpack8(load_raw8<T>(dy + b * sb + i * sn + h * sh + lane * 8, 8, true), a);
+      unpack8(load_raw8<T>(reinterpret_cast<const T*>(p.y) + (((int64_t)b * p.Nq + i) * p.H + h) * p.D + lane * 8, 8, true), c);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum = fmaf(a[k], c[k], sum);
+      for (int k = 0; k < 8; ++k) sum = fmaf(a[k], c[k], sum);
+    }
   }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (live && lane == 0) delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = -sum;
 }
 
@@ -637,16 +629,18 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   if (const int rc = begin(a, l, p, stream)) return rc;
   float* const delta = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.workspace) + l.delta);
   p.delta = delta;
-  const int64_t blocks = ((int64_t)a.B * l.Nqp * a.H * 16 + 255) / 256;
-  if (blocks > INT_MAX) return FLARE_ERR_UNSUPPORTED;
+  const int lanes = a.D <= 64 ? 8 : 16;
+  const int64_t blocks = ((int64_t)l.Nqp * a.H * lanes + 255) / 256;
+  if (blocks * (256 / lanes) > UINT_MAX - 256 || a.B > 65535) return FLARE_ERR_UNSUPPORTED;
   {
     LaunchTimer timer("attention_delta_kernel", stream);
-    if (a.dtype == FLARE_F16)
-      FLARE_CUDA_CHECK(launch_pdl(delta_kernel<__half>, dim3((unsigned)blocks), dim3(256), 0, stream, p, reinterpret_cast<const __half*>(a.dy),
-                                  a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, delta));
-    else
-      FLARE_CUDA_CHECK(launch_pdl(delta_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, stream, p,
-                                  reinterpret_cast<const __nv_bfloat16*>(a.dy), a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, delta));
+    const dim3 grid((unsigned)blocks, (unsigned)a.B);
+    const auto run = [&](auto t, auto* kernel) {
+      using T = decltype(t);
+      return launch_pdl(kernel, grid, dim3(256), 0, stream, p, reinterpret_cast<const T*>(a.dy), a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, delta);
+    };
+    if (a.dtype == FLARE_F16) FLARE_CUDA_CHECK(run(__half(), lanes == 8 ? delta_kernel<__half, 8> : delta_kernel<__half, 16>));
+    else FLARE_CUDA_CHECK(run(__nv_bfloat16(), lanes == 8 ? delta_kernel<__nv_bfloat16, 8> : delta_kernel<__nv_bfloat16, 16>));
   }
   return launch_backward_tc(a, p, stream);
 }
