@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) forward_kernel(const Sc
   if (at.channel < 0) return;
   if (ENDS) {
     store_pairs<P>(p.carry + carry_at, h);
-    if (at.sub == 0) p.decay[(int64_t)blockIdx.x * a.C + at.channel] = sum < 0.0f ? -1.0f : sum;
+    if (at.sub == 0) p.decay[(int64_t)blockIdx.x * a.C + at.channel] = sum;
   } else if (a.state_out != nullptr && at.seg == p.segments - 1) {
     store_pairs<P>(a.state_out + state_at, h);
   }
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
         }
       }
     } else {
-      const auto move = [&](int t, uint64_t (&f)[P], uint64_t (&before)[P]) {  // h over token t; its factors; what they multiply
+      const auto move = [&](int t, uint64_t (&f)[P]) {  // h over token t; its factors
         if (DOCS && sm.in.reset[t]) {
 #pragma unroll
           for (int i = 0; i < P; ++i) h[i] = 0;
@@ -473,7 +473,6 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           f[i] = factor(A2[i], d2);
-          before[i] = h[i];
           h[i] = f2_fma(f[i], h[i], f2_mul(x2, b[i]));
         }
       };
@@ -483,17 +482,23 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
         if (q + 1 < kTile / SUB) {
 #pragma unroll
           for (int k = 0; k < SUB; ++k) {
-            uint64_t f[P], before[P];
-            move(q * SUB + k, f, before);
+            uint64_t f[P];
+            move(q * SUB + k, f);
           }
         }
       }
 #pragma unroll 1
       for (int q = kTile / SUB - 1; q >= 0; --q) {
-        uint64_t f[SUB][P], before[SUB][P];
-        load_pairs<P>(sm.starts[q][threadIdx.x], h);
+        uint64_t f[SUB][P], behind[SUB][P], start[P];  // factors; states behind the tokens and in front of them all
+        load_pairs<P>(sm.starts[q][threadIdx.x], start);
 #pragma unroll
-        for (int k = 0; k < SUB; ++k) move(q * SUB + k, f[k], before[k]);
+        for (int i = 0; i < P; ++i) h[i] = start[i];
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) {
+          move(q * SUB + k, f[k]);
+#pragma unroll
+          for (int i = 0; i < P; ++i) behind[k][i] = h[i];
+        }
 #pragma unroll
         for (int k0 = SUB - LANES; k0 >= 0; k0 -= LANES) {
           float p1[LANES], p2[LANES], yv[LANES];
@@ -508,14 +513,13 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               const uint64_t g = f2_fma(c[i], gy, G[i]);
-              const uint64_t moved = f2_mul(f[k0 + k][i], before[k0 + k][i]);
-              const uint64_t now = f2_fma(x2, b[i], moved);
-              const uint64_t u = f2_mul(g, moved);
+              const uint64_t before = DOCS && sm.in.reset[t] ? 0 : k0 + k ? behind[k0 + k - 1][i] : start[i], now = behind[k0 + k][i];
+              const uint64_t next = f2_mul(g, f[k0 + k][i]), u = f2_mul(next, before);
               s1 = i ? f2_fma(g, b[i], s1) : f2_mul(g, b[i]);
               s2 = i ? f2_fma(u, A2[i], s2) : f2_mul(u, A2[i]);
               s3 = i ? f2_fma(now, c[i], s3) : f2_mul(now, c[i]);
               tile_dA[i] = f2_fma(u, d2, tile_dA[i]);
-              G[i] = f2_mul(g, f[k0 + k][i]);
+              G[i] = next;
               f2_unpack(f2_mul(g, x2), v[2 * i], v[2 * i + 1]);
               f2_unpack(f2_mul(now, gy), v[NS + 2 * i], v[NS + 2 * i + 1]);
             }
@@ -588,7 +592,7 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
   if (ENDS) {
     if (at.channel >= 0) {
       store_pairs<P>(p.carry + carry_at, G);
-      if (at.sub == 0) p.decay[(int64_t)blockIdx.x * a.C + at.channel] = sum < 0.0f ? -1.0f : sum;
+      if (at.sub == 0) p.decay[(int64_t)blockIdx.x * a.C + at.channel] = sum;
     }
     return;
   }
@@ -773,7 +777,7 @@ __global__ void __launch_bounds__(256) join_kernel(const ScanParams p) {
     const bool ends = k + 1 < p.segments;  // (of the one behind which nothing follows there is no end)
     const float end = ends ? p.carry[at * per + cs] : 0.0f, sum = ends ? p.decay[at * a.C + c] : 0.0f;
     p.carry[at * per + cs] = in;
-    in = sum < 0.0f ? end : fmaf(expf(A * sum), in, end);
+    in = sum == -INFINITY ? end : fmaf(expf(A * sum), in, end);
   }
 }
 

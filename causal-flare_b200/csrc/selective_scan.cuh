@@ -22,8 +22,8 @@ struct ScanParams {
   int channels;   // of a group
   int blocks_c;   // blocks along a group's channels (of the kernels at hand: forward and backward differ)
   int segments, seg_tokens;  // tokens of a row are cut into segments of whole tiles
-  // of every segment: what it leaves behind from zero, then (after the join) what it starts from; the sum of its deltas, -1: a
-  // document begins in it
+  // of every segment: what it leaves behind from zero, then (after the join) what it starts from; the sum of its deltas,
+  // -infinity: a document begins in it
   float* carry;      // [B][segments][C][S]
   float* decay;      // [B][segments][C]
   float* partial_bc; // [B][N][G * blocks_c][2 S]

@@ -199,6 +199,23 @@ def test_scan_without_softplus_and_positive_exponents():
     close(cf.flare_selective_scan(**t), want, magnitudes(t)[0], 40, "y")
 
 
+def test_scan_of_negative_time_steps():
+    # without softplus a time step is what it is, also where its sum over a part of a long row is negative
+    g = gen(6)
+    t = scan_inputs(g, 1, 900, 16, 16, 1, torch.float32, True, False, False)
+    t["dt"] = randn(g, 1, 900, 16) * 0.02 - 0.01
+    t["A"] = randn(g, 16, 16) * 0.2
+    for v in t.values():
+        v.requires_grad_()
+    y = cf.flare_selective_scan(**t)
+    got = torch.autograd.grad(y.sum(), list(t.values()))
+    ex = {k: v.detach().double().requires_grad_() for k, v in t.items()}
+    want = orc.selective_scan(**ex)[0]
+    near(y, want.detach(), torch.float32, 900, "y")
+    for name, a, b in zip(t, got, torch.autograd.grad(want.sum(), list(ex.values()))):
+        near(a, b, torch.float32, 900, name)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(3, 41, 24, 16, 1), (2, 500, 16, 8, 2), (2, 300, 37, 32, 1)], ids=str)
 def test_scan_prompt_and_tokens_continue_one_another(dtype, shape):
