@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch import autograd
 
 from . import _lib
 
@@ -160,7 +161,23 @@ def whole_numbers(name: str, what: str, t, shape):
     if t.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
         raise ValueError(f"{name} expects {what} of an integer type. Got {t.dtype}.")
     has_shape(name, what, t, shape)
+    if t.dtype == torch.int64:
+        t = _narrow_ids(t) if what == "documents" else t.clamp(-1, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
+
+
+def _narrow_ids(t):
+    """Ids of 64 bits need not fit 32: documents are numbered anew, in the order of their runs."""
+    new = torch.zeros(t.shape, dtype=torch.int32, device=t.device)
+    torch.cumsum(t[:, 1:] != t[:, :-1], 1, dtype=torch.int32, out=new[:, 1:])
+    return new.masked_fill_(t < 0, -1)
+
+
+def written(*tensors) -> None:
+    """What a kernel wrote in place has a new version: autograd notices graphs that hold the old one."""
+    for t in tensors:
+        if not t.is_inference():
+            autograd.graph.increment_version(t)
 
 
 def rows(t):

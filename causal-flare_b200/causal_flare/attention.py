@@ -5,7 +5,7 @@ single tokens on it (``flare_causal_attention_decode``).  Tensors are [B, N, hea
 share J key / value heads (head h reads h // (H // J)).  No counterpart in the operator API this package mirrors.
 
 The score of the query at position i for the key at position j is ``cap * tanh(scale * <q, k> / cap) - slopes[h] * |i - j|`` (without
-``cap``: ``scale * <q, k>``), and i sees the keys j <= i, subject to
+``cap``: ``scale * <q, k>``; a cap is at most 1024), and i sees the keys j <= i, subject to
 
 * ``documents`` [B, N]: an id per token.  A document is a run of equal ids, and tokens see their own document only.  A negative id marks
   padding: it sees nothing and nobody sees it, output and gradients are 0.
@@ -45,6 +45,8 @@ def _attention_args(name, q, k, v, scale, cap, slopes, window, tokens):
         raise ValueError(f"{name} expects a positive scale. Got {scale}.")
     if cap is not None and not (0.0 < float(cap) < float("inf")):
         raise ValueError(f"{name} expects a positive cap. Got {cap}.")
+    if cap is not None and float(cap) > 1024:
+        raise ValueError(f"{name} supports caps up to 1024 (scores are off by up to cap * 2 ** -21). Got {cap}.")
     if window is not None and (int(window) != window or not 1 <= window):
         raise ValueError(f"{name} expects a window of at least one token. Got {window}.")
     has_shape(name, "slopes", slopes, (H,))
@@ -190,6 +192,7 @@ def flare_causal_attention_prefill(q, k, v, k_cache, v_cache, *, cached=None, le
     c = _fill_cache(kt, vt, k_cache, v_cache, cached)
     c.N, c.lengths = N, _lib.ptr(lengths)
     _mixers.run("flare_attention_append", c, q.device)
+    _mixers.written(k_cache, v_cache)
     slopes = None if slopes is None else slopes.contiguous()
     a = _fill(qt, k_cache, v_cache, how, slopes, prefix=prefix)
     a.cached, a.lengths, a.y = cached.data_ptr(), _lib.ptr(lengths), y.data_ptr()
@@ -226,4 +229,5 @@ def flare_causal_attention_decode(q, k, v, k_cache, v_cache, cached, *, scale=No
     put_strides(a, "q", q, "bh")
     a.scale, a.cap, a.window = how
     _mixers.run("flare_attention_decode", a, q.device, "flare_attention_decode_workspace_bytes")
+    _mixers.written(k_cache, v_cache)
     return y

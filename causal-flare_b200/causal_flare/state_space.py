@@ -163,6 +163,7 @@ def flare_causal_conv_decode(x, weight, bias=None, state=None, *, activation=Non
         a = _fill_conv(x, weight, bias, code)
         a.state_out, a.y = state.data_ptr(), y.data_ptr()
         _mixers.run("flare_conv_decode", a, x.device)
+        _mixers.written(state)
     return y, state
 
 
@@ -346,4 +347,5 @@ def flare_selective_scan_decode(x, dt, A, B, C, state=None, *, D=None, z=None, d
         a, held = _fill_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus)
         a.state_out, a.y = state.data_ptr(), y.data_ptr()
         _mixers.run("flare_scan_decode", a, x.device)
+        _mixers.written(state)
     return y, state

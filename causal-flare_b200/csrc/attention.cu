@@ -2,6 +2,7 @@
 #include "attention.cuh"
 
 #include <limits.h>
+#include <math.h>
 #include <string.h>
 
 #include "prefill_tc.cuh"
@@ -213,6 +214,12 @@ Layout layout(const flare_attention_args_t& a, bool backward) {
   return l;
 }
 
+// Scores and caps that fp32 holds.  Behind a cap a score is off by up to cap 2^-21: from 1024 on that would be more than the rounding of
+// the weights.
+bool bad_scores(float scale, float cap, int window) {
+  return !(scale > 0.0f) || !isfinite(scale) || !(cap >= 0.0f) || cap > 1024.0f || (cap > 0.0f && !isfinite(4.0f * scale / cap)) || window < 0;
+}
+
 bool strides_fit(const void* p, std::initializer_list<int64_t> strides) {
   if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u)) return false;
   for (int64_t s : strides)
@@ -226,7 +233,7 @@ int check(const flare_attention_args_t* args) {
   if (a.B <= 0 || a.Nq <= 0 || a.Nk <= 0 || a.H <= 0 || a.J <= 0 || a.D <= 0 || a.H % a.J) return FLARE_ERR_BAD_SHAPE;
   if (a.D % 8 || a.D > 128 || a.Nq > INT_MAX - 8192 || a.Nk > INT_MAX - 8192) return FLARE_ERR_UNSUPPORTED;
   if (a.dtype != FLARE_BF16 && a.dtype != FLARE_F16) return FLARE_ERR_BAD_DTYPE;
-  if (!(a.scale > 0.0f) || !(a.cap >= 0.0f) || a.window < 0) return FLARE_ERR_BAD_CONFIG;
+  if (bad_scores(a.scale, a.cap, a.window)) return FLARE_ERR_BAD_CONFIG;
   if (a.cached == nullptr ? a.Nk != a.Nq : a.documents != nullptr) return FLARE_ERR_BAD_CONFIG;
   if (!strides_fit(a.q, {a.q_stride_b, a.q_stride_n, a.q_stride_h}) || !strides_fit(a.k, {a.k_stride_b, a.k_stride_n, a.k_stride_h}) ||
       !strides_fit(a.v, {a.v_stride_b, a.v_stride_n, a.v_stride_h}) || !strides_fit(a.y, {}))
@@ -569,7 +576,7 @@ int check_cache(const flare_cache_args_t* args, bool decode) {
       !strides_fit(a.k_cache, {a.k_stride_b, a.k_stride_n, a.k_stride_h}) || !strides_fit(a.v_cache, {a.v_stride_b, a.v_stride_n, a.v_stride_h}))
     return FLARE_ERR_BAD_POINTER;
   if (!decode) return FLARE_OK;
-  if (!(a.scale > 0.0f) || !(a.cap >= 0.0f) || a.window < 0) return FLARE_ERR_BAD_CONFIG;
+  if (bad_scores(a.scale, a.cap, a.window)) return FLARE_ERR_BAD_CONFIG;
   if (!strides_fit(a.q, {a.q_stride_b, a.q_stride_h}) || a.y == nullptr || a.cached == nullptr) return FLARE_ERR_BAD_POINTER;
   return FLARE_OK;
 }

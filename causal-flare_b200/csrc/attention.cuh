@@ -35,7 +35,6 @@ struct AttnParams {
   float scale, cap;
 };
 
-struct TensorMaps;
 int launch_forward_tc(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream);
 int launch_backward_tc(const flare_attention_args_t& a, const AttnParams& p, cudaStream_t stream);
 

@@ -119,16 +119,28 @@ bool tensor_or_none(const py::object& o, Tensor* out) {
   *out = THPVariable_Unpack(o.ptr());
   return true;
 }
-// whole numbers as the kernels read them; false: the Python layer has to look
-bool whole(const py::object& o, const Tensor& x, at::IntArrayRef sizes, Tensor* out) {
+// Whole numbers as the kernels read them; false: the Python layer has to look.  Ids of 64 bits need not fit 32: documents are numbered anew,
+// in the order of their runs.
+bool whole(const py::object& o, const Tensor& x, at::IntArrayRef sizes, Tensor* out, bool ids = false) {
   Tensor t;
   if (!tensor_or_none(o, &t)) return false;
   if (!t.defined()) return true;
   if (!ordinary(t) || t.device() != x.device() || t.sizes() != sizes) return false;
   const auto type = t.scalar_type();
   if (type != at::kInt && type != at::kLong) return false;
-  *out = t.to(at::kInt).contiguous();
+  if (type == at::kLong && ids) {
+    const int64_t n = t.size(1) - 1;
+    Tensor runs = at::zeros(sizes, t.options().dtype(at::kInt));
+    if (n > 0) runs.narrow(1, 1, n).copy_(t.narrow(1, 1, n).ne(t.narrow(1, 0, n)).cumsum(1, at::kInt));
+    *out = runs.masked_fill_(t.lt(0), -1);
+  } else {
+    *out = (type == at::kLong ? t.clamp(-1, INT_MAX) : t).to(at::kInt).contiguous();
+  }
   return true;
+}
+// what a kernel wrote in place has a new version: autograd notices graphs that hold the old one
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 Tensor rows(const Tensor& t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
@@ -255,7 +267,7 @@ py::object conv(const Tensor& x, const Tensor& w, const py::object& bias, const 
   const int act = activation_of(activation);
   if (act < 0 || !tensor_or_none(bias, &b) || !plain_conv(x, w, b, 3)) return py::none();
   const c10::cuda::CUDAGuard guard(x.device());
-  if (!whole(documents, x, x.sizes().slice(0, 2), &ids)) return py::none();
+  if (!whole(documents, x, x.sizes().slice(0, 2), &ids, true)) return py::none();
   if (wants_grad(x, w, b)) return py::cast(ConvNode::apply(x, w, maybe(b), (int64_t)act, maybe(ids))[0]);
   return py::cast(run_conv(x, w, b, act, ids));
 }
@@ -292,6 +304,7 @@ py::object conv_decode(const Tensor& x_in, const Tensor& w, const py::object& bi
   fill_conv(a, x, wc, bc, act);
   a.state_out = st.data_ptr(); a.y = y.data_ptr();
   check(api.conv_decode(&a, stream_of(x)), "flare_conv_decode");
+  written(st);
   return py::make_tuple(y, state);
 }
 
@@ -388,7 +401,7 @@ py::object scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor
   Tensor ids;
   if (!scan_inputs(s, D, z, bias, 3)) return py::none();
   const c10::cuda::CUDAGuard guard(x.device());
-  if (!whole(documents, x, x.sizes().slice(0, 2), &ids)) return py::none();
+  if (!whole(documents, x, x.sizes().slice(0, 2), &ids, true)) return py::none();
   if (wants_grad(x, dt, A, B, C, s.D, s.z, s.bias)) return py::cast(ScanNode::apply(x, dt, A, s.B, s.C, maybe(s.D), maybe(s.z), maybe(s.bias), softplus, maybe(ids))[0]);
   flare_scan_args_t a;
   const ScanHeld h = fill_scan(a, s);
@@ -434,6 +447,7 @@ py::object scan_decode(const Tensor& x_in, const Tensor& dt, const Tensor& A, co
   const Tensor y = new_like(x_in);
   a.state_out = ptr<float>(st); a.y = y.data_ptr();
   check(api.scan_decode(&a, stream_of(x_in)), "flare_scan_decode");
+  written(st);
   return py::make_tuple(y, state);
 }
 
@@ -467,7 +481,7 @@ bool score_inputs(const Tensor& q, const py::object& scale, const py::object& ca
   if (scale.is_none()) s->scale = D <= 8 ? 1.0 : std::pow((double)D, -0.5);
   else if (!number(scale, &s->scale)) return false;
   if (!(s->scale > 0.0) || std::isinf(s->scale)) return false;
-  if (!cap.is_none() && (!number(cap, &s->cap) || !(s->cap > 0.0) || std::isinf(s->cap))) return false;
+  if (!cap.is_none() && (!number(cap, &s->cap) || !(s->cap > 0.0) || s->cap > 1024.0)) return false;
   if (!window.is_none()) {
     if (!PyLong_Check(window.ptr())) return false;
     int overflow = 0;
@@ -548,7 +562,7 @@ py::object attention(const Tensor& q, const Tensor& k, const Tensor& v, const py
   Tensor ids, led;
   if (!plain_attention(q, k, v, 4) || !score_inputs(q, scale, cap, slopes, window, &s) || !truth(prefix, q, &led)) return py::none();
   const c10::cuda::CUDAGuard guard(q.device());
-  if (!whole(documents, q, q.sizes().slice(0, 2), &ids)) return py::none();
+  if (!whole(documents, q, q.sizes().slice(0, 2), &ids, true)) return py::none();
   if (wants_grad(q, k, v)) return py::cast(AttentionNode::apply(q, k, v, s.scale, s.cap, s.window, maybe(s.slopes), maybe(ids), maybe(led))[0]);
   const Tensor qt = tiled(q), kt = tiled(k), vt = tiled(v), y = new_like(q);
   flare_attention_args_t a;
@@ -593,6 +607,8 @@ py::object attention_prefill(const Tensor& q0, const Tensor& k0, const Tensor& v
   c.N = (int32_t)q.size(1);
   c.cached = ptr<int32_t>(at_); c.lengths = ptr<int32_t>(len);
   check(api.attention_append(&c, stream_of(q)), "flare_attention_append");
+  written(kc);
+  written(vc);
   flare_attention_args_t a;
   fill_attention(a, q, kc, vc, s, Tensor(), led);
   a.cached = ptr<int32_t>(at_); a.lengths = ptr<int32_t>(len); a.y = y.data_ptr();
@@ -619,6 +635,8 @@ py::object attention_decode(const Tensor& q_in, const Tensor& k_in, const Tensor
   a.scale = (float)s.scale; a.cap = (float)s.cap; a.window = (int32_t)s.window;
   const Tensor ws = workspace(a, api.attention_decode_workspace_bytes(&a), q);
   check(api.attention_decode(&a, stream_of(q)), "flare_attention_decode");
+  written(kc);
+  written(vc);
   return py::cast(y);
 }
 

@@ -751,16 +751,12 @@ extern template int launch<float>(Pass, const ScanParams&, cudaStream_t);
 extern template int launch<__nv_bfloat16>(Pass, const ScanParams&, cudaStream_t);
 extern template int launch<__half>(Pass, const ScanParams&, cudaStream_t);
 
-namespace {
-
-using namespace mixer;
-
-// (the configurations of launch() below)
-}  // namespace
-
+// (the configurations of launch() above)
 Shape shape_of(int S, bool backward) { return S == 8 ? Shape{4, 256} : S == 16 ? (backward ? Shape{8, 512} : Shape{4, 256}) : Shape{8, 256}; }
 
 namespace {
+
+using namespace mixer;
 
 // What enters a segment: what enters the one in front of it (REVERSE: behind it), decayed, plus what that one leaves behind.
 template <bool REVERSE>

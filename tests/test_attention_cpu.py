@@ -57,7 +57,7 @@ def call(fn=None, **kw):
     (dict(q=torch.randn(2, 5, 4, 64), k=torch.randn(2, 5, 2, 64), v=torch.randn(2, 5, 2, 64)), "bfloat16 and float16"),
     (dict(k=torch.randn(2, 5, 2, 64).half()), "inputs' type"),
     (dict(scale=0.0), "positive scale"), (dict(scale=float("nan")), "positive scale"),
-    (dict(cap=-1.0), "positive cap"), (dict(cap=float("inf")), "positive cap"),
+    (dict(cap=2000.0), "caps up to 1024"), (dict(cap=-1.0), "positive cap"), (dict(cap=float("inf")), "positive cap"),
     (dict(window=0), "window"), (dict(window=2.5), "window"),
     (dict(slopes=torch.rand(3)), "slopes"), (dict(slopes=torch.rand(4).half()), "slopes"),
     (dict(slopes=torch.rand(4, requires_grad=True)), "no gradient of the slopes"),
@@ -104,7 +104,7 @@ def args(**kw):
 
 @pytest.mark.parametrize("call_, kw, status", [
     ("forward", dict(H=3), 1), ("forward", dict(D=68), 2), ("forward", dict(D=192), 2), ("forward", dict(dtype=0), 5), ("forward", dict(scale=-1.0), 6),
-    ("forward", dict(cap=float("nan")), 6), ("forward", dict(window=-1), 6), ("forward", dict(Nk=65), 6), ("forward", dict(cached=0x1000, documents=0x1000), 6),
+    ("forward", dict(cap=float("nan")), 6), ("forward", dict(cap=1025.0), 6), ("forward", dict(cap=1e-40), 6), ("forward", dict(scale=float("inf")), 6), ("forward", dict(window=-1), 6), ("forward", dict(Nk=65), 6), ("forward", dict(cached=0x1000, documents=0x1000), 6),
     ("forward", dict(q=0x1008), 3), ("forward", dict(k_stride_n=260), 3), ("forward", {}, 4), ("backward", dict(cached=0x1000, Nk=100), 6),
     ("backward", dict(dy=None), 3), ("backward", dict(lse=None), 3), ("backward", {}, 4),
 ])
@@ -129,3 +129,11 @@ def cache_args(**kw):
 ])
 def test_cache_entry_points_refuse(call_, kw, status):
     assert getattr(_mixers.load(), "flare_attention_" + call_)(C.byref(cache_args(**kw)), None) == status
+
+
+def test_ids_and_positions_of_64_bits():
+    big = 1 << 32
+    ids = torch.tensor([[big, big, 2 * big, 2 * big, -big, 0, 1 << 31, -1]])
+    assert _mixers.whole_numbers("f", "documents", ids, (1, 8)).tolist() == [[0, 0, 1, 1, -1, 3, 4, -1]]
+    assert _mixers.whole_numbers("f", "documents", ids[:, :0], (1, 0)).shape == (1, 0)
+    assert _mixers.whole_numbers("f", "cached", torch.tensor([big, 5, -big]), (3,)).tolist() == [2 ** 31 - 1, 5, -1]

@@ -111,6 +111,53 @@ def test_inputs_changed_behind_the_forward_are_noticed(native, monkeypatch):
 
 
 @pytest.mark.parametrize("native", [True, False])
+def test_states_written_in_place_are_noticed(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_mixers, "_host", Nothing())
+    g = gen(5)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    conv, scan = randn(g, 2, 2, 16), randn(g, 2, 16, 8)
+    kc, vc = randn(g, 2, 9, 1, 64, dtype=torch.float16), randn(g, 2, 9, 1, 64, dtype=torch.float16)
+    x, bc, q = randn(g, 2, 16), randn(g, 2, 8), randn(g, 2, 1, 64, dtype=torch.float16)
+    at = torch.zeros(2, device="cuda", dtype=torch.int32)
+    calls_ = [lambda: cf.flare_causal_conv_decode(x, x[0, :, None].expand(16, 3), None, conv),
+              lambda: cf.flare_selective_scan_decode(x, x, -torch.ones(16, 8, device="cuda"), bc, bc, scan),
+              lambda: cf.flare_causal_attention_decode(q, q, q, kc, vc, at),
+              lambda: cf.flare_causal_attention_prefill(q[:, None], q[:, None], q[:, None], kc, vc)]
+    for call, states in zip(calls_, ((conv,), (scan,), (kc, vc), (kc, vc))):
+        for state in states:
+            graph = (w * state).sum()
+            call()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(graph, w)
+    with torch.inference_mode():
+        state = torch.zeros(2, 2, 16, device="cuda")
+        cf.flare_causal_conv_decode(x, x[0, :, None].expand(16, 3), None, state)
+    cf.flare_causal_conv_decode(x, x[0, :, None].expand(16, 3), None, state)  # (a tensor without versions)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_ids_and_positions_of_64_bits(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_mixers, "_host", Nothing())
+    g = gen(6)
+    big = 1 << 32
+    ids = torch.tensor([[7, 7, 7, 8, 8, -3, 9, 9]], device="cuda")
+    wide = ids * big  # (32 bits of these are 0)
+    x, w = randn(g, 1, 8, 16), randn(g, 16, 3)
+    assert torch.equal(cf.flare_causal_conv(x, w, documents=wide), cf.flare_causal_conv(x, w, documents=ids.int()))
+    q = randn(g, 1, 8, 2, 64, dtype=torch.float16)
+    assert torch.equal(cf.flare_causal_attention(q, q, q, documents=wide), cf.flare_causal_attention(q, q, q, documents=ids.int()))
+    one = wide[:, :1]
+    assert torch.equal(cf.flare_causal_conv(x[:, :1], w, documents=one), cf.flare_causal_conv(x[:, :1], w, documents=ids[:, :1].int()))
+    kc, vc = (torch.zeros(1, 9, 2, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+    y = cf.flare_causal_attention_decode(q[:, 0], q[:, 0], q[:, 0], kc, vc, torch.tensor([big], device="cuda"))  # behind the cache: idle
+    assert not y.any() and not kc.any()
+    y, _ = cf.flare_causal_conv_prefill(x, w, lengths=torch.tensor([big + 3], device="cuda"))  # longer than the row: all of it
+    assert torch.equal(y, cf.flare_causal_conv(x, w))
+
+
+@pytest.mark.parametrize("native", [True, False])
 def test_states_that_cannot_be_written_in_place_come_back_as_new_ones(native, monkeypatch):
     if not native:
         monkeypatch.setattr(_mixers, "_host", Nothing())
