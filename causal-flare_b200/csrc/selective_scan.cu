@@ -34,11 +34,12 @@ using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int S_, int NS_, int THREADS_, int BLOCKS_ = 1, int SUB_ = 8>
+template <int S_, int NS_, int THREADS_, int BLOCKS_ = 1, int CT_ = 1>
 struct Config {
   static constexpr int BLOCKS = BLOCKS_;  // of an SM, at least
-  static constexpr int SUB = SUB_;        // tokens that the backward recomputes at a time
-  static constexpr int S = S_, NS = NS_, THREADS = THREADS_, P = NS / 2, LANES = S / NS, CH = THREADS / LANES, WARPS = THREADS / 32;
+  static constexpr int CT = CT_;          // channels of a thread, CH / CT apart (1 in the forward)
+  static constexpr int SUB = 8;           // tokens that the backward recomputes at a time
+  static constexpr int S = S_, NS = NS_, THREADS = THREADS_, P = NS / 2, LANES = S / NS, CH = THREADS / LANES * CT, APART = CH / CT, WARPS = THREADS / 32;
   static constexpr int V = kTile * CH / THREADS;   // neighbouring channels of a token that a thread stages
   static constexpr int PER = CH / V;               // threads of a token, staging
   static constexpr int BC = kTile * S / THREADS;   // elements of b and of c that a thread stages
@@ -65,7 +66,7 @@ struct BackwardSmem {
   float gy[kTile][K::ROW];
   float p1[kTile][K::ROW], p2[kTile][K::ROW], y[kTile][K::ROW];
   float bc[kTile][K::WARPS][2 * K::S];
-  alignas(16) float starts[kTile / K::SUB][K::THREADS][K::NS];  // (each thread its own)
+  alignas(16) float starts[kTile / K::SUB][K::THREADS][K::CT * K::NS];  // (each thread its own)
 };
 
 // softplus(u) = max(u, 0) + log(1 + t), t = exp(-|u|), and its slope 1 / (1 + exp(-u)).  log(1 + t) = 2 atanh(s) with s = t / (2 + t) <= 1 / 3: the
@@ -86,7 +87,7 @@ __device__ __forceinline__ float softplus(float u, float& slope) {
 template <typename K>
 struct Place {
   int b, seg, t0, t1, len;   // tokens of the segment
-  int group, c0;             // first channel of the block
+  int group, c0, here;       // first channel of the block, how many it has
   int token, cg, count;      // staging: token of the tile, first of V channels, how many of them there are
   int ch, sub, channel;      // walking: channel of the block, part of its states, channel (-1: none)
   const int32_t* ids;
@@ -100,7 +101,7 @@ struct Place {
     group = blockIdx.y / p.blocks_c;
     const int in_group = (blockIdx.y % p.blocks_c) * K::CH;
     c0 = group * p.channels + in_group;
-    const int here = min(K::CH, p.channels - in_group);
+    here = min(K::CH, p.channels - in_group);
     token = threadIdx.x / K::PER;
     cg = threadIdx.x % K::PER * K::V;
     count = max(0, min(K::V, here - cg));
@@ -199,9 +200,13 @@ __device__ __forceinline__ void load_bc(const float (*p)[4], uint64_t (&b)[P], u
 }
 
 __device__ __forceinline__ uint64_t twice(float x) { return f2_pack(x, x); }
+// exp(delta A).  ex2.approx is low by 0.4 units in the last place on average (over arguments from -0.5 to 0 its error has mean -2.1e-8 and
+// deviation 3.3e-8, measured against 64 bits), which adds up over the tokens that a state remembers: a shift of the argument takes the mean
+// away.  (A factor of 1 stays 1: 2^shift is nearer to it than to its neighbour.)
+constexpr float kShift = 3.3e-8f;
 __device__ __forceinline__ uint64_t factor(uint64_t a2, uint64_t delta2) {
   float lo, hi;
-  f2_unpack(f2_mul(a2, delta2), lo, hi);
+  f2_unpack(f2_fma(a2, delta2, f2_pack(kShift, kShift)), lo, hi);
   return f2_pack(ex2_approx(lo), ex2_approx(hi));
 }
 __device__ __forceinline__ float low(uint64_t v) {
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
   const flare_scan_args_t& a = p.a;
   const Place<K> at(p);
   if (ENDS && at.seg == 0) return;
-  constexpr int S = K::S, P = K::P, NS = K::NS, V = K::V, LANES = K::LANES, SUB = K::SUB;
+  constexpr int S = K::S, P = K::P, NS = K::NS, V = K::V, LANES = K::LANES, SUB = K::SUB, CT = K::CT, APART = K::APART;
   float bias[V], D[V], sum_d[V], sum_bias[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -395,29 +400,37 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
     D[i] = i < at.count && a.D != nullptr ? a.D[c] : 0.0f;
     sum_d[i] = sum_bias[i] = 0.0f;
   }
-  uint64_t A2[P], G[P], dA[P];  // G: gradient of the state behind the token at hand, times that token's successor's factor
-  const int64_t weight_at = (int64_t)max(at.channel, 0) * S + at.sub * NS;
-  const int64_t carry_at = (int64_t)blockIdx.x * a.C * S + weight_at;
-  float sum = 0.0f;
+  // of channel ch + j APART.  G: gradient of the state behind the token at hand, times that token's successor's factor
+  uint64_t A2[CT][P], G[CT][P], dA[CT][P];
+  const auto there = [&](int j) { return at.ch + j * APART < at.here; };
+  const auto weight_at = [&](int j) { return (int64_t)(at.c0 + (there(j) ? at.ch + j * APART : 0)) * S + at.sub * NS; };
+  const int64_t carry_at = (int64_t)blockIdx.x * a.C * S;
+  float sum[CT] = {};
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const float* A = a.A + weight_at + 2 * i;
-    A2[i] = f2_pack(A[0] * kLog2e, A[1] * kLog2e);
-    G[i] = dA[i] = 0;
-  }
-  if (!ENDS && p.segments > 1) load_pairs<P>(p.carry + carry_at, G);
+  for (int j = 0; j < CT; ++j)
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float* A = a.A + weight_at(j) + 2 * i;
+      A2[j][i] = f2_pack(A[0] * kLog2e, A[1] * kLog2e);
+      G[j][i] = dA[j][i] = 0;
+    }
+  if (!ENDS && p.segments > 1)
+    for (int j = 0; j < CT; ++j) load_pairs<P>(p.carry + carry_at + weight_at(j), G[j]);
   const T* const zp = reinterpret_cast<const T*>(a.z);
   const int tiles = (a.N + kTile - 1) / kTile;
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
   Rows<T, K, WIDE> rows;
   Raw<T, V> dy, z;
-  uint64_t kept[P];
+  uint64_t kept[CT][P];
   const auto fetch = [&](int t0) {
     rows.load(p, at, t0);
     const int t = t0 + at.token, n = rows.on ? at.count : 0;
     dy = load_raw<T, V>(reinterpret_cast<const T*>(a.dy) + at.b * a.dy_stride_b + t * a.dy_stride_n + at.c0 + at.cg, n, WIDE);
     if (zp != nullptr) z = load_raw<T, V>(zp + at.b * a.z_stride_b + t * a.z_stride_n + at.c0 + at.cg, n, WIDE);
-    if (!ENDS) load_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at, kept);
+    if (!ENDS) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) load_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at(j), kept[j]);
+    }
   };
   fetch(last);
 #pragma unroll 1
@@ -437,99 +450,127 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
 #pragma unroll
       for (int i = 0; i < V; ++i) sm.gy[at.token][at.cg + i] = on ? g[i] : 0.0f;
     }
-    uint64_t h[P], tile_dA[P];  // (summed tile by tile: thousands of tokens one by one would lose digits)
+    uint64_t h[CT][P], tile_dA[CT][P];  // (summed tile by tile: thousands of tokens one by one would lose digits)
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      h[i] = kept[i];
-      tile_dA[i] = 0;
-    }
+    for (int j = 0; j < CT; ++j)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        h[j][i] = kept[j][i];
+        tile_dA[j][i] = 0;
+      }
     __syncthreads();
     if (t0 > at.t0) fetch(t0 - kTile);
     if (ENDS) {
 #pragma unroll 4
       for (int t = kTile - 1; t >= 0; --t) {
-        const uint64_t d2 = *reinterpret_cast<const uint64_t*>(&sm.in.dd[t][padded(at.ch)]), gy = twice(sm.gy[t][at.ch]);
         uint64_t b[P], c[P];
         load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
-        sum += low(d2);
 #pragma unroll
-        for (int i = 0; i < P; ++i) G[i] = f2_mul(f2_fma(c[i], gy, G[i]), factor(A2[i], d2));
+        for (int j = 0; j < CT; ++j) {
+          const uint64_t d2 = *reinterpret_cast<const uint64_t*>(&sm.in.dd[t][padded(at.ch + j * APART)]), gy = twice(sm.gy[t][at.ch + j * APART]);
+          sum[j] += low(d2);
+#pragma unroll
+          for (int i = 0; i < P; ++i) G[j][i] = f2_mul(f2_fma(c[i], gy, G[j][i]), factor(A2[j][i], d2));
+        }
         if (DOCS && sm.in.reset[t]) {
 #pragma unroll
-          for (int i = 0; i < P; ++i) G[i] = 0;
-          sum = -INFINITY;
+          for (int j = 0; j < CT; ++j) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) G[j][i] = 0;
+            sum[j] = -INFINITY;
+          }
         }
       }
     } else {
-      const auto move = [&](int t, uint64_t (&f)[P]) {  // h over token t; its factors
+      const auto move = [&](int t, uint64_t (&f)[CT][P]) {  // h over token t; its factors
         if (DOCS && sm.in.reset[t]) {
 #pragma unroll
-          for (int i = 0; i < P; ++i) h[i] = 0;
+          for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int i = 0; i < P; ++i) h[j][i] = 0;
         }
-        const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch)]);
-        const uint64_t d2 = dd.x, x2 = dd.y;
         uint64_t b[P], c[P];
         load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          f[i] = factor(A2[i], d2);
-          h[i] = f2_fma(f[i], h[i], f2_mul(x2, b[i]));
+        for (int j = 0; j < CT; ++j) {
+          const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch + j * APART)]);
+          const uint64_t d2 = dd.x, x2 = dd.y;
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            f[j][i] = factor(A2[j][i], d2);
+            h[j][i] = f2_fma(f[j][i], h[j][i], f2_mul(x2, b[i]));
+          }
         }
       };
 #pragma unroll 1
       for (int q = 0; q < kTile / SUB; ++q) {
-        store_pairs<P>(sm.starts[q][threadIdx.x], h);
+#pragma unroll
+        for (int j = 0; j < CT; ++j) store_pairs<P>(&sm.starts[q][threadIdx.x][j * NS], h[j]);
         if (q + 1 < kTile / SUB) {
 #pragma unroll
           for (int k = 0; k < SUB; ++k) {
-            uint64_t f[P];
+            uint64_t f[CT][P];
             move(q * SUB + k, f);
           }
         }
       }
 #pragma unroll 1
       for (int q = kTile / SUB - 1; q >= 0; --q) {
-        uint64_t f[SUB][P], behind[SUB][P], start[P];  // factors; states behind the tokens and in front of them all
-        load_pairs<P>(sm.starts[q][threadIdx.x], start);
+        uint64_t f[SUB][CT][P], behind[SUB][CT][P], start[CT][P];  // factors; states behind the tokens and in front of them all
 #pragma unroll
-        for (int i = 0; i < P; ++i) h[i] = start[i];
+        for (int j = 0; j < CT; ++j) {
+          load_pairs<P>(&sm.starts[q][threadIdx.x][j * NS], start[j]);
+#pragma unroll
+          for (int i = 0; i < P; ++i) h[j][i] = start[j][i];
+        }
 #pragma unroll
         for (int k = 0; k < SUB; ++k) {
           move(q * SUB + k, f[k]);
 #pragma unroll
-          for (int i = 0; i < P; ++i) behind[k][i] = h[i];
+          for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int i = 0; i < P; ++i) behind[k][j][i] = h[j][i];
         }
 #pragma unroll
         for (int k0 = SUB - LANES; k0 >= 0; k0 -= LANES) {
-          float p1[LANES], p2[LANES], yv[LANES];
+          float p1[CT][LANES], p2[CT][LANES], yv[CT][LANES];
 #pragma unroll
           for (int k = LANES - 1; k >= 0; --k) {
             const int t = q * SUB + k0 + k;
-            const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch)]);
-            const uint64_t d2 = dd.x, x2 = dd.y, gy = twice(sm.gy[t][at.ch]);
-            uint64_t b[P], c[P], s1 = 0, s2 = 0, s3 = 0;
+            uint64_t b[P], c[P], db[P], dc[P];
             load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
+#pragma unroll
+            for (int j = 0; j < CT; ++j) {
+              const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch + j * APART)]);
+              const uint64_t d2 = dd.x, x2 = dd.y, gy = twice(sm.gy[t][at.ch + j * APART]);
+              uint64_t s1 = 0, s2 = 0, s3 = 0;
+#pragma unroll
+              for (int i = 0; i < P; ++i) {
+                const uint64_t g = f2_fma(c[i], gy, G[j][i]);
+                const uint64_t before = DOCS && sm.in.reset[t] ? 0 : k0 + k ? behind[k0 + k - 1][j][i] : start[j][i], now = behind[k0 + k][j][i];
+                const uint64_t next = f2_mul(g, f[k0 + k][j][i]), u = f2_mul(next, before);
+                s1 = i ? f2_fma(g, b[i], s1) : f2_mul(g, b[i]);
+                s2 = i ? f2_fma(u, A2[j][i], s2) : f2_mul(u, A2[j][i]);
+                s3 = i ? f2_fma(now, c[i], s3) : f2_mul(now, c[i]);
+                tile_dA[j][i] = f2_fma(u, d2, tile_dA[j][i]);
+                G[j][i] = next;
+                db[i] = j ? f2_fma(g, x2, db[i]) : f2_mul(g, x2);
+                dc[i] = j ? f2_fma(now, gy, dc[i]) : f2_mul(now, gy);
+              }
+              if (DOCS && sm.in.reset[t]) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) G[j][i] = 0;
+              }
+              p1[j][k] = pair_sum(s1);
+              p2[j][k] = pair_sum(s2);
+              yv[j][k] = pair_sum(s3);
+            }
             float v[2 * NS];
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-              const uint64_t g = f2_fma(c[i], gy, G[i]);
-              const uint64_t before = DOCS && sm.in.reset[t] ? 0 : k0 + k ? behind[k0 + k - 1][i] : start[i], now = behind[k0 + k][i];
-              const uint64_t next = f2_mul(g, f[k0 + k][i]), u = f2_mul(next, before);
-              s1 = i ? f2_fma(g, b[i], s1) : f2_mul(g, b[i]);
-              s2 = i ? f2_fma(u, A2[i], s2) : f2_mul(u, A2[i]);
-              s3 = i ? f2_fma(now, c[i], s3) : f2_mul(now, c[i]);
-              tile_dA[i] = f2_fma(u, d2, tile_dA[i]);
-              G[i] = next;
-              f2_unpack(f2_mul(g, x2), v[2 * i], v[2 * i + 1]);
-              f2_unpack(f2_mul(now, gy), v[NS + 2 * i], v[NS + 2 * i + 1]);
+              f2_unpack(db[i], v[2 * i], v[2 * i + 1]);
+              f2_unpack(dc[i], v[NS + 2 * i], v[NS + 2 * i + 1]);
             }
-            if (DOCS && sm.in.reset[t]) {
-#pragma unroll
-              for (int i = 0; i < P; ++i) G[i] = 0;
-            }
-            p1[k] = pair_sum(s1);
-            p2[k] = pair_sum(s2);
-            yv[k] = pair_sum(s3);
             // (a channel that does not exist has delta x = gy = 0: it adds nothing)
             const int first = channel_sums<2 * NS, LANES>(v, threadIdx.x & 31);
             if (first >= 0) {
@@ -542,13 +583,18 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
             }
           }
           const int t = q * SUB + k0 + at.sub;
-          sm.p1[t][at.ch] = lane_sums<LANES>(p1, at.sub);
-          sm.p2[t][at.ch] = lane_sums<LANES>(p2, at.sub);
-          if (zp != nullptr) sm.y[t][at.ch] = lane_sums<LANES>(yv, at.sub);
+#pragma unroll
+          for (int j = 0; j < CT; ++j) {
+            sm.p1[t][at.ch + j * APART] = lane_sums<LANES>(p1[j], at.sub);
+            sm.p2[t][at.ch + j * APART] = lane_sums<LANES>(p2[j], at.sub);
+            if (zp != nullptr) sm.y[t][at.ch + j * APART] = lane_sums<LANES>(yv[j], at.sub);
+          }
         }
       }
 #pragma unroll
-      for (int i = 0; i < P; ++i) dA[i] = f2_add(dA[i], tile_dA[i]);
+      for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int i = 0; i < P; ++i) dA[j][i] = f2_add(dA[j][i], tile_dA[j][i]);
     }
     __syncthreads();
     if (ENDS) continue;
@@ -590,14 +636,18 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
     }
   }
   if (ENDS) {
-    if (at.channel >= 0) {
-      store_pairs<P>(p.carry + carry_at, G);
-      if (at.sub == 0) p.decay[(int64_t)blockIdx.x * a.C + at.channel] = sum;
-    }
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+      if (there(j)) {
+        store_pairs<P>(p.carry + carry_at + weight_at(j), G[j]);
+        if (at.sub == 0) p.decay[(int64_t)blockIdx.x * a.C + at.c0 + at.ch + j * APART] = sum[j];
+      }
     return;
   }
   float* out = p.partial_w + (int64_t)blockIdx.x * weight_sums(a);
-  if (at.channel >= 0) store_pairs<P>(out + weight_at, dA);
+#pragma unroll
+  for (int j = 0; j < CT; ++j)
+    if (there(j)) store_pairs<P>(out + weight_at(j), dA[j]);
   // the sums that the staging threads hold, over the tokens of a tile
   __syncthreads();
 #pragma unroll
@@ -606,7 +656,7 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
     sm.p2[at.token][at.cg + i] = sum_bias[i];
   }
   __syncthreads();
-  if (threadIdx.x < K::CH && (int)threadIdx.x < min(K::CH, p.channels - (int)(blockIdx.y % p.blocks_c) * K::CH)) {
+  if ((int)threadIdx.x < at.here) {
     float d = 0.0f, e = 0.0f;
     for (int t = 0; t < kTile; ++t) {
       d += sm.p1[t][threadIdx.x];
@@ -739,7 +789,7 @@ int launch(Pass pass, const ScanParams& p, cudaStream_t stream) {
     default:
       if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256>, true>(ends, p, stream);
       // (16 states in twos, B=4 N=4096 C=2048: 1 220 us; in fours 1 235 with the registers of one block on an SM, 2 000 where two share them)
-      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 512>, true>(ends, p, stream);
+      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 256, 1, 2>, true>(ends, p, stream);
       return launch_walk<T, Config<32, 4, 256>, true>(ends, p, stream);
   }
 }

@@ -107,7 +107,7 @@ int flare_scan_decode(const flare_scan_args_t* args, flare_stream_t stream);
 /*
  * Causal attention of H query heads over J key / value heads (H a multiple of J, head h reads h / (H / J)) of width D (a
  * multiple of 8, at most 128), bf16 or fp16.  The score of the query at position i for the key at position j is
- *   cap tanh(scale <q, k> / cap) - slopes[h] |i - j|          (cap = 0: scale <q, k>; slopes NULL: no bias)
+ *   cap tanh(scale <q, k> / cap) - slopes[h] |i - j|          (cap = 0: scale <q, k>, at most 1024; slopes NULL: no bias)
  * and token i sees the keys j <= i of its document, with `window` > 0 only j > i - window; where `prefix` [B, N] (bytes,
  * non-zero: true) holds for the first tokens of a document, all tokens of the document see those.  Without a key in
  * sight y and all gradients are 0.
