@@ -294,11 +294,13 @@ __global__ void __launch_bounds__(256) append_kernel(const flare_cache_args_t a)
 
 struct DecodeParams {
   flare_cache_args_t a;
-  float* part;  // [splits][B][H][D + 2]: unnormalised sums, maximum (log 2), denominator; null: one split, y is written
+  float* part;  // [splits][B][H][D + 2]: unnormalised sums, maximum (log 2), denominator; null: y is written
   int splits, head_groups;
+  bool cluster;  // a row's splits form a cluster
 };
 
 constexpr int kDecodeWarps = 4, kHeads = 16;  // heads of a block: the rows of a product
+constexpr int kCluster = 8;                   // (what a cluster may have without being asked for more)
 
 // rows 8 to 15 of the product: none of them has a head (EIGHT), or they are there
 template <bool F16, bool EIGHT>
@@ -325,7 +327,8 @@ __device__ __forceinline__ void mma16816(float (&d)[EIGHT ? 2 : 4], const uint32
 // them.  A warp takes 16 keys at a time, straight from memory into the operands of m16n8k16 products: heads are the rows, so the
 // scores come out as the A operand that the product with V takes.  A thread's 16-byte piece of a key covers the contraction in an
 // order of its own (the queries are laid out in the same one); pairs of keys of V are formed by byte permutes.  Rows are cut into `splits` parts
-// for the SMs, whose sums a second kernel joins; the warps of a block join theirs in shared memory.
+// for the SMs; the warps of a block join theirs in shared memory, the blocks of a row theirs in a second kernel or, where all of them run
+// at once, as a cluster that reads one another's shared memory (plan_decode).
 template <int DB, bool F16, bool EIGHT>
 __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeParams p) {
   constexpr int HALVES = EIGHT ? 1 : 2;  // of the sixteen rows
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
   const int h0 = j * group + (blockIdx.y % p.head_groups) * kHeads, heads = min(kHeads, (j + 1) * group - h0);
   const int position = a.cached[b];
   const bool idle = position < 0 || position >= a.L;
-  __shared__ float joined[kDecodeWarps][8 * HALVES][64 * DB + 2];
+  __shared__ float joined[kDecodeWarps][8 * HALVES][64 * DB + 2], block_ends[8 * HALVES][2];
   const uint16_t* const new_k = reinterpret_cast<const uint16_t*>(a.new_k) + b * a.new_k_stride_b + j * a.new_k_stride_h;
   const uint16_t* const new_v = reinterpret_cast<const uint16_t*>(a.new_v) + b * a.new_v_stride_b + j * a.new_v_stride_h;
   const uint16_t* const keys = reinterpret_cast<const uint16_t*>(a.k_cache) + b * a.k_stride_b + j * a.k_stride_h;
@@ -534,8 +537,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
       v = fmaf(joined[w][h][d], f, v);
     }
     const int64_t row = (int64_t)b * a.H + h0 + h;
-    if (p.part == nullptr) {
+    if (p.splits == 1) {
       store1(a.y, a.dtype, row * a.D + d, idle ? 0.0f : v / l);
+    } else if (p.cluster) {
+      joined[0][h][d] = v;  // (no other thread reads this one)
+      if (d == 0) {
+        block_ends[h][0] = t;
+        block_ends[h][1] = l;
+      }
     } else {
       float* const out = p.part + ((int64_t)split * a.B * a.H + row) * (a.D + 2);
       out[d] = v;
@@ -544,6 +553,31 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
         out[a.D + 1] = l;
       }
     }
+  }
+  if (p.cluster) {
+    __syncwarp();
+    sm100::cluster_sync_all();
+    const uint32_t sums = sm100::smem_u32(&joined[0][0][0]), ends = sm100::smem_u32(&block_ends[0][0]);
+    for (int idx = split * 32 * kDecodeWarps + threadIdx.x; idx < heads * a.D; idx += p.splits * 32 * kDecodeWarps) {
+      const int h = idx / a.D, d = idx - h * a.D;
+      float top_of[kCluster], t = -INFINITY, l = 0.0f, v = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kCluster; ++s) {
+        top_of[s] = s < p.splits ? sm100::ld_cluster_f32(sm100::mapa_shared(ends + h * 8, s)) : -INFINITY;
+        t = fmaxf(t, top_of[s]);
+      }
+      const float frame = t == -INFINITY ? 0.0f : t;
+#pragma unroll
+      for (int s = 0; s < kCluster; ++s)
+        if (s < p.splits) {
+          const float f = exp2f(top_of[s] - frame);
+          l = fmaf(sm100::ld_cluster_f32(sm100::mapa_shared(ends + h * 8 + 4, s)), f, l);
+          v = fmaf(sm100::ld_cluster_f32(sm100::mapa_shared(sums + (h * (64 * DB + 2) + d) * 4, s)), f, v);
+        }
+      store1(a.y, a.dtype, ((int64_t)b * a.H + h0 + h) * a.D + d, l == 0.0f ? 0.0f : v / l);  // (0: an idle row)
+    }
+    __syncwarp();
+    sm100::cluster_sync_all();  // (a block's shared memory is read by others until here)
   }
 }
 
@@ -592,6 +626,9 @@ DecodeParams plan_decode(const flare_cache_args_t& a) {
   int64_t splits = ((int64_t)sm_count() * 4 + blocks - 1) / blocks;
   if (splits > (sight + 63) / 64) splits = (sight + 63) / 64;
   p.splits = (int)splits;
+  // A cluster saves the second launch (B=1 H=8 D=64 L=512: 8.5 us, with it 11.3), but its blocks come and go together: where a grid takes
+  // several rounds of two blocks per SM, that costs more (B=32 H=32 J=8 D=128 L=4096, rows of different lengths: 97 us, apart 87).
+  p.cluster = splits > 1 && splits <= kCluster && splits * blocks <= 2 * (int64_t)sm_count();
   return p;
 }
 
@@ -665,14 +702,14 @@ int flare_attention_append(const flare_cache_args_t* args, flare_stream_t stream
 size_t flare_attention_decode_workspace_bytes(const flare_cache_args_t* args) {
   if (check_cache(args, true)) return 0;
   const DecodeParams p = plan_decode(*args);
-  return p.splits > 1 ? (size_t)p.splits * args->B * args->H * (args->D + 2) * sizeof(float) : 0;
+  return p.splits > 1 && !p.cluster ? (size_t)p.splits * args->B * args->H * (args->D + 2) * sizeof(float) : 0;
 }
 
 int flare_attention_decode(const flare_cache_args_t* args, flare_stream_t stream) {
   if (const int rc = check_cache(args, true)) return rc;
   const flare_cache_args_t& a = *args;
   DecodeParams p = plan_decode(a);
-  if (p.splits > 1) {
+  if (p.splits > 1 && !p.cluster) {
     if (a.workspace == nullptr || a.workspace_bytes < flare_attention_decode_workspace_bytes(args)) return FLARE_ERR_WORKSPACE;
     p.part = reinterpret_cast<float*>(a.workspace);
   }
@@ -684,9 +721,21 @@ int flare_attention_decode(const flare_cache_args_t* args, flare_stream_t stream
                                           : (f16 ? decode_kernel<2, true, false> : decode_kernel<2, false, false>));
   {
     LaunchTimer timer("attention_decode_kernel", stream);
-    FLARE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)p.splits, (unsigned)(a.J * p.head_groups), (unsigned)a.B), dim3(32 * kDecodeWarps), 0, stream, p));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.splits, (unsigned)(a.J * p.head_groups), (unsigned)a.B);
+    cfg.blockDim = dim3(32 * kDecodeWarps);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.splits;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.cluster ? 2 : 1;
+    FLARE_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
   }
-  if (p.splits == 1) return FLARE_OK;
+  if (p.part == nullptr) return FLARE_OK;
   const int64_t blocks = ((int64_t)a.B * a.H * a.D + 255) / 256;
   if (blocks > INT_MAX) return FLARE_ERR_UNSUPPORTED;
   LaunchTimer timer("attention_decode_join_kernel", stream);

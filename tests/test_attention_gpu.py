@@ -287,6 +287,27 @@ def test_single_tokens(case, dtype):
     assert not y[3].any() and not y[4].any()
 
 
+@pytest.mark.parametrize("heads", [(4, 8, 2), (4, 18, 1), (60, 8, 2)], ids=str)
+@pytest.mark.parametrize("parts", range(1, 11))
+def test_caches_in_every_number_of_parts(parts, heads):
+    # parts of 64 keys and more: up to eight are joined by the blocks among themselves, more of them, or those of many rows, by a second kernel
+    B, H, J = heads
+    D, L = 72, 64 * parts - 3
+    g = gen(parts)
+    q, k, v = randn(g, B, H, D, dtype=torch.float16), randn(g, B, J, D, dtype=torch.float16), randn(g, B, J, D, dtype=torch.float16)
+    kc, vc = randn(g, B, L, J, D, dtype=torch.float16), randn(g, B, L, J, D, dtype=torch.float16)
+    cached = torch.tensor([L - 1, -1, 0, L // 3], device="cuda").repeat(B // 4)  # (of the last ones most parts have no keys)
+    kw, vw = kc.clone(), vc.clone()
+    for b in range(B):
+        if b % 4 != 1:
+            kw[b, cached[b]], vw[b, cached[b]] = k[b], v[b]
+    y = cf.flare_causal_attention_decode(q, k, v, kc, vc, cached)
+    o = orc.Attention(q[:, None].double(), kw.double(), vw.double(), behind_a_cache(B, 1, L, cached, torch.ones(B, device="cuda"), None),
+                      _resolve_attn_scale(None, D), None, None, cached, eps=2.0 ** -11)
+    close(y, o.y[:, 0], o.y_off[:, 0], "y")
+    assert not y[1::4].any()
+
+
 def test_tokens_follow_a_prompt():
     # a whole sequence at once, as a prompt and tokens one by one
     g = gen(4)
