@@ -38,7 +38,7 @@ class ScanArgs(C.Structure):
 
 class AttentionArgs(C.Structure):
     _fields_ = [
-        *((name, C.c_void_p) for name in ("q", "k", "v", "y", "lse", "documents", "prefix", "cached", "lengths", "slopes", "dy", "dq", "dk", "dv",
+        *((name, C.c_void_p) for name in ("q", "k", "v", "y", "lse", "plan", "documents", "prefix", "cached", "lengths", "slopes", "dy", "dq", "dk", "dv",
                                           "workspace")),
         ("workspace_bytes", C.c_size_t),
         *((name, C.c_int32) for name in ("B", "Nq", "Nk", "H", "J", "D")),
@@ -65,7 +65,7 @@ _CALLS = {"flare_conv_forward": ConvArgs, "flare_conv_backward": ConvArgs, "flar
           "flare_attention_append": CacheArgs, "flare_attention_decode": CacheArgs}
 _SIZES = {"flare_conv_backward_workspace_bytes": ConvArgs, "flare_scan_keep_bytes": ScanArgs,
           "flare_scan_forward_workspace_bytes": ScanArgs, "flare_scan_backward_workspace_bytes": ScanArgs,
-          "flare_attention_forward_workspace_bytes": AttentionArgs, "flare_attention_backward_workspace_bytes": AttentionArgs,
+          "flare_attention_plan_bytes": AttentionArgs, "flare_attention_forward_workspace_bytes": AttentionArgs, "flare_attention_backward_workspace_bytes": AttentionArgs,
           "flare_attention_decode_workspace_bytes": CacheArgs}
 
 _bound = None

@@ -15,6 +15,8 @@ The score of the query at position i for the key at position j is ``cap * tanh(s
 
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 from torch import autograd
 from torch.autograd.function import once_differentiable
@@ -88,16 +90,17 @@ class CausalAttention(autograd.Function):
         ctx.how = how
         B, N, H, D = q.shape
         y = torch.empty((B, N, H, D), device=q.device, dtype=q.dtype)
-        lse = None
+        lse = plan = None
         if y.numel():
             qt, kt, vt = tiled(q), tiled(k), tiled(v)
             a = _fill(qt, kt, vt, how, slopes, documents, prefix)
             a.y = y.data_ptr()
             if any(ctx.needs_input_grad):
                 lse = torch.empty((B, H, (N + 127) // 128 * 128), device=q.device, dtype=torch.float32)
-                a.lse = lse.data_ptr()
+                plan = torch.empty(_mixers.load().flare_attention_plan_bytes(C.byref(a)), device=q.device, dtype=torch.uint8)
+                a.lse, a.plan = lse.data_ptr(), plan.data_ptr()
             _mixers.run("flare_attention_forward", a, q.device, "flare_attention_forward_workspace_bytes")
-        ctx.save_for_backward(q, k, v, y, lse, slopes, documents, prefix)
+        ctx.save_for_backward(q, k, v, y, lse, slopes, documents, prefix, plan)
         return y
 
     @staticmethod
@@ -105,13 +108,13 @@ class CausalAttention(autograd.Function):
     def backward(ctx, dy):
         if dy is None:
             return (None,) * 7
-        q, k, v, y, lse, slopes, documents, prefix = ctx.saved_tensors
+        q, k, v, y, lse, slopes, documents, prefix, plan = ctx.saved_tensors
         new = torch.empty if y.numel() else torch.zeros
         dq, dk, dv = (new(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
         if y.numel():
             qt, kt, vt, dyt = tiled(q), tiled(k), tiled(v), tiled(dy)
             a = _fill(qt, kt, vt, ctx.how, slopes, documents, prefix)
-            a.y, a.lse, a.dy = y.data_ptr(), lse.data_ptr(), dyt.data_ptr()
+            a.y, a.lse, a.plan, a.dy = y.data_ptr(), lse.data_ptr(), plan.data_ptr(), dyt.data_ptr()
             put_strides(a, "dy", dyt, "bnh")
             a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
             _mixers.run("flare_attention_backward", a, q.device, "flare_attention_backward_workspace_bytes")

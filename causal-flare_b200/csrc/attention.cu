@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(256) delta_kernel(const AttnParams p, const T*
 }
 
 struct Layout {
-  size_t range, query_span, key_span, dirty, ends, delta, bytes;
+  size_t range, query_span, key_span, dirty, ends, plan_bytes;  // in `plan`, or in front of the workspace
+  size_t delta, bytes;                                          // in the workspace
   int Nqp, Nkp;
 };
 Layout layout(const flare_attention_args_t& a, bool backward) {
@@ -209,6 +210,8 @@ Layout layout(const flare_attention_args_t& a, bool backward) {
   l.key_span = take((size_t)a.B * (l.Nkp / 128) * sizeof(int2));
   l.dirty = take((size_t)a.B * (l.Nkp / 64));
   l.ends = take((size_t)a.B * 4);
+  l.plan_bytes = at;
+  if (a.plan != nullptr) at = 0;
   l.delta = take(backward ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
   l.bytes = at;
   return l;
@@ -235,16 +238,21 @@ int check(const flare_attention_args_t* args) {
   if (a.dtype != FLARE_BF16 && a.dtype != FLARE_F16) return FLARE_ERR_BAD_DTYPE;
   if (bad_scores(a.scale, a.cap, a.window)) return FLARE_ERR_BAD_CONFIG;
   if (a.cached == nullptr ? a.Nk != a.Nq : a.documents != nullptr) return FLARE_ERR_BAD_CONFIG;
+  if (reinterpret_cast<uintptr_t>(a.plan) & 255u) return FLARE_ERR_BAD_POINTER;
   if (!strides_fit(a.q, {a.q_stride_b, a.q_stride_n, a.q_stride_h}) || !strides_fit(a.k, {a.k_stride_b, a.k_stride_n, a.k_stride_h}) ||
       !strides_fit(a.v, {a.v_stride_b, a.v_stride_n, a.v_stride_h}) || !strides_fit(a.y, {}))
     return FLARE_ERR_BAD_POINTER;
   return FLARE_OK;
 }
 
-// parameters, and the masks' kernel
-int begin(const flare_attention_args_t& a, const Layout& l, AttnParams& p, cudaStream_t stream) {
+bool workspace_fits(const flare_attention_args_t& a, const Layout& l) {
+  return l.bytes == 0 || (a.workspace != nullptr && a.workspace_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(a.workspace) & 255u) == 0);
+}
+
+// parameters, and the masks' kernel (unless the forward left what it finds)
+int begin(const flare_attention_args_t& a, const Layout& l, AttnParams& p, bool backward, cudaStream_t stream) {
   memset(&p, 0, sizeof(p));
-  uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
+  uint8_t* const ws = reinterpret_cast<uint8_t*>(a.plan != nullptr ? a.plan : a.workspace);
   PlanParams plan;
   plan.range = reinterpret_cast<int2*>(ws + l.range);
   plan.query_span = reinterpret_cast<int2*>(ws + l.query_span);
@@ -262,6 +270,7 @@ int begin(const flare_attention_args_t& a, const Layout& l, AttnParams& p, cudaS
   p.B = a.B; p.Nq = a.Nq; p.Nk = a.Nk; p.H = a.H; p.J = a.J; p.D = a.D;
   p.scale = a.scale; p.cap = a.cap;
   if (const int rc = tc_error_word(&p.err)) return rc;
+  if (backward && a.plan != nullptr) return FLARE_OK;
   LaunchTimer timer("attention_plan_kernel", stream);
   FLARE_CUDA_CHECK(launch_pdl(plan_kernel, dim3((unsigned)a.B), dim3(kPlanThreads), 0, stream, plan));
   return FLARE_OK;
@@ -641,6 +650,10 @@ using namespace flare::attn;
 
 extern "C" {
 
+size_t flare_attention_plan_bytes(const flare_attention_args_t* args) {
+  if (args == nullptr || args->B <= 0 || args->Nq <= 0 || args->Nk <= 0) return 0;
+  return layout(*args, false).plan_bytes;
+}
 size_t flare_attention_forward_workspace_bytes(const flare_attention_args_t* args) {
   if (args == nullptr || args->B <= 0 || args->Nq <= 0 || args->Nk <= 0) return 0;
   return layout(*args, false).bytes;
@@ -654,9 +667,9 @@ int flare_attention_forward(const flare_attention_args_t* args, flare_stream_t s
   if (const int rc = check(args)) return rc;
   const flare_attention_args_t& a = *args;
   const Layout l = layout(a, false);
-  if (a.workspace == nullptr || a.workspace_bytes < l.bytes || (reinterpret_cast<uintptr_t>(a.workspace) & 255u)) return FLARE_ERR_WORKSPACE;
+  if (!workspace_fits(a, l)) return FLARE_ERR_WORKSPACE;
   AttnParams p;
-  if (const int rc = begin(a, l, p, stream)) return rc;
+  if (const int rc = begin(a, l, p, false, stream)) return rc;
   return launch_forward_tc(a, p, stream);
 }
 
@@ -668,9 +681,9 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
       !strides_fit(a.dv, {}) || !strides_fit(a.lse, {}))
     return FLARE_ERR_BAD_POINTER;
   const Layout l = layout(a, true);
-  if (a.workspace == nullptr || a.workspace_bytes < l.bytes || (reinterpret_cast<uintptr_t>(a.workspace) & 255u)) return FLARE_ERR_WORKSPACE;
+  if (!workspace_fits(a, l)) return FLARE_ERR_WORKSPACE;
   AttnParams p;
-  if (const int rc = begin(a, l, p, stream)) return rc;
+  if (const int rc = begin(a, l, p, true, stream)) return rc;
   float* const delta = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.workspace) + l.delta);
   p.delta = delta;
   const int lanes = a.D <= 64 ? 8 : 16;

@@ -35,6 +35,7 @@ struct Api {
   decltype(&flare_scan_forward) scan_forward = nullptr, scan_backward = nullptr, scan_decode = nullptr;
   decltype(&flare_scan_keep_bytes) scan_keep_bytes = nullptr, scan_forward_workspace_bytes = nullptr, scan_backward_workspace_bytes = nullptr;
   decltype(&flare_attention_forward) attention_forward = nullptr, attention_backward = nullptr;
+  decltype(&flare_attention_plan_bytes) attention_plan_bytes = nullptr;
   decltype(&flare_attention_forward_workspace_bytes) attention_forward_workspace_bytes = nullptr, attention_backward_workspace_bytes = nullptr;
   decltype(&flare_attention_append) attention_append = nullptr, attention_decode = nullptr;
   decltype(&flare_attention_decode_workspace_bytes) attention_decode_workspace_bytes = nullptr;
@@ -65,6 +66,7 @@ void bind(const py::dict& table) {
   take(api.scan_backward_workspace_bytes, table, "flare_scan_backward_workspace_bytes");
   take(api.attention_forward, table, "flare_attention_forward");
   take(api.attention_backward, table, "flare_attention_backward");
+  take(api.attention_plan_bytes, table, "flare_attention_plan_bytes");
   take(api.attention_forward_workspace_bytes, table, "flare_attention_forward_workspace_bytes");
   take(api.attention_backward_workspace_bytes, table, "flare_attention_backward_workspace_bytes");
   take(api.attention_append, table, "flare_attention_append");
@@ -528,9 +530,11 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     const Tensor lse = at::empty({q.size(0), q.size(2), (q.size(1) + 127) / 128 * 128}, q.options().dtype(at::kFloat).requires_grad(false));
     a.y = y.data_ptr();
     a.lse = ptr<float>(lse);
+    const Tensor plan = bytes(api.attention_plan_bytes(&a), q);
+    a.plan = ptr(plan);
     const Tensor ws = workspace(a, api.attention_forward_workspace_bytes(&a), q);
     check(api.attention_forward(&a, stream_of(q)), "flare_attention_forward");
-    ctx->save_for_backward({q0, k0, v0, y, lse, slopes, documents, prefix});
+    ctx->save_for_backward({q0, k0, v0, y, lse, slopes, documents, prefix, plan});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["cap"] = cap;
     ctx->saved_data["window"] = window;
@@ -546,6 +550,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
     fill_attention(a, q, k, v, {ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["window"].toInt(), s[5]}, s[6], s[7]);
     a.y = s[3].data_ptr();
     a.lse = ptr<float>(s[4]);
+    a.plan = ptr(s[8]);
     a.dy = dy.data_ptr();
     a.dy_stride_b = step_of(dy, 0); a.dy_stride_n = step_of(dy, 1); a.dy_stride_h = step_of(dy, 2);
     for (int i = 0; i < 3; ++i) out[i] = new_like(s[i]);

@@ -122,6 +122,7 @@ typedef struct flare_attention_args {
   const void* v;            /* [B, Nk, J, D] */
   void* y;                  /* [B, Nq, H, D] contiguous */
   float* lse;               /* [B, H, Nq rounded up to 128]: minus log2 of the softmax denominators, for the backward; may be NULL */
+  void* plan;               /* flare_attention_plan_bytes(args), 256-byte aligned: who sees whom, left by the forward for the backward; NULL: formed again */
   const int32_t* documents; /* [B, Nq] contiguous or NULL */
   const uint8_t* prefix;    /* [B, Nq] contiguous or NULL */
   const int32_t* cached;    /* [B] or NULL */
@@ -141,9 +142,10 @@ typedef struct flare_attention_args {
   int32_t dtype;
 } flare_attention_args_t;
 
+size_t flare_attention_plan_bytes(const flare_attention_args_t* args);
 size_t flare_attention_forward_workspace_bytes(const flare_attention_args_t* args);
 int flare_attention_forward(const flare_attention_args_t* args, flare_stream_t stream);
-/* y and lse as the forward of the same problem left them */
+/* y, lse and (if given) plan as the forward of the same problem left them */
 size_t flare_attention_backward_workspace_bytes(const flare_attention_args_t* args);
 int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t stream);
 

@@ -106,7 +106,7 @@ def args(**kw):
     ("forward", dict(H=3), 1), ("forward", dict(D=68), 2), ("forward", dict(D=192), 2), ("forward", dict(dtype=0), 5), ("forward", dict(scale=-1.0), 6),
     ("forward", dict(cap=float("nan")), 6), ("forward", dict(cap=1025.0), 6), ("forward", dict(cap=1e-40), 6), ("forward", dict(scale=float("inf")), 6), ("forward", dict(window=-1), 6), ("forward", dict(Nk=65), 6), ("forward", dict(cached=0x1000, documents=0x1000), 6),
     ("forward", dict(q=0x1008), 3), ("forward", dict(k_stride_n=260), 3), ("forward", {}, 4), ("backward", dict(cached=0x1000, Nk=100), 6),
-    ("backward", dict(dy=None), 3), ("backward", dict(lse=None), 3), ("backward", {}, 4),
+    ("forward", dict(plan=0x1010), 3), ("backward", dict(dy=None), 3), ("backward", dict(plan=0x1000), 4), ("backward", dict(lse=None), 3), ("backward", {}, 4),
 ])
 def test_entry_points_refuse(call_, kw, status):
     assert getattr(_mixers.load(), "flare_attention_" + call_)(C.byref(args(**kw)), None) == status

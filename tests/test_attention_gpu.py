@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import causal_flare as cf
-from causal_flare import _ops
+from causal_flare import _mixers, _ops, attention
 from causal_flare._common import _resolve_attn_scale
 from oracle import mixers_oracle as orc
 
@@ -184,6 +184,26 @@ def test_same_bits_on_another_stream_and_from_a_graph():
     torch.cuda.synchronize()
     for a, b, c in zip(first, second, third):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_a_backward_without_the_forwards_plan_forms_it_again():
+    case = (2, 300, 4, 2, 64, None, True, 100, "holes", True)
+    q, k, v, dy, how = inputs(case, torch.bfloat16)
+    for t in (q, k, v):
+        t.requires_grad_()
+    y = cf.flare_causal_attention(q, k, v, **how)
+    want = torch.autograd.grad(y, (q, k, v), dy)
+    a = attention._fill(q, k, v, (64 ** -0.5, 0.0, 100), how["slopes"], how["documents"], how["prefix"])
+    out, lse = torch.empty_like(y), torch.empty(2, 4, 384, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    a.y, a.lse = out.data_ptr(), lse.data_ptr()
+    _mixers.run("flare_attention_forward", a, q.device, "flare_attention_forward_workspace_bytes")
+    a.dy = dy.data_ptr()
+    _mixers.put_strides(a, "dy", dy, "bnh")
+    a.dq, a.dk, a.dv = (t.data_ptr() for t in grads)
+    _mixers.run("flare_attention_backward", a, q.device, "flare_attention_backward_workspace_bytes")
+    for x, z in zip((out, *grads), (y, *want)):
+        assert torch.equal(x, z)
 
 
 def test_no_tokens():
