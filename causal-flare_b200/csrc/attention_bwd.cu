@@ -7,9 +7,9 @@
 // dP = X1 Y1^T into tensor memory, rows of the own side on the lanes; the threads turn them into P and dS, laid down over S and dP
 // as packed 16-bit values, from where the products that are summed over the walk take their A operand (dV += P Y1,
 // dK or dQ += dS Y0): neither P nor dS passes through shared memory, and no gradient is added by two CTAs (a key head's dK and dV walk its
-// query heads one after the other).  The price is S and dP twice, and dS in two
-// parts 18 instead of 10 products of D operations for a pair.  Two slots take every
+// query heads one after the other).  The price is S and dP twice and dS in two parts: 18 D instead of 10 D operations for a pair.  Two slots take every
 // other tile, with eight warps each (32 of the 64 columns a warp), so that one's exponentials run under the other's products.
+// B200, B=2 N=4096 H=16 D=128 bf16: 550 us for both kernels (0.67 of the measured matrix rate for 18 D), with a cap 632.
 //
 // Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P is rounded once, to the type of the
 // operands it meets; dS goes to its product as a rounded value and what that lost, rounded again: rounded once it made dK and dQ 1.6 times as far

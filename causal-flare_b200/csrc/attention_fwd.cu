@@ -11,7 +11,8 @@
 //
 // Tensor memory: S / P of the groups, two buffers each, at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, the
 // first two tiles of K, four stages of a tile of V and one of K.  Floors per 64 keys and both groups, in cycles: products 1 024 (M = 128, N = 64 from shared memory: 1 280),
-// exponentials 1 024.
+// exponentials 1 024.  B200, B=2 N=4096 H=16 D=128 bf16: 150 us (0.55 of the measured matrix rate), with a cap 195: the caps' seven
+// products and sums for every score come on top of a group's own work, which is what bounds either.
 #include <limits.h>
 
 #include "attention_tc.cuh"
