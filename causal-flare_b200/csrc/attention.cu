@@ -166,28 +166,86 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   }
 }
 
-// -delta = -<dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  Bound by memory.
+struct DeltaParams {
+  AttnParams p;
+  const void *q, *k, *v, *dy;
+  int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, dy_b, dy_n, dy_h;
+  float* delta;
+};
+// Keys up to which a row's delta is the sum of P dP itself.  <dy, y> has y's rounding and that of the weights in y, about 2^-9 |dy| |v| / sqrt(keys),
+// which dS = P (dP - delta) keeps: with two to five keys dQ and dK were 1.7 to 4 times as far off as their own rounding, with 50 and more 1.1.
+constexpr int kFewKeys = 32;
+
+// -delta, delta = sum P dP = <dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  Bound by memory.
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) delta_kernel(const AttnParams p, const T* dy, int64_t sb, int64_t sn, int64_t sh, float* delta) {
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ DeltaParams d) {
   pdl_begin();
+  const AttnParams& p = d.p;
   const int lane = threadIdx.x % LANES, b = blockIdx.y;
   const unsigned idx = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int i = (int)(idx / (unsigned)p.H), h = (int)(idx % (unsigned)p.H);
-  const bool live = i < p.masks.Nqp;
-  float sum = 0.0f;
-  if (live && i < p.Nq && lane * 8 < p.D) {
-    const int2 r = p.masks.range[(int64_t)b * p.masks.Nqp + i];
-    if (r.y > r.x) {
-      float a[8], c[8];
-      unpack8(load_raw8<T>(dy + b * sb + i * sn + h * sh + lane * 8, 8, true), a);
-      unpack8(load_raw8<T>(reinterpret_cast<const T*>(p.y) + (((int64_t)b * p.Nq + i) * p.H + h) * p.D + lane * 8, 8, true), c);
+  const bool live = i < p.masks.Nqp, mine = live && i < p.Nq && lane * 8 < p.D;
+  const int2 r = live && i < p.Nq ? p.masks.range[(int64_t)b * p.masks.Nqp + i] : make_int2(0, 0);
+  const auto eight = [&](const void* base, int64_t at, float (&out)[8]) {  // of a row
+    unpack8(load_raw8<T>(reinterpret_cast<const T*>(base) + at + lane * 8, 8, true), out);
+  };
+  const auto dot = [](const float (&a)[8], const float (&c)[8]) {
+    float s = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum = fmaf(a[k], c[k], sum);
+    for (int k = 0; k < 8; ++k) s = fmaf(a[k], c[k], s);
+    return s;
+  };
+  const auto joined = [](float s) {  // over the row's threads
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+  };
+  float dy[8] = {}, sum = 0.0f;
+  const int keys = r.y - r.x;
+  const bool few = keys <= kFewKeys;
+  if (mine && keys > 0) {
+    eight(d.dy, b * d.dy_b + i * d.dy_n + h * d.dy_h, dy);
+    if (!few) {
+      float y[8];
+      eight(p.y, (((int64_t)b * p.Nq + i) * p.H + h) * p.D, y);
+      sum = dot(dy, y);
     }
   }
+  sum = joined(sum);
+  const int steps = __reduce_max_sync(0xffffffffu, few ? max(keys, 0) : 0);
+  if (steps > 0) {
+    float q[8] = {}, weights = 0.0f, weighted = 0.0f;
+    if (mine && few && keys > 0) eight(d.q, b * d.q_b + i * d.q_n + h * d.q_h, q);
+    const int kv = h / (p.H / p.J);
+    const float lse = few && keys > 0 ? p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] : 0.0f, slope = p.slopes != nullptr ? p.slopes[h] : 0.0f;
+    constexpr int GROUP = 4;  // keys on their way together
+    for (int t0 = 0; t0 < steps; t0 += GROUP) {
+      Raw8<T> k[GROUP], v[GROUP];
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (live && lane == 0) delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = -sum;
+      for (int g = 0; g < GROUP; ++g) {
+        const int64_t j = r.x + t0 + g;
+        const int count = mine && few && t0 + g < keys ? 8 : 0;
+        k[g] = load_raw8<T>(reinterpret_cast<const T*>(d.k) + b * d.k_b + j * d.k_n + kv * d.k_h + lane * 8, count, true);
+        v[g] = load_raw8<T>(reinterpret_cast<const T*>(d.v) + b * d.v_b + j * d.v_n + kv * d.v_h + lane * 8, count, true);
+      }
+#pragma unroll
+      for (int g = 0; g < GROUP; ++g) {
+        const bool on = few && t0 + g < keys;
+        float f[8];
+        unpack8(k[g], f);
+        float s = joined(dot(q, f)) * p.scale;
+        unpack8(v[g], f);
+        const float dp = joined(dot(dy, f));
+        if (p.cap > 0.0f) s = p.cap * tanhf(s / p.cap);
+        s = fmaf(-slope, (float)abs(i - (r.x + t0 + g)), s);
+        const float w = on ? exp2f(fmaf(s, kLog2e, lse)) : 0.0f;
+        weights += w;
+        weighted = on ? fmaf(w, dp, weighted) : weighted;
+      }
+    }
+    if (few) sum = keys > 0 ? weighted / weights : 0.0f;
+  }
+  if (live && lane == 0) d.delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = -sum;
 }
 
 struct Layout {
@@ -693,12 +751,17 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   {
     LaunchTimer timer("attention_delta_kernel", stream);
     const dim3 grid((unsigned)blocks, (unsigned)a.B);
-    const auto run = [&](auto t, auto* kernel) {
-      using T = decltype(t);
-      return launch_pdl(kernel, grid, dim3(256), 0, stream, p, reinterpret_cast<const T*>(a.dy), a.dy_stride_b, a.dy_stride_n, a.dy_stride_h, delta);
-    };
-    if (a.dtype == FLARE_F16) FLARE_CUDA_CHECK(run(__half(), lanes == 8 ? delta_kernel<__half, 8> : delta_kernel<__half, 16>));
-    else FLARE_CUDA_CHECK(run(__nv_bfloat16(), lanes == 8 ? delta_kernel<__nv_bfloat16, 8> : delta_kernel<__nv_bfloat16, 16>));
+    DeltaParams d;
+    d.p = p;
+    d.q = a.q; d.k = a.k; d.v = a.v; d.dy = a.dy;
+    d.q_b = a.q_stride_b; d.q_n = a.q_stride_n; d.q_h = a.q_stride_h;
+    d.k_b = a.k_stride_b; d.k_n = a.k_stride_n; d.k_h = a.k_stride_h;
+    d.v_b = a.v_stride_b; d.v_n = a.v_stride_n; d.v_h = a.v_stride_h;
+    d.dy_b = a.dy_stride_b; d.dy_n = a.dy_stride_n; d.dy_h = a.dy_stride_h;
+    d.delta = delta;
+    auto* const kernel = a.dtype == FLARE_F16 ? (lanes == 8 ? delta_kernel<__half, 8> : delta_kernel<__half, 16>)
+                                              : (lanes == 8 ? delta_kernel<__nv_bfloat16, 8> : delta_kernel<__nv_bfloat16, 16>);
+    FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(256), 0, stream, d));
   }
   return launch_backward_tc(a, p, stream);
 }

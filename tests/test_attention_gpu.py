@@ -186,6 +186,26 @@ def test_same_bits_on_another_stream_and_from_a_graph():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(3, 2, 2, 1, 128, None, None), (2, 32, 4, 2, 64, 15.0, None), (1, 200, 3, 1, 40, None, 3), (1, 150, 6, 2, 96, 20.0, 32)], ids=str)
+def test_few_keys_whose_values_are_much_alike(case, dtype):
+    # dP - <dy, y> is a twentieth of either: the rounding of y, or of the weights in it, would show twenty times.  Rows of up to 32 keys go without either:
+    # half a step of the result is left, dS within half^2 (two parts), and roundings of 2^-22 of sums twenty times as large.
+    B, N, H, J, D, cap, window = case
+    g = gen(N)
+    q, k, dy = randn(g, B, N, H, D, dtype=dtype), randn(g, B, N, J, D, dtype=dtype), randn(g, B, N, H, D, dtype=dtype)
+    v = (1 + 0.05 * randn(g, B, N, J, D)).to(dtype)
+    slopes = torch.rand(H, generator=g, device="cuda") * 0.1
+    for t in (q, k, v):
+        t.requires_grad_()
+    got = torch.autograd.grad(cf.flare_causal_attention(q, k, v, cap=cap, window=window, slopes=slopes), (q, k), dy)
+    half = torch.finfo(dtype).eps / 2
+    o = orc.Attention(q.detach().double(), k.detach().double(), v.detach().double(), orc.in_sight(N, window=window).cuda(), D ** -0.5, cap, slopes.double(),
+                      dy=dy.double(), eps=half)
+    for a, b in zip(got, (o.dq, o.dk)):
+        assert float((a.double() - b).norm() / b.norm()) <= 1.01 * half + half ** 2 + 20 * 30 * 2.0 ** -22
+
+
 def test_a_backward_without_the_forwards_plan_forms_it_again():
     case = (2, 300, 4, 2, 64, None, True, 100, "holes", True)
     q, k, v, dy, how = inputs(case, torch.bfloat16)
