@@ -203,19 +203,17 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
   float dy[8] = {}, sum = 0.0f;
   const int keys = r.y - r.x;
   const bool few = keys <= kFewKeys;
-  if (mine && keys > 0) {
+  if (mine) {  // (the loads do not wait for the row's keys)
+    float y[8];
     eight(d.dy, b * d.dy_b + i * d.dy_n + h * d.dy_h, dy);
-    if (!few) {
-      float y[8];
-      eight(p.y, (((int64_t)b * p.Nq + i) * p.H + h) * p.D, y);
-      sum = dot(dy, y);
-    }
+    eight(p.y, (((int64_t)b * p.Nq + i) * p.H + h) * p.D, y);
+    sum = dot(dy, y);
   }
   sum = joined(sum);
   const int steps = __reduce_max_sync(0xffffffffu, few ? max(keys, 0) : 0);
   if (steps > 0) {
     float q[8] = {}, weights = 0.0f, weighted = 0.0f;
-    if (mine && few && keys > 0) eight(d.q, b * d.q_b + i * d.q_n + h * d.q_h, q);
+    if (mine) eight(d.q, b * d.q_b + i * d.q_n + h * d.q_h, q);
     const int kv = h / (p.H / p.J);
     const float lse = few && keys > 0 ? p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] : 0.0f, slope = p.slopes != nullptr ? p.slopes[h] : 0.0f;
     constexpr int GROUP = 4;  // keys on their way together
@@ -243,8 +241,9 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
         weighted = on ? fmaf(w, dp, weighted) : weighted;
       }
     }
-    if (few) sum = keys > 0 ? weighted / weights : 0.0f;
+    if (few) sum = weighted / weights;
   }
+  if (keys <= 0) sum = 0.0f;
   if (live && lane == 0) d.delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = -sum;
 }
 
