@@ -5,10 +5,10 @@
 // Bound by the special-function unit: S exponentials for every token and channel, at 16 per cycle and SM, where the rows
 // themselves are 6 to 8 bytes.  A channel belongs to S / NS threads with NS states each in registers; a block walks its channels' tokens
 // in tiles of 32: delta, delta x, b and c of a tile are laid down in shared memory as fp32 (softplus once per token and channel, not
-// once per state), twice, so that the next tile is laid down while this one is walked and a tile costs one barrier; the rows of the
-// tile after that are on their way into registers meanwhile.  The recurrence's products are packed in pairs.  The sum over a
+// once per state), twice, so that the next tile is laid down while this one is walked (by threads of their own, where a block has an SM to itself) and a tile
+// costs one barrier; the rows of the tile after that are on their way into registers meanwhile.  The recurrence's products are packed in pairs.  The sum over a
 // channel's states is taken for as many tokens as the channel has threads at a time: three exchanges for four tokens.  B200, B=4 N=4096 C=2048 S=16
-// bf16: 396 us (the exponentials alone: 120; what is issued and its latencies bound it).
+// bf16: 340 us (the exponentials alone: 120; what is issued and its latencies bound it).
 //
 // Few channels: a row's tokens are cut into segments that run side by side.  A first pass over all segments but the last forms
 // what each leaves behind from a zero state (every exponential once more, no read-out), a small kernel joins them in order
@@ -85,9 +85,10 @@ __device__ __forceinline__ float softplus(float u, float& slope) {
   return fmaxf(u, 0.0f) + 2.0f * fmaf(s * q, a, s);
 }
 
-// Where a block and a thread work.
-template <typename K>
+// Where a block and a thread work.  SPLIT: half of the threads stage, the others walk.
+template <typename K, bool SPLIT = false>
 struct Place {
+  __device__ static __forceinline__ unsigned tid() { return SPLIT ? threadIdx.x % K::THREADS : threadIdx.x; }
   int b, seg, t0, t1, len;   // tokens of the segment
   int group, c0, here;       // first channel of the block, how many it has
   int token, cg, count;      // staging: token of the tile, first of V channels, how many of them there are
@@ -104,11 +105,11 @@ struct Place {
     const int in_group = (blockIdx.y % p.blocks_c) * K::CH;
     c0 = group * p.channels + in_group;
     here = min(K::CH, p.channels - in_group);
-    token = threadIdx.x / K::PER;
-    cg = threadIdx.x % K::PER * K::V;
+    token = tid() / K::PER;
+    cg = tid() % K::PER * K::V;
     count = max(0, min(K::V, here - cg));
-    ch = threadIdx.x / K::LANES;
-    sub = threadIdx.x % K::LANES;
+    ch = tid() / K::LANES;
+    sub = tid() % K::LANES;
     channel = ch < here ? c0 + ch : -1;
     ids = a.documents != nullptr ? a.documents + (int64_t)b * a.N : nullptr;
   }
@@ -122,7 +123,8 @@ struct Rows {
   T b[K::BC], c[K::BC];
   bool on, bc_on[K::BC], reset;
 
-  __device__ __forceinline__ void load(const ScanParams& p, const Place<K>& at, int t0) {
+  template <typename At>
+  __device__ __forceinline__ void load(const ScanParams& p, const At& at, int t0) {
     const flare_scan_args_t& a = p.a;
     const int t = t0 + at.token;
     on = at.on(t);
@@ -131,7 +133,7 @@ struct Rows {
     dt = load_raw<T, K::V>(reinterpret_cast<const T*>(a.dt) + at.b * a.dt_stride_b + t * a.dt_stride_n + at.c0 + at.cg, n, WIDE);
 #pragma unroll
     for (int i = 0; i < K::BC; ++i) {
-      const int idx = threadIdx.x + i * K::THREADS, tt = t0 + idx / K::S, s = idx % K::S;
+      const int idx = at.tid() + i * K::THREADS, tt = t0 + idx / K::S, s = idx % K::S;
       bc_on[i] = at.on(tt);
       b[i] = c[i] = from_float<T>(0.0f);
       if (bc_on[i]) {
@@ -139,12 +141,13 @@ struct Rows {
         c[i] = reinterpret_cast<const T*>(a.c)[at.b * a.c_stride_b + tt * a.c_stride_n + at.group * a.c_stride_g + s];
       }
     }
-    const int r = t0 + threadIdx.x;
+    const int r = t0 + at.tid();
     reset = false;
-    if (at.ids != nullptr && threadIdx.x < kTile && r < at.t1) reset = r == 0 || at.ids[r] != at.ids[r - 1];
+    if (at.ids != nullptr && at.tid() < kTile && r < at.t1) reset = r == 0 || at.ids[r] != at.ids[r - 1];
   }
   // into shared memory; padding: delta = delta x = b = c = 0, so that it leaves the state as it is
-  __device__ __forceinline__ void stage(const ScanParams& p, const Place<K>& at, const float (&bias)[K::V], Tile<K>& to, float (&delta)[K::V],
+  template <typename At>
+  __device__ __forceinline__ void stage(const ScanParams& p, const At& at, const float (&bias)[K::V], Tile<K>& to, float (&delta)[K::V],
                                         float (&slope)[K::V], float (&xf)[K::V]) const {
     unpack<T, K::V>(x, xf);
     unpack<T, K::V>(dt, delta);
@@ -160,11 +163,11 @@ struct Rows {
     for (int i = 0; i < K::V; ++i) row[i] = make_float4(delta[i], delta[i], delta[i] * xf[i], delta[i] * xf[i]);
 #pragma unroll
     for (int i = 0; i < K::BC; ++i) {
-      const int idx = threadIdx.x + i * K::THREADS, s = idx % K::S;
+      const int idx = at.tid() + i * K::THREADS, s = idx % K::S;
       to.bc[idx / K::S][s >> 1][s & 1] = to_float<T>(b[i]);
       to.bc[idx / K::S][s >> 1][2 + (s & 1)] = to_float<T>(c[i]);
     }
-    if (threadIdx.x < kTile) to.reset[threadIdx.x] = reset;
+    if (at.tid() < kTile) to.reset[at.tid()] = reset;
   }
 };
 
@@ -262,13 +265,15 @@ __device__ __forceinline__ int channel_sums(float (&v)[M], int lane) {
   return mine ? first : -1;
 }
 
-template <typename T, typename K, bool ENDS, bool WIDE, bool DOCS>
-__global__ void __launch_bounds__(K::THREADS, K::BLOCKS) forward_kernel(const ScanParams p) {
+// SPLIT: half of the threads walk, the others lay down the next tile and read out the last one meanwhile
+template <typename T, typename K, bool ENDS, bool WIDE, bool DOCS, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 2 * K::THREADS : K::THREADS, SPLIT ? 1 : K::BLOCKS) forward_kernel(const ScanParams p) {
   pdl_wait();
   extern __shared__ __align__(16) uint8_t smem[];
   ForwardSmem<K>& sm = *reinterpret_cast<ForwardSmem<K>*>(smem);
   const flare_scan_args_t& a = p.a;
-  const Place<K> at(p);
+  const bool walks = !SPLIT || threadIdx.x < K::THREADS, stages = !SPLIT || !walks;
+  const Place<K, SPLIT> at(p);
   if (ENDS && at.seg == p.segments - 1) return;  // (nothing follows it)
   constexpr int S = K::S, P = K::P, V = K::V, LANES = K::LANES;
   float bias[V], D[V];
@@ -303,79 +308,88 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) forward_kernel(const Sc
     if (!ENDS && zp != nullptr)
       z = load_raw<T, V>(zp + at.b * a.z_stride_b + t * a.z_stride_n + at.c0 + at.cg, rows.on ? at.count : 0, WIDE);
   };
-  // of the tile that is walked
-  Raw<T, V> x_now, z_now;
-  bool on_now;
   const auto lay_down = [&](int buffer) {
     float delta[V], slope[V], x[V];
     rows.stage(p, at, bias, sm.in[buffer], delta, slope, x);
   };
-  fetch(at.t0);
-  lay_down(0);
-  x_now = rows.x;
-  z_now = z;
-  on_now = rows.on;
-  if (at.t0 + kTile < at.t1) fetch(at.t0 + kTile);
+  // what the read-out of a tile takes: of the tile that is walked, and of the one before it
+  Raw<T, V> x_now, z_now, x_out, z_out;
+  bool on_now = false, on_out = false;
+  const auto read_out = [&](int t, int buffer) {
+    if (ENDS || t >= at.t1 || at.count <= 0) return;
+    float y[V], x[V], g[V];
+    unpack<T, V>(x_out, x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = fmaf(D[i], x[i], sm.y[buffer][at.token][at.cg + i]);
+    if (zp != nullptr) {
+      unpack<T, V>(z_out, g);
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] *= g[i] * sigmoid(g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = on_out ? y[i] : 0.0f;
+    store_all<T, V>(reinterpret_cast<T*>(a.y) + ((int64_t)at.b * a.N + t) * a.C + at.c0 + at.cg, y, at.count, WIDE);
+  };
+  if (stages) {
+    fetch(at.t0);
+    lay_down(0);
+    x_now = rows.x;
+    z_now = z;
+    on_now = rows.on;
+    if (at.t0 + kTile < at.t1) fetch(at.t0 + kTile);
+  }
   __syncthreads();
   int buffer = 0;
 #pragma unroll 1
   for (int t0 = at.t0; t0 < at.t1; t0 += kTile, buffer ^= 1) {
-    const Tile<K>& in = sm.in[buffer];
-    if (!ENDS && a.keep != nullptr && at.channel >= 0)
-      store_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at, h);
-    constexpr int STEP = ENDS ? 4 : LANES;
+    if (walks) {
+      const Tile<K>& in = sm.in[buffer];
+      if (!ENDS && a.keep != nullptr && at.channel >= 0)
+        store_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at, h);
+      constexpr int STEP = ENDS ? 4 : LANES;
 #pragma unroll(16 / STEP)
-    for (int t = 0; t < kTile; t += STEP) {
-      float v[STEP];
+      for (int t = 0; t < kTile; t += STEP) {
+        float v[STEP];
 #pragma unroll
-      for (int k = 0; k < STEP; ++k) {
-        if (DOCS && in.reset[t + k]) {
+        for (int k = 0; k < STEP; ++k) {
+          if (DOCS && in.reset[t + k]) {
 #pragma unroll
-          for (int i = 0; i < P; ++i) h[i] = 0;
-          if (ENDS) sum = -INFINITY;
+            for (int i = 0; i < P; ++i) h[i] = 0;
+            if (ENDS) sum = -INFINITY;
+          }
+          const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t + k][padded(at.ch)]);
+          const uint64_t d2 = dd.x, x2 = dd.y;
+          uint64_t b[P], c[P], acc = 0;
+          load_bc<P>(&in.bc[t + k][at.sub * P], b, c);
+          if (ENDS) sum += low(d2);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            h[i] = f2_fma(factor(A2[i], d2), h[i], f2_mul(x2, b[i]));
+            if (!ENDS) acc = i ? f2_fma(h[i], c[i], acc) : f2_mul(h[i], c[i]);
+          }
+          v[k] = pair_sum(acc);
         }
-        const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t + k][padded(at.ch)]);
-        const uint64_t d2 = dd.x, x2 = dd.y;
-        uint64_t b[P], c[P], acc = 0;
-        load_bc<P>(&in.bc[t + k][at.sub * P], b, c);
-        if (ENDS) sum += low(d2);
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          h[i] = f2_fma(factor(A2[i], d2), h[i], f2_mul(x2, b[i]));
-          if (!ENDS) acc = i ? f2_fma(h[i], c[i], acc) : f2_mul(h[i], c[i]);
-        }
-        v[k] = pair_sum(acc);
+        if constexpr (!ENDS) sm.y[buffer][t + at.sub][at.ch] = lane_sums<LANES>(v, at.sub);
       }
-      if constexpr (!ENDS) sm.y[buffer][t + at.sub][at.ch] = lane_sums<LANES>(v, at.sub);
     }
-    const Raw<T, V> x_out = x_now, z_out = z_now;
-    const bool on_out = on_now;
-    if (t0 + kTile < at.t1) {
-      lay_down(buffer ^ 1);
-      x_now = rows.x;
-      z_now = z;
-      on_now = rows.on;
-      if (t0 + 2 * kTile < at.t1) fetch(t0 + 2 * kTile);
+    if (stages) {
+      if (SPLIT && t0 > at.t0) read_out(t0 - kTile + at.token, buffer ^ 1);
+      x_out = x_now;
+      z_out = z_now;
+      on_out = on_now;
+      if (t0 + kTile < at.t1) {
+        lay_down(buffer ^ 1);
+        x_now = rows.x;
+        z_now = z;
+        on_now = rows.on;
+        if (t0 + 2 * kTile < at.t1) fetch(t0 + 2 * kTile);
+      }
     }
     __syncthreads();
-    if (!ENDS) {
-      const int t = t0 + at.token;
-      if (t < at.t1 && at.count > 0) {
-        float y[V], x[V], g[V];
-        unpack<T, V>(x_out, x);
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = fmaf(D[i], x[i], sm.y[buffer][at.token][at.cg + i]);
-        if (zp != nullptr) {
-          unpack<T, V>(z_out, g);
-#pragma unroll
-          for (int i = 0; i < V; ++i) y[i] *= g[i] * sigmoid(g[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = on_out ? y[i] : 0.0f;
-        store_all<T, V>(reinterpret_cast<T*>(a.y) + ((int64_t)at.b * a.N + t) * a.C + at.c0 + at.cg, y, at.count, WIDE);
-      }
-    }
+    if (!SPLIT) read_out(t0 + at.token, buffer);
   }
+  if (SPLIT && stages) read_out(at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile + at.token, buffer ^ 1);
+  if (!walks) return;
   if (at.channel < 0) return;
   if (ENDS) {
     store_pairs<P>(p.carry + carry_at, h);
@@ -758,19 +772,23 @@ template <typename T, typename K, bool BACKWARD>
 int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
   using Smem = typename std::conditional<BACKWARD, BackwardSmem<K>, ForwardSmem<K>>::type;
   static_assert(sizeof(Smem) <= (size_t)kMaxDynamicSmem, "shared memory");
+  const dim3 grid((unsigned)(p.a.B * (int64_t)p.segments), (unsigned)(p.a.G * p.blocks_c));
+  // Where every block has an SM of its own, twice the threads hide what lies between two walks (B=4 N=4096 C=2048 bf16: 340 us, 395 without; N=2048 fp32: 184,
+  // 278); where blocks share one, they do that for one another (B=8 N=2048 C=4096: 666 us, 590 without).
+  const bool split = !BACKWARD && !ends && p.wide && (int64_t)grid.x * grid.y <= sm_count();
   const auto pick = [&](auto ends_, auto wide, auto docs) -> void (*)(ScanParams) {
     constexpr bool E = decltype(ends_)::value, W = decltype(wide)::value, DOCS = decltype(docs)::value;
     if constexpr (BACKWARD) return backward_kernel<T, K, E, W, DOCS>;
-    else return forward_kernel<T, K, E, W, DOCS>;
+    else if constexpr (E) return forward_kernel<T, K, E, W, DOCS, false>;
+    else return split ? forward_kernel<T, K, E, W, DOCS, true> : forward_kernel<T, K, E, W, DOCS, false>;
   };
   const auto with_docs = [&](auto ends_, auto wide) { return p.a.documents != nullptr ? pick(ends_, wide, std::true_type()) : pick(ends_, wide, std::false_type()); };
   const auto with_wide = [&](auto ends_) { return p.wide ? with_docs(ends_, std::true_type()) : with_docs(ends_, std::false_type()); };
   auto* const kernel = ends ? with_wide(std::true_type()) : with_wide(std::false_type());
-  const dim3 grid((unsigned)(p.a.B * (int64_t)p.segments), (unsigned)(p.a.G * p.blocks_c));
   FLARE_CUDA_CHECK(allow_smem(kernel));
   LaunchTimer timer(BACKWARD ? (ends ? "scan_backward_kernel (ends)" : "scan_backward_kernel") : (ends ? "scan_forward_kernel (ends)" : "scan_forward_kernel"),
                     stream);
-  FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(K::THREADS), sizeof(Smem), stream, p));
+  FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(split ? 2 * K::THREADS : K::THREADS), sizeof(Smem), stream, p));
   return FLARE_OK;
 }
 
