@@ -18,8 +18,8 @@
 // tile.  A tile is walked forward once (which leaves the states in front of every eight tokens in shared memory), then eight
 // tokens at a time are recomputed, with their factors, and walked in reverse.  The gradients of b and c are sums over channels: over
 // the channels of a warp by exchanges that halve the values they carry, over a block's warps in shared memory, over blocks in order
-// by a kernel of their own.  No atomics: the same call gives the same bits.  The same sizes: 1 169 us; eight warps an SM, which is all that
-// there are channels for, issue in every second cycle.
+// by a kernel of their own.  No atomics: the same call gives the same bits.  The same sizes: 1 053 us, bound by latencies: eight warps an SM walk,
+// which is all that there are channels for.
 #include "selective_scan.cuh"
 
 #include "sm100_ptx.cuh"
@@ -36,8 +36,9 @@ using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int S_, int NS_, int THREADS_, int BLOCKS_ = 1, int CT_ = 1>
+template <int S_, int NS_, int THREADS_, int BLOCKS_ = 1, int CT_ = 1, int STAGERS_ = 0>
 struct Config {
+  static constexpr int STAGERS = STAGERS_;  // of the backward: threads that stage while the others walk (0: all do both)
   static constexpr int BLOCKS = BLOCKS_;  // of an SM, at least
   static constexpr int CT = CT_;          // channels of a thread, CH / CT apart (1 in the forward)
   static constexpr int SUB = 8;           // tokens that the backward recomputes at a time
@@ -62,13 +63,14 @@ struct ForwardSmem {
   Tile<K> in[2];
   float y[2][kTile][K::ROW];
 };
-template <typename K>
+template <typename K, bool SPLIT>
 struct BackwardSmem {
-  Tile<K> in;
-  float gy[kTile][K::ROW];
-  float p1[kTile][K::ROW], p2[kTile][K::ROW], y[kTile][K::ROW];
-  float bc[kTile][K::WARPS][2 * K::S];
-  alignas(16) float starts[kTile / K::SUB][K::THREADS][K::CT * K::NS];  // (each thread its own)
+  static constexpr int BUFFERS = SPLIT ? 2 : 1;
+  Tile<K> in[BUFFERS];
+  float gy[BUFFERS][kTile][K::ROW];
+  float p1[BUFFERS][kTile][K::ROW], p2[BUFFERS][kTile][K::ROW], y[BUFFERS][kTile][K::ROW];
+  float bc[BUFFERS][kTile][K::WARPS][2 * K::S];
+  alignas(16) float starts[kTile / K::SUB - 1][K::THREADS][K::CT * K::NS];  // (each thread its own)
 };
 
 // softplus(u) = max(u, 0) + log(1 + t), t = exp(-|u|), and its slope 1 / (1 + exp(-u)).  log(1 + t) = 2 atanh(s) with s = t / (2 + t) <= 1 / 3: the
@@ -85,16 +87,19 @@ __device__ __forceinline__ float softplus(float u, float& slope) {
   return fmaxf(u, 0.0f) + 2.0f * fmaf(s * q, a, s);
 }
 
-// Where a block and a thread work.  SPLIT: half of the threads stage, the others walk.
-template <typename K, bool SPLIT = false>
+// Where a block and a thread work.  A thread is one of K::THREADS: itself, HALVES: one of the first half (which walks) or of the second (which
+// stages), GIVEN: what the caller says.
+enum Who { ITSELF, HALVES, GIVEN };
+template <typename K, Who WHO = ITSELF>
 struct Place {
-  __device__ static __forceinline__ unsigned tid() { return SPLIT ? threadIdx.x % K::THREADS : threadIdx.x; }
+  unsigned given;
+  __device__ __forceinline__ unsigned tid() const { return WHO == GIVEN ? given : WHO == HALVES ? threadIdx.x % K::THREADS : threadIdx.x; }
   int b, seg, t0, t1, len;   // tokens of the segment
   int group, c0, here;       // first channel of the block, how many it has
   int token, cg, count;      // staging: token of the tile, first of V channels, how many of them there are
   int ch, sub, channel;      // walking: channel of the block, part of its states, channel (-1: none)
   const int32_t* ids;
-  __device__ __forceinline__ Place(const ScanParams& p) {
+  __device__ __forceinline__ explicit Place(const ScanParams& p, unsigned given_ = 0) : given(given_) {
     const flare_scan_args_t& a = p.a;
     b = blockIdx.x / p.segments;
     seg = blockIdx.x % p.segments;
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(SPLIT ? 2 * K::THREADS : K::THREADS, SPLIT ? 1
   ForwardSmem<K>& sm = *reinterpret_cast<ForwardSmem<K>*>(smem);
   const flare_scan_args_t& a = p.a;
   const bool walks = !SPLIT || threadIdx.x < K::THREADS, stages = !SPLIT || !walks;
-  const Place<K, SPLIT> at(p);
+  const Place<K, SPLIT ? HALVES : ITSELF> at(p);
   if (ENDS && at.seg == p.segments - 1) return;  // (nothing follows it)
   constexpr int S = K::S, P = K::P, V = K::V, LANES = K::LANES;
   float bias[V], D[V];
@@ -399,13 +404,18 @@ __global__ void __launch_bounds__(SPLIT ? 2 * K::THREADS : K::THREADS, SPLIT ? 1
   }
 }
 
-template <typename T, typename K, bool ENDS, bool WIDE, bool DOCS>
-__global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const ScanParams p) {
+// SPLIT: the first K::THREADS threads walk, K::STAGERS more lay down the next tile and form the gradients of the last one meanwhile, each for as
+// many places of a tile as it takes
+template <typename T, typename K, bool ENDS, bool WIDE, bool DOCS, bool SPLIT>
+__global__ void __launch_bounds__(K::THREADS + (SPLIT ? K::STAGERS : 0), K::BLOCKS) backward_kernel(const ScanParams p) {
   pdl_wait();
   extern __shared__ __align__(16) uint8_t smem[];
-  BackwardSmem<K>& sm = *reinterpret_cast<BackwardSmem<K>*>(smem);
+  BackwardSmem<K, SPLIT>& sm = *reinterpret_cast<BackwardSmem<K, SPLIT>*>(smem);
   const flare_scan_args_t& a = p.a;
-  const Place<K> at(p);
+  constexpr int STAGERS = SPLIT ? K::STAGERS : K::THREADS, ROUNDS = K::THREADS / STAGERS;
+  const bool walks = !SPLIT || threadIdx.x < K::THREADS, stages = !SPLIT || !walks;
+  const unsigned self = SPLIT && !walks ? threadIdx.x - K::THREADS : threadIdx.x;
+  const Place<K, SPLIT ? GIVEN : ITSELF> at(p, self);
   if (ENDS && at.seg == 0) return;
   constexpr int S = K::S, P = K::P, NS = K::NS, V = K::V, LANES = K::LANES, SUB = K::SUB, CT = K::CT, APART = K::APART;
   float bias[V], D[V], sum_d[V], sum_bias[V];
@@ -435,37 +445,108 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
   const T* const zp = reinterpret_cast<const T*>(a.z);
   const int tiles = (a.N + kTile - 1) / kTile;
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
-  Rows<T, K, WIDE> rows;
-  Raw<T, V> dy, z;
-  uint64_t kept[CT][P];
+  // staging
+  Rows<T, K, WIDE> rows[ROUNDS];
+  Raw<T, V> dy[ROUNDS], z[ROUNDS];
+  const auto place = [&](int round) { return Place<K, SPLIT ? GIVEN : ITSELF>(p, self + round * STAGERS); };
   const auto fetch = [&](int t0) {
-    rows.load(p, at, t0);
-    const int t = t0 + at.token, n = rows.on ? at.count : 0;
-    dy = load_raw<T, V>(reinterpret_cast<const T*>(a.dy) + at.b * a.dy_stride_b + t * a.dy_stride_n + at.c0 + at.cg, n, WIDE);
-    if (zp != nullptr) z = load_raw<T, V>(zp + at.b * a.z_stride_b + t * a.z_stride_n + at.c0 + at.cg, n, WIDE);
-    if (!ENDS) {
 #pragma unroll
-      for (int j = 0; j < CT; ++j) load_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at(j), kept[j]);
+    for (int r = 0; r < ROUNDS; ++r) {
+      const auto here = place(r);
+      rows[r].load(p, here, t0);
+      const int t = t0 + here.token, n = rows[r].on ? here.count : 0;
+      dy[r] = load_raw<T, V>(reinterpret_cast<const T*>(a.dy) + at.b * a.dy_stride_b + t * a.dy_stride_n + at.c0 + at.cg, n, WIDE);
+      if (zp != nullptr) z[r] = load_raw<T, V>(zp + at.b * a.z_stride_b + t * a.z_stride_n + at.c0 + at.cg, n, WIDE);
     }
   };
-  fetch(last);
-#pragma unroll 1
-  for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
-    float delta[V], slope[V], x[V];
-    rows.stage(p, at, bias, sm.in, delta, slope, x);
-    const Raw<T, V> dy_raw = dy, z_raw = z;
-    const bool on = rows.on;
-    {
+  // what the gradients of a tile take (SPLIT: fetched and formed once more)
+  float delta[V], slope[V], x[V];
+  Raw<T, V> dy_raw, z_raw;
+  bool on = false;
+  const auto lay_down = [&](int buffer) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const auto here = place(r);
+      rows[r].stage(p, here, bias, sm.in[buffer], delta, slope, x);
+      dy_raw = dy[r];
+      z_raw = z[r];
+      on = rows[r].on;
       float g[V], zf[V];
-      unpack<T, V>(dy, g);
+      unpack<T, V>(dy_raw, g);
       if (zp != nullptr) {
-        unpack<T, V>(z, zf);
+        unpack<T, V>(z_raw, zf);
 #pragma unroll
         for (int i = 0; i < V; ++i) g[i] *= zf[i] * sigmoid(zf[i]);
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) sm.gy[at.token][at.cg + i] = on ? g[i] : 0.0f;
+      for (int i = 0; i < V; ++i) sm.gy[buffer][here.token][at.cg + i] = on ? g[i] : 0.0f;
     }
+  };
+  const auto gradients = [&](int t0, int buffer) {
+#pragma unroll 1
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int token = at.token + r * (STAGERS / K::PER), t = t0 + token;
+      if (SPLIT) {
+        on = at.on(t);
+        const int n = on ? at.count : 0;
+        const Raw<T, V> xr = load_raw<T, V>(reinterpret_cast<const T*>(a.x) + at.b * a.x_stride_b + t * a.x_stride_n + at.c0 + at.cg, n, WIDE);
+        const Raw<T, V> dr = load_raw<T, V>(reinterpret_cast<const T*>(a.dt) + at.b * a.dt_stride_b + t * a.dt_stride_n + at.c0 + at.cg, n, WIDE);
+        dy_raw = load_raw<T, V>(reinterpret_cast<const T*>(a.dy) + at.b * a.dy_stride_b + t * a.dy_stride_n + at.c0 + at.cg, n, WIDE);
+        if (zp != nullptr) z_raw = load_raw<T, V>(zp + at.b * a.z_stride_b + t * a.z_stride_n + at.c0 + at.cg, n, WIDE);
+        unpack<T, V>(xr, x);
+        unpack<T, V>(dr, delta);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          delta[i] += bias[i];
+          slope[i] = 1.0f;
+          if (a.dt_softplus) delta[i] = softplus(delta[i], slope[i]);
+        }
+      }
+      if (t >= at.t1 || at.count <= 0) continue;
+      float dx[V], ddt[V], dyf[V], gate[V], zf[V];
+      unpack<T, V>(dy_raw, dyf);
+      if (zp != nullptr) unpack<T, V>(z_raw, zf);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float p1 = sm.p1[buffer][token][at.cg + i], gy = sm.gy[buffer][token][at.cg + i];
+        ddt[i] = fmaf(x[i], p1, sm.p2[buffer][token][at.cg + i] * (1.0f / kLog2e)) * slope[i];
+        dx[i] = fmaf(delta[i], p1, D[i] * gy);
+        if (!on) dx[i] = ddt[i] = 0.0f;
+        sum_bias[i] += ddt[i];
+        if (on) sum_d[i] = fmaf(gy, x[i], sum_d[i]);
+      }
+      const int64_t row = ((int64_t)at.b * a.N + t) * a.C + at.c0 + at.cg;
+      store_all<T, V>(reinterpret_cast<T*>(a.dx) + row, dx, at.count, WIDE);
+      store_all<T, V>(reinterpret_cast<T*>(a.ddt) + row, ddt, at.count, WIDE);
+      if (zp != nullptr) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float r = sigmoid(zf[i]);
+          gate[i] = on ? dyf[i] * fmaf(D[i], x[i], sm.y[buffer][token][at.cg + i]) * r * fmaf(zf[i], 1.0f - r, 1.0f) : 0.0f;
+        }
+        store_all<T, V>(reinterpret_cast<T*>(a.dz) + row, gate, at.count, WIDE);
+      }
+    }
+#pragma unroll (SPLIT ? 2 : 1)
+    for (int idx = self; idx < kTile * 2 * S; idx += STAGERS) {
+      const int tt = idx / (2 * S), j = idx % (2 * S);
+      if (t0 + tt < at.t1) {
+        float v = sm.bc[buffer][tt][0][j];
+#pragma unroll
+        for (int w = 1; w < K::WARPS; ++w) v += sm.bc[buffer][tt][w][j];
+        p.partial_bc[(((int64_t)at.b * a.N + t0 + tt) * gridDim.y + blockIdx.y) * (2 * S) + j] = v;
+      }
+    }
+  };
+  uint64_t kept[CT][P];  // the states in front of a tile
+  const auto fetch_states = [&](int t0) {
+    if (ENDS) return;
+#pragma unroll
+    for (int j = 0; j < CT; ++j) load_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at(j), kept[j]);
+  };
+  const auto walk = [&](int t0, int buffer) {
+    const Tile<K>& in = sm.in[buffer];
+    const auto& gys = sm.gy[buffer];
     uint64_t h[CT][P], tile_dA[CT][P];  // (summed tile by tile: thousands of tokens one by one would lose digits)
 #pragma unroll
     for (int j = 0; j < CT; ++j)
@@ -474,21 +555,25 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
         h[j][i] = kept[j][i];
         tile_dA[j][i] = 0;
       }
-    __syncthreads();
-    if (t0 > at.t0) fetch(t0 - kTile);
+    uint64_t first[CT][P];
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+#pragma unroll
+      for (int i = 0; i < P; ++i) first[j][i] = kept[j][i];
+    if (t0 > at.t0) fetch_states(t0 - kTile);
     if (ENDS) {
 #pragma unroll 4
       for (int t = kTile - 1; t >= 0; --t) {
         uint64_t b[P], c[P];
-        load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
+        load_bc<P>(&in.bc[t][at.sub * P], b, c);
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          const uint64_t d2 = *reinterpret_cast<const uint64_t*>(&sm.in.dd[t][padded(at.ch + j * APART)]), gy = twice(sm.gy[t][at.ch + j * APART]);
+          const uint64_t d2 = *reinterpret_cast<const uint64_t*>(&in.dd[t][padded(at.ch + j * APART)]), gy = twice(gys[t][at.ch + j * APART]);
           sum[j] += low(d2);
 #pragma unroll
           for (int i = 0; i < P; ++i) G[j][i] = f2_mul(f2_fma(c[i], gy, G[j][i]), factor(A2[j][i], d2));
         }
-        if (DOCS && sm.in.reset[t]) {
+        if (DOCS && in.reset[t]) {
 #pragma unroll
           for (int j = 0; j < CT; ++j) {
 #pragma unroll
@@ -499,17 +584,17 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
       }
     } else {
       const auto move = [&](int t, uint64_t (&f)[CT][P]) {  // h over token t; its factors
-        if (DOCS && sm.in.reset[t]) {
+        if (DOCS && in.reset[t]) {
 #pragma unroll
           for (int j = 0; j < CT; ++j)
 #pragma unroll
             for (int i = 0; i < P; ++i) h[j][i] = 0;
         }
         uint64_t b[P], c[P];
-        load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
+        load_bc<P>(&in.bc[t][at.sub * P], b, c);
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch + j * APART)]);
+          const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t][padded(at.ch + j * APART)]);
           const uint64_t d2 = dd.x, x2 = dd.y;
 #pragma unroll
           for (int i = 0; i < P; ++i) {
@@ -521,7 +606,8 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
 #pragma unroll 1
       for (int q = 0; q < kTile / SUB; ++q) {
 #pragma unroll
-        for (int j = 0; j < CT; ++j) store_pairs<P>(&sm.starts[q][threadIdx.x][j * NS], h[j]);
+        for (int j = 0; j < CT; ++j)
+          if (q > 0) store_pairs<P>(&sm.starts[q - 1][threadIdx.x][j * NS], h[j]);
         if (q + 1 < kTile / SUB) {
 #pragma unroll
           for (int k = 0; k < SUB; ++k) {
@@ -535,9 +621,12 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
         uint64_t f[SUB][CT][P], behind[SUB][CT][P], start[CT][P];  // factors; states behind the tokens and in front of them all
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          load_pairs<P>(&sm.starts[q][threadIdx.x][j * NS], start[j]);
+          if (q > 0) load_pairs<P>(&sm.starts[q - 1][threadIdx.x][j * NS], start[j]);
 #pragma unroll
-          for (int i = 0; i < P; ++i) h[j][i] = start[j][i];
+          for (int i = 0; i < P; ++i) {
+            if (q == 0) start[j][i] = first[j][i];
+            h[j][i] = start[j][i];
+          }
         }
 #pragma unroll
         for (int k = 0; k < SUB; ++k) {
@@ -554,16 +643,16 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
           for (int k = LANES - 1; k >= 0; --k) {
             const int t = q * SUB + k0 + k;
             uint64_t b[P], c[P], db[P], dc[P];
-            load_bc<P>(&sm.in.bc[t][at.sub * P], b, c);
+            load_bc<P>(&in.bc[t][at.sub * P], b, c);
 #pragma unroll
             for (int j = 0; j < CT; ++j) {
-              const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&sm.in.dd[t][padded(at.ch + j * APART)]);
-              const uint64_t d2 = dd.x, x2 = dd.y, gy = twice(sm.gy[t][at.ch + j * APART]);
+              const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t][padded(at.ch + j * APART)]);
+              const uint64_t d2 = dd.x, x2 = dd.y, gy = twice(gys[t][at.ch + j * APART]);
               uint64_t s1 = 0, s2 = 0, s3 = 0;
 #pragma unroll
               for (int i = 0; i < P; ++i) {
                 const uint64_t g = f2_fma(c[i], gy, G[j][i]);
-                const uint64_t before = DOCS && sm.in.reset[t] ? 0 : k0 + k ? behind[k0 + k - 1][j][i] : start[j][i], now = behind[k0 + k][j][i];
+                const uint64_t before = DOCS && in.reset[t] ? 0 : k0 + k ? behind[k0 + k - 1][j][i] : start[j][i], now = behind[k0 + k][j][i];
                 const uint64_t next = f2_mul(g, f[k0 + k][j][i]), u = f2_mul(next, before);
                 s1 = i ? f2_fma(g, b[i], s1) : f2_mul(g, b[i]);
                 s2 = i ? f2_fma(u, A2[j][i], s2) : f2_mul(u, A2[j][i]);
@@ -573,7 +662,7 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
                 db[i] = j ? f2_fma(g, x2, db[i]) : f2_mul(g, x2);
                 dc[i] = j ? f2_fma(now, gy, dc[i]) : f2_mul(now, gy);
               }
-              if (DOCS && sm.in.reset[t]) {
+              if (DOCS && in.reset[t]) {
 #pragma unroll
                 for (int i = 0; i < P; ++i) G[j][i] = 0;
               }
@@ -594,16 +683,16 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
 #pragma unroll
               for (int i = 0; i < R; ++i) {
                 const int j = first + i;  // (dB of this thread's states, then dC)
-                sm.bc[t][threadIdx.x >> 5][(j / NS) * S + at.sub * NS + j % NS] = v[i];
+                sm.bc[buffer][t][threadIdx.x >> 5][(j / NS) * S + at.sub * NS + j % NS] = v[i];
               }
             }
           }
           const int t = q * SUB + k0 + at.sub;
 #pragma unroll
           for (int j = 0; j < CT; ++j) {
-            sm.p1[t][at.ch + j * APART] = lane_sums<LANES>(p1[j], at.sub);
-            sm.p2[t][at.ch + j * APART] = lane_sums<LANES>(p2[j], at.sub);
-            if (zp != nullptr) sm.y[t][at.ch + j * APART] = lane_sums<LANES>(yv[j], at.sub);
+            sm.p1[buffer][t][at.ch + j * APART] = lane_sums<LANES>(p1[j], at.sub);
+            sm.p2[buffer][t][at.ch + j * APART] = lane_sums<LANES>(p2[j], at.sub);
+            if (zp != nullptr) sm.y[buffer][t][at.ch + j * APART] = lane_sums<LANES>(yv[j], at.sub);
           }
         }
       }
@@ -612,43 +701,45 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
 #pragma unroll
         for (int i = 0; i < P; ++i) dA[j][i] = f2_add(dA[j][i], tile_dA[j][i]);
     }
-    __syncthreads();
-    if (ENDS) continue;
-    const int t = t0 + at.token;
-    if (t < at.t1 && at.count > 0) {
-      float dx[V], ddt[V], dyf[V], gate[V], zf[V];
-      unpack<T, V>(dy_raw, dyf);
-      if (zp != nullptr) unpack<T, V>(z_raw, zf);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float p1 = sm.p1[at.token][at.cg + i], gy = sm.gy[at.token][at.cg + i];
-        ddt[i] = fmaf(x[i], p1, sm.p2[at.token][at.cg + i] * (1.0f / kLog2e)) * slope[i];
-        dx[i] = fmaf(delta[i], p1, D[i] * gy);
-        if (!on) dx[i] = ddt[i] = 0.0f;
-        sum_bias[i] += ddt[i];
-        if (on) sum_d[i] = fmaf(gy, x[i], sum_d[i]);
-      }
-      const int64_t row = ((int64_t)at.b * a.N + t) * a.C + at.c0 + at.cg;
-      store_all<T, V>(reinterpret_cast<T*>(a.dx) + row, dx, at.count, WIDE);
-      store_all<T, V>(reinterpret_cast<T*>(a.ddt) + row, ddt, at.count, WIDE);
-      if (zp != nullptr) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float r = sigmoid(zf[i]);
-          gate[i] = on ? dyf[i] * fmaf(D[i], x[i], sm.y[at.token][at.cg + i]) * r * fmaf(zf[i], 1.0f - r, 1.0f) : 0.0f;
-        }
-        store_all<T, V>(reinterpret_cast<T*>(a.dz) + row, gate, at.count, WIDE);
-      }
+  };
+  if (stages) fetch(last);
+  if (walks) fetch_states(last);
+  if (SPLIT) {
+    if (stages) {
+      lay_down(0);
+      if (last > at.t0) fetch(last - kTile);
     }
-#pragma unroll
-    for (int idx = threadIdx.x; idx < kTile * 2 * S; idx += K::THREADS) {
-      const int tt = idx / (2 * S), j = idx % (2 * S);
-      if (t0 + tt < at.t1) {
-        float v = sm.bc[tt][0][j];
-#pragma unroll
-        for (int w = 1; w < K::WARPS; ++w) v += sm.bc[tt][w][j];
-        p.partial_bc[(((int64_t)at.b * a.N + t0 + tt) * gridDim.y + blockIdx.y) * (2 * S) + j] = v;
+    // (loops of their own: neither side's registers are the other's)
+    const auto tile_done = [] { asm volatile("bar.sync 1, %0;" ::"n"(K::THREADS + K::STAGERS) : "memory"); };
+    tile_done();
+    int buffer = 0;
+    if (walks) {
+#pragma unroll 1
+      for (int t0 = last; t0 >= at.t0; t0 -= kTile, buffer ^= 1) {
+        walk(t0, buffer);
+        tile_done();
       }
+    } else {
+#pragma unroll 1
+      for (int t0 = last; t0 >= at.t0; t0 -= kTile, buffer ^= 1) {
+        if (t0 < last) gradients(t0 + kTile, buffer ^ 1);
+        if (t0 > at.t0) {
+          lay_down(buffer ^ 1);
+          if (t0 - kTile > at.t0) fetch(t0 - 2 * kTile);
+        }
+        tile_done();
+      }
+      gradients(at.t0, buffer ^ 1);
+    }
+  } else {
+#pragma unroll 1
+    for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
+      lay_down(0);
+      __syncthreads();
+      if (t0 > at.t0) fetch(t0 - kTile);
+      walk(t0, 0);
+      __syncthreads();
+      if (!ENDS) gradients(t0, 0);
     }
   }
   if (ENDS) {
@@ -663,20 +754,22 @@ __global__ void __launch_bounds__(K::THREADS, K::BLOCKS) backward_kernel(const S
   float* out = p.partial_w + (int64_t)blockIdx.x * weight_sums(a);
 #pragma unroll
   for (int j = 0; j < CT; ++j)
-    if (there(j)) store_pairs<P>(out + weight_at(j), dA[j]);
+    if (walks && there(j)) store_pairs<P>(out + weight_at(j), dA[j]);
   // the sums that the staging threads hold, over the tokens of a tile
   __syncthreads();
+  if (stages) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    sm.p1[at.token][at.cg + i] = sum_d[i];
-    sm.p2[at.token][at.cg + i] = sum_bias[i];
+    for (int i = 0; i < V; ++i) {
+      sm.p1[0][at.token][at.cg + i] = sum_d[i];
+      sm.p2[0][at.token][at.cg + i] = sum_bias[i];
+    }
   }
   __syncthreads();
   if ((int)threadIdx.x < at.here) {
     float d = 0.0f, e = 0.0f;
-    for (int t = 0; t < kTile; ++t) {
-      d += sm.p1[t][threadIdx.x];
-      e += sm.p2[t][threadIdx.x];
+    for (int t = 0; t < STAGERS / K::PER; ++t) {
+      d += sm.p1[0][t][threadIdx.x];
+      e += sm.p2[0][t][threadIdx.x];
     }
     out[(int64_t)a.C * S + at.c0 + threadIdx.x] = d;
     out[(int64_t)a.C * (S + 1) + at.c0 + threadIdx.x] = e;
@@ -770,7 +863,8 @@ int launch_decode(const ScanParams& p, cudaStream_t stream) {
 
 template <typename T, typename K, bool BACKWARD>
 int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
-  using Smem = typename std::conditional<BACKWARD, BackwardSmem<K>, ForwardSmem<K>>::type;
+  constexpr bool STAGERS = BACKWARD && K::STAGERS > 0;
+  using Smem = typename std::conditional<BACKWARD, BackwardSmem<K, STAGERS>, ForwardSmem<K>>::type;
   static_assert(sizeof(Smem) <= (size_t)kMaxDynamicSmem, "shared memory");
   const dim3 grid((unsigned)(p.a.B * (int64_t)p.segments), (unsigned)(p.a.G * p.blocks_c));
   // Where every block has an SM of its own, twice the threads hide what lies between two walks (B=4 N=4096 C=2048 bf16: 340 us, 395 without; N=2048 fp32: 184,
@@ -778,7 +872,7 @@ int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
   const bool split = !BACKWARD && !ends && p.wide && (int64_t)grid.x * grid.y <= sm_count();
   const auto pick = [&](auto ends_, auto wide, auto docs) -> void (*)(ScanParams) {
     constexpr bool E = decltype(ends_)::value, W = decltype(wide)::value, DOCS = decltype(docs)::value;
-    if constexpr (BACKWARD) return backward_kernel<T, K, E, W, DOCS>;
+    if constexpr (BACKWARD) return backward_kernel<T, K, E, W, DOCS, STAGERS && !E>;
     else if constexpr (E) return forward_kernel<T, K, E, W, DOCS, false>;
     else return split ? forward_kernel<T, K, E, W, DOCS, true> : forward_kernel<T, K, E, W, DOCS, false>;
   };
@@ -788,7 +882,7 @@ int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
   FLARE_CUDA_CHECK(allow_smem(kernel));
   LaunchTimer timer(BACKWARD ? (ends ? "scan_backward_kernel (ends)" : "scan_backward_kernel") : (ends ? "scan_forward_kernel (ends)" : "scan_forward_kernel"),
                     stream);
-  FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(split ? 2 * K::THREADS : K::THREADS), sizeof(Smem), stream, p));
+  FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(split ? 2 * K::THREADS : K::THREADS + (STAGERS && !ends ? K::STAGERS : 0)), sizeof(Smem), stream, p));
   return FLARE_OK;
 }
 
@@ -808,9 +902,10 @@ int launch(Pass pass, const ScanParams& p, cudaStream_t stream) {
       return launch_walk<T, Config<32, 4, 256, 2>, false>(ends, p, stream);
     default:
       if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256>, true>(ends, p, stream);
-      // (16 states in twos, two channels a thread, whose sums over channels cost half the exchanges: B=4 N=4096 C=2048 1 169 us; one channel a thread
-      // and twice the threads 1 183; in fours 1 235 with the registers of one block on an SM, 2 000 where two share them)
-      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 256, 1, 2>, true>(ends, p, stream);
+      // (16 states in twos, two channels a thread, whose sums over channels cost half the exchanges, and four warps more that stage: B=4 N=4096 C=2048
+      // 1 053 us; without those 1 169; one channel a thread and twice the threads 1 183; in fours 1 235 with the registers of one block on an SM, 2 000
+      // where two share them.  With `setmaxnreg` between the two sides 1 711, spills; sums over lanes exchanged token by token, in fewer registers, 1 217)
+      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 256, 1, 2, 128>, true>(ends, p, stream);
       return launch_walk<T, Config<32, 4, 256>, true>(ends, p, stream);
   }
 }
