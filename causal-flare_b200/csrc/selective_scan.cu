@@ -8,7 +8,7 @@
 // once per state), twice, so that the next tile is laid down while this one is walked (by threads of their own, where a block has an SM to itself) and a tile
 // costs one barrier; the rows of the tile after that are on their way into registers meanwhile.  The recurrence's products are packed in pairs.  The sum over a
 // channel's states is taken for as many tokens as the channel has threads at a time: three exchanges for four tokens.  B200, B=4 N=4096 C=2048 S=16
-// bf16: 340 us (the exponentials alone: 120; what is issued and its latencies bound it).
+// bf16: 317 us (the exponentials alone: 120; what is issued and its latencies bound it).
 //
 // Few channels: a row's tokens are cut into segments that run side by side.  A first pass over all segments but the last forms
 // what each leaves behind from a zero state (every exponential once more, no read-out), a small kernel joins them in order
@@ -335,6 +335,36 @@ __global__ void __launch_bounds__(SPLIT ? 2 * K::THREADS : K::THREADS, SPLIT ? 1
     for (int i = 0; i < V; ++i) y[i] = on_out ? y[i] : 0.0f;
     store_all<T, V>(reinterpret_cast<T*>(a.y) + ((int64_t)at.b * a.N + t) * a.C + at.c0 + at.cg, y, at.count, WIDE);
   };
+  const auto walk = [&](int t0, int buffer) {
+    const Tile<K>& in = sm.in[buffer];
+    if (!ENDS && a.keep != nullptr && at.channel >= 0)
+      store_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at, h);
+    constexpr int STEP = ENDS ? 4 : LANES;
+#pragma unroll(ENDS ? 4 : kTile / STEP)
+    for (int t = 0; t < kTile; t += STEP) {
+      float v[STEP];
+#pragma unroll
+      for (int k = 0; k < STEP; ++k) {
+        if (DOCS && in.reset[t + k]) {
+#pragma unroll
+          for (int i = 0; i < P; ++i) h[i] = 0;
+          if (ENDS) sum = -INFINITY;
+        }
+        const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t + k][padded(at.ch)]);
+        const uint64_t d2 = dd.x, x2 = dd.y;
+        uint64_t b[P], c[P], acc = 0;
+        load_bc<P>(&in.bc[t + k][at.sub * P], b, c);
+        if (ENDS) sum += low(d2);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          h[i] = f2_fma(factor(A2[i], d2), h[i], f2_mul(x2, b[i]));
+          if (!ENDS) acc = i ? f2_fma(h[i], c[i], acc) : f2_mul(h[i], c[i]);
+        }
+        v[k] = pair_sum(acc);
+      }
+      if constexpr (!ENDS) sm.y[buffer][t + at.sub][at.ch] = lane_sums<LANES>(v, at.sub);
+    }
+  };
   if (stages) {
     fetch(at.t0);
     lay_down(0);
@@ -343,58 +373,49 @@ __global__ void __launch_bounds__(SPLIT ? 2 * K::THREADS : K::THREADS, SPLIT ? 1
     on_now = rows.on;
     if (at.t0 + kTile < at.t1) fetch(at.t0 + kTile);
   }
-  __syncthreads();
+  const auto stage = [&](int t0, int buffer) {  // the next tile, while this one is walked
+    x_out = x_now;
+    z_out = z_now;
+    on_out = on_now;
+    if (t0 + kTile < at.t1) {
+      lay_down(buffer ^ 1);
+      x_now = rows.x;
+      z_now = z;
+      on_now = rows.on;
+      if (t0 + 2 * kTile < at.t1) fetch(t0 + 2 * kTile);
+    }
+  };
   int buffer = 0;
-#pragma unroll 1
-  for (int t0 = at.t0; t0 < at.t1; t0 += kTile, buffer ^= 1) {
+  if constexpr (SPLIT) {
+    // (loops of their own: neither side's registers are the other's)
+    const auto tile_done = [] { asm volatile("bar.sync 1, %0;" ::"n"(2 * K::THREADS) : "memory"); };
+    tile_done();
     if (walks) {
-      const Tile<K>& in = sm.in[buffer];
-      if (!ENDS && a.keep != nullptr && at.channel >= 0)
-        store_pairs<P>(a.keep + ((int64_t)at.b * tiles + t0 / kTile) * a.C * S + weight_at, h);
-      constexpr int STEP = ENDS ? 4 : LANES;
-#pragma unroll(16 / STEP)
-      for (int t = 0; t < kTile; t += STEP) {
-        float v[STEP];
-#pragma unroll
-        for (int k = 0; k < STEP; ++k) {
-          if (DOCS && in.reset[t + k]) {
-#pragma unroll
-            for (int i = 0; i < P; ++i) h[i] = 0;
-            if (ENDS) sum = -INFINITY;
-          }
-          const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(&in.dd[t + k][padded(at.ch)]);
-          const uint64_t d2 = dd.x, x2 = dd.y;
-          uint64_t b[P], c[P], acc = 0;
-          load_bc<P>(&in.bc[t + k][at.sub * P], b, c);
-          if (ENDS) sum += low(d2);
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            h[i] = f2_fma(factor(A2[i], d2), h[i], f2_mul(x2, b[i]));
-            if (!ENDS) acc = i ? f2_fma(h[i], c[i], acc) : f2_mul(h[i], c[i]);
-          }
-          v[k] = pair_sum(acc);
-        }
-        if constexpr (!ENDS) sm.y[buffer][t + at.sub][at.ch] = lane_sums<LANES>(v, at.sub);
+#pragma unroll 1
+      for (int t0 = at.t0; t0 < at.t1; t0 += kTile, buffer ^= 1) {
+        walk(t0, buffer);
+        tile_done();
       }
-    }
-    if (stages) {
-      if (SPLIT && t0 > at.t0) read_out(t0 - kTile + at.token, buffer ^ 1);
-      x_out = x_now;
-      z_out = z_now;
-      on_out = on_now;
-      if (t0 + kTile < at.t1) {
-        lay_down(buffer ^ 1);
-        x_now = rows.x;
-        z_now = z;
-        on_now = rows.on;
-        if (t0 + 2 * kTile < at.t1) fetch(t0 + 2 * kTile);
+    } else {
+#pragma unroll 1
+      for (int t0 = at.t0; t0 < at.t1; t0 += kTile, buffer ^= 1) {
+        if (t0 > at.t0) read_out(t0 - kTile + at.token, buffer ^ 1);
+        stage(t0, buffer);
+        tile_done();
       }
+      read_out(at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile + at.token, buffer ^ 1);
+      return;
     }
+  } else {
     __syncthreads();
-    if (!SPLIT) read_out(t0 + at.token, buffer);
+#pragma unroll 1
+    for (int t0 = at.t0; t0 < at.t1; t0 += kTile, buffer ^= 1) {
+      walk(t0, buffer);
+      stage(t0, buffer);
+      __syncthreads();
+      read_out(t0 + at.token, buffer);
+    }
   }
-  if (SPLIT && stages) read_out(at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile + at.token, buffer ^ 1);
-  if (!walks) return;
   if (at.channel < 0) return;
   if (ENDS) {
     store_pairs<P>(p.carry + carry_at, h);
@@ -867,7 +888,7 @@ int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
   using Smem = typename std::conditional<BACKWARD, BackwardSmem<K, STAGERS>, ForwardSmem<K>>::type;
   static_assert(sizeof(Smem) <= (size_t)kMaxDynamicSmem, "shared memory");
   const dim3 grid((unsigned)(p.a.B * (int64_t)p.segments), (unsigned)(p.a.G * p.blocks_c));
-  // Where every block has an SM of its own, twice the threads hide what lies between two walks (B=4 N=4096 C=2048 bf16: 340 us, 395 without; N=2048 fp32: 184,
+  // Where every block has an SM of its own, twice the threads hide what lies between two walks (B=4 N=4096 C=2048 bf16: 317 us, 395 without; N=2048 fp32: 184,
   // 278); where blocks share one, they do that for one another (B=8 N=2048 C=4096: 666 us, 590 without).
   const bool split = !BACKWARD && !ends && p.wide && (int64_t)grid.x * grid.y <= sm_count();
   const auto pick = [&](auto ends_, auto wide, auto docs) -> void (*)(ScanParams) {
