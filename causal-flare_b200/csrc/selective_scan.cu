@@ -911,6 +911,7 @@ int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
 
 template <typename T>
 int launch(Pass pass, const ScanParams& p, cudaStream_t stream) {
+  constexpr int STAGERS = sizeof(T) == 2 ? 128 : 0;  // (the rows of fp32 take the registers that they would save: S=8 B=2 N=2048 C=2048 402 us, 321 without)
   const bool ends = pass == FORWARD_ENDS || pass == BACKWARD_ENDS;
   switch (pass) {
     case DECODE:
@@ -922,11 +923,11 @@ int launch(Pass pass, const ScanParams& p, cudaStream_t stream) {
       if (p.a.S == 16) return launch_walk<T, Config<16, 4, 256, 2>, false>(ends, p, stream);
       return launch_walk<T, Config<32, 4, 256, 2>, false>(ends, p, stream);
     default:
-      if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256>, true>(ends, p, stream);
+      if (p.a.S == 8) return launch_walk<T, Config<8, 2, 256, 1, 1, STAGERS>, true>(ends, p, stream);
       // (16 states in twos, two channels a thread, whose sums over channels cost half the exchanges, and four warps more that stage: B=4 N=4096 C=2048
       // 1 053 us; without those 1 169; one channel a thread and twice the threads 1 183; in fours 1 235 with the registers of one block on an SM, 2 000
       // where two share them.  With `setmaxnreg` between the two sides 1 711, spills; sums over lanes exchanged token by token, in fewer registers, 1 217)
-      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 256, 1, 2, 128>, true>(ends, p, stream);
+      if (p.a.S == 16) return launch_walk<T, Config<16, 2, 256, 1, 2, STAGERS>, true>(ends, p, stream);
       return launch_walk<T, Config<32, 4, 256>, true>(ends, p, stream);
   }
 }
