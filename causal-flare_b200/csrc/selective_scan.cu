@@ -887,6 +887,7 @@ int launch_walk(bool ends, const ScanParams& p, cudaStream_t stream) {
   constexpr bool STAGERS = BACKWARD && K::STAGERS > 0;
   using Smem = typename std::conditional<BACKWARD, BackwardSmem<K, STAGERS>, ForwardSmem<K>>::type;
   static_assert(sizeof(Smem) <= (size_t)kMaxDynamicSmem, "shared memory");
+  static_assert(K::CH == block_channels(K::S), "channels of a block");
   const dim3 grid((unsigned)(p.a.B * (int64_t)p.segments), (unsigned)(p.a.G * p.blocks_c));
   // Where every block has an SM of its own, twice the threads hide what lies between two walks (B=4 N=4096 C=2048 bf16: 317 us, 395 without; N=2048 fp32: 184,
   // 278); where blocks share one, they do that for one another (B=8 N=2048 C=4096: 666 us, 590 without).
@@ -938,9 +939,6 @@ template int launch<FLARE_SCAN_TYPE>(Pass, const ScanParams&, cudaStream_t);
 extern template int launch<float>(Pass, const ScanParams&, cudaStream_t);
 extern template int launch<__nv_bfloat16>(Pass, const ScanParams&, cudaStream_t);
 extern template int launch<__half>(Pass, const ScanParams&, cudaStream_t);
-
-// (the configurations of launch() above)
-Shape shape_of(int S, bool backward) { return S == 8 ? Shape{4, 256} : S == 16 ? (backward ? Shape{8, 512} : Shape{4, 256}) : Shape{8, 256}; }
 
 namespace {
 
@@ -994,11 +992,11 @@ int check(const flare_scan_args_t* args) {
 
 // Segments where the channels alone leave SMs idle: as many as fill two blocks per SM, of four tiles at least.  Below three they
 // do not pay for the pass over their ends.
-void plan(ScanParams& p, const flare_scan_args_t& a, bool backward) {
+void plan(ScanParams& p, const flare_scan_args_t& a) {
   memset(&p, 0, sizeof(p));
   p.a = a;
   p.channels = a.C / a.G;
-  const int block = shape_of(a.S, backward).channels();
+  const int block = block_channels(a.S);
   p.blocks_c = (p.channels + block - 1) / block;
   const int64_t blocks = (int64_t)a.B * a.G * p.blocks_c, tiles = (a.N + kTile - 1) / kTile;
   int64_t segments = 2 * (int64_t)sm_count() / blocks;
@@ -1062,7 +1060,7 @@ size_t flare_scan_keep_bytes(const flare_scan_args_t* args) {
 size_t flare_scan_forward_workspace_bytes(const flare_scan_args_t* args) {
   if (check(args)) return 0;
   ScanParams p;
-  plan(p, *args, false);
+  plan(p, *args);
   return carry_bytes(p);
 }
 
@@ -1072,7 +1070,7 @@ int flare_scan_forward(const flare_scan_args_t* args, flare_stream_t stream) {
   if (a.y == nullptr || (a.state_out != nullptr && a.state_out == a.state_in)) return FLARE_ERR_BAD_POINTER;
   if (a.documents != nullptr && (a.state_in != nullptr || a.state_out != nullptr)) return FLARE_ERR_BAD_CONFIG;
   ScanParams p;
-  plan(p, a, false);
+  plan(p, a);
   if (carry_bytes(p) > 0) {
     if (a.workspace == nullptr || a.workspace_bytes < carry_bytes(p)) return FLARE_ERR_WORKSPACE;
     take_carry(p, reinterpret_cast<uint8_t*>(a.workspace));
@@ -1085,7 +1083,7 @@ int flare_scan_forward(const flare_scan_args_t* args, flare_stream_t stream) {
 size_t flare_scan_backward_workspace_bytes(const flare_scan_args_t* args) {
   if (check(args)) return 0;
   ScanParams p;
-  plan(p, *args, true);
+  plan(p, *args);
   return carry_bytes(p) + partial_bc_bytes(p) + partial_w_bytes(p);
 }
 
@@ -1097,7 +1095,7 @@ int flare_scan_backward(const flare_scan_args_t* args, flare_stream_t stream) {
     return FLARE_ERR_BAD_POINTER;
   if (a.state_in != nullptr || a.state_out != nullptr || a.lengths != nullptr) return FLARE_ERR_BAD_CONFIG;
   ScanParams p;
-  plan(p, a, true);
+  plan(p, a);
   if (a.workspace == nullptr || a.workspace_bytes < flare_scan_backward_workspace_bytes(args)) return FLARE_ERR_WORKSPACE;
   uint8_t* ws = take_carry(p, reinterpret_cast<uint8_t*>(a.workspace));
   p.partial_bc = reinterpret_cast<float*>(ws);
@@ -1130,7 +1128,7 @@ int flare_scan_decode(const flare_scan_args_t* args, flare_stream_t stream) {
   if (const int rc = check(&a)) return rc;
   if (a.y == nullptr || a.state_out == nullptr) return FLARE_ERR_BAD_POINTER;
   ScanParams p;
-  plan(p, a, false);
+  plan(p, a);
   return run(DECODE, p, stream);
 }
 

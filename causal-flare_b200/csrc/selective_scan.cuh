@@ -9,18 +9,13 @@ namespace scan {
 
 constexpr int kTile = 32;  // tokens of a tile, and between two kept states
 
-// How a block works: threads of a channel (each with S / lanes states), threads
-struct Shape {
-  int lanes, threads;
-  int channels() const { return threads / lanes; }
-};
-Shape shape_of(int S, bool backward);
+constexpr int block_channels(int S) { return S == 32 ? 32 : 64; }  // of a block, in either direction
 
 struct ScanParams {
   flare_scan_args_t a;
   int wide;       // rows of x, dt, z, y, dy and their gradients in 16-byte pieces
   int channels;   // of a group
-  int blocks_c;   // blocks along a group's channels (of the kernels at hand: forward and backward differ)
+  int blocks_c;   // blocks along a group's channels
   int segments, seg_tokens;  // tokens of a row are cut into segments of whole tiles
   // of every segment: what it leaves behind from zero, then (after the join) what it starts from; the sum of its deltas,
   // -infinity: a document begins in it
