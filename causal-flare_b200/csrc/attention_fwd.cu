@@ -11,7 +11,7 @@
 //
 // Tensor memory: S / P of the groups, two buffers each, at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, the
 // first two tiles of K, four stages of a tile of V and one of K.  Floors per 64 keys and both groups, in cycles: products 1 024 (M = 128, N = 64 from shared memory: 1 280),
-// exponentials 1 024.  B200, B=2 N=4096 H=16 D=128 bf16: 150 us (0.55 of the measured matrix rate), with a cap 195: the caps' seven
+// exponentials 1 024.  B200, B=2 N=4096 H=16 D=128 bf16: 150 us (0.55 of the measured matrix rate), with a cap 192: the caps' seven
 // products and sums for every score come on top of a group's own work, which is what bounds either.
 #include <limits.h>
 
@@ -194,7 +194,12 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
       tmem_fence_regs(s[0]);
       tmem_fence_regs(s[1]);
       const bool full = __all_sync(0xffffffffu, keys.x <= key0 && keys.y >= key0 + kKeys) != 0;
-      const int from = keys.x - key0, to_ = keys.y - key0;
+      unsigned in_sight[2];  // a bit for every key
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int from = min(max(keys.x - key0 - c * 32, 0), 32), to_ = min(max(keys.y - key0 - c * 32, 0), 32);
+        in_sight[c] = (unsigned)(((1ull << to_) - 1) & ~((1ull << from) - 1));
+      }
       // Weights are formed in the frame so far, caps and biases on the way, the maximum behind them: only where it has grown too far (a
       // few of the first tiles) are they formed once more.  So no exponential waits for the maximum, and caps, biases and exponentials,
       // which have pipes of their own, are worked on side by side.  Not so the first tile, and what needs masks or the other form of caps.
@@ -238,7 +243,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
             for (int c = 0; c < 2; ++c)
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0u;
+                if (!(in_sight[c] >> k & 1)) s[c][k] = 0u;
           }
           cap_scores(s[0], series, sc.in);
           cap_scores(s[1], series, sc.in);
@@ -248,7 +253,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             if (BIAS) s[c][k] = __float_as_uint(fmaf(-sc.slope, fabsf(d0 - (float)(c * 32 + k)), __uint_as_float(s[c][k]) * sc.unit));
-            if (c * 32 + k < from || c * 32 + k >= to_) s[c][k] = 0xff800000u;  // -inf
+            if (!(in_sight[c] >> k & 1)) s[c][k] = 0xff800000u;  // -inf
           }
       }
 #pragma unroll
