@@ -170,13 +170,14 @@ struct DeltaParams {
   AttnParams p;
   const void *q, *k, *v, *dy;
   int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, dy_b, dy_n, dy_h;
-  float* delta;
+  float *delta, *dy_norm, *v_norm;  // (v_norm: [B][J][Nqp])
 };
 // Keys up to which a row's delta is the sum of P dP itself.  <dy, y> has y's rounding and that of the weights in y, about 2^-9 |dy| |v| / sqrt(keys),
 // which dS = P (dP - delta) keeps: with two to five keys dQ and dK were 1.7 to 4 times as far off as their own rounding, with 50 and more 1.1.
 constexpr int kFewKeys = 32;
 
-// -delta, delta = sum P dP = <dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  Bound by memory.
+// -delta, delta = sum P dP = <dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  For fp16 the norms too
+// from which the kernels behind it know how large dS can be.  Bound by memory: B=2 N=4096 H=16 D=128 29 us, in fp16 with the values' rows 45.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ DeltaParams d) {
   pdl_begin();
@@ -201,7 +202,10 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
     return s;
   };
   float dy[8] = {}, sum = 0.0f;
-  const int keys = r.y - r.x;
+  constexpr bool NORMS = std::is_same<T, __half>::value;
+  const int keys = r.y - r.x, kv = h / (p.H / p.J);
+  const bool value = NORMS && mine && h == kv * (p.H / p.J);  // (one of its heads looks at the token's value)
+  Raw8<T> own_value;
   const bool few = keys <= kFewKeys;
   if (mine) {  // (the loads do not wait for the row's keys)
     float y[8];
@@ -209,12 +213,12 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
     eight(p.y, (((int64_t)b * p.Nq + i) * p.H + h) * p.D, y);
     sum = dot(dy, y);
   }
+  if (NORMS) own_value = load_raw8<T>(reinterpret_cast<const T*>(d.v) + b * d.v_b + i * d.v_n + kv * d.v_h + lane * 8, value ? 8 : 0, true);
   sum = joined(sum);
   const int steps = __reduce_max_sync(0xffffffffu, few ? max(keys, 0) : 0);
   if (steps > 0) {
     float q[8] = {}, weights = 0.0f, weighted = 0.0f;
     if (mine) eight(d.q, b * d.q_b + i * d.q_n + h * d.q_h, q);
-    const int kv = h / (p.H / p.J);
     const float lse = few && keys > 0 ? p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] : 0.0f, slope = p.slopes != nullptr ? p.slopes[h] : 0.0f;
     constexpr int GROUP = 4;  // keys on their way together
     for (int t0 = 0; t0 < steps; t0 += GROUP) {
@@ -244,12 +248,52 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
     if (few) sum = weighted / weights;
   }
   if (keys <= 0) sum = 0.0f;
-  if (live && lane == 0) d.delta[((int64_t)b * p.H + h) * p.masks.Nqp + i] = -sum;
+  const int64_t at = ((int64_t)b * p.H + h) * p.masks.Nqp + i;
+  if (live && lane == 0) d.delta[at] = -sum;
+  if constexpr (NORMS) {
+    float v[8];
+    unpack8(own_value, v);
+    const float dy_norm = joined(dot(dy, dy)), v_norm = joined(dot(v, v));
+    if (live && lane == 0) {  // (comparisons with what is no number are false)
+      d.dy_norm[at] = keys > 0 && dy_norm < INFINITY ? dy_norm : 0.0f;
+      if (h == kv * (p.H / p.J)) d.v_norm[((int64_t)b * p.J + kv) * p.masks.Nqp + i] = keys > 0 && v_norm < INFINITY ? v_norm : 0.0f;
+    }
+  }
+}
+
+// The largest norms of a key head's tokens: |dy|^2 of its query heads, |v|^2.  One block for each: 6.5 us for two times 4 096 of them.
+__global__ void __launch_bounds__(1024) largest_norms_kernel(const float* dy_norm, const float* v_norm, float* out, int group, int Nqp) {
+  pdl_begin();
+  const int64_t head = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;  // key head of the batch
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float tops[2][32];
+  const auto largest = [&](const float* from, int64_t n) {  // (n: a multiple of 128)
+    float top = 0.0f;
+    for (int64_t i = threadIdx.x; i < n / 4; i += 1024) {
+      const float4 v = reinterpret_cast<const float4*>(from)[i];
+      top = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), top);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+  };
+  const float dy = largest(dy_norm + head * group * Nqp, (int64_t)group * Nqp), v = largest(v_norm + head * Nqp, Nqp);
+  if (lane == 0) {
+    tops[0][warp] = dy;
+    tops[1][warp] = v;
+  }
+  __syncthreads();
+  if (warp < 2) {
+    float top = tops[warp][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) out[head * 2 + warp] = top;
+  }
 }
 
 struct Layout {
   size_t range, query_span, key_span, dirty, ends, plan_bytes;  // in `plan`, or in front of the workspace
-  size_t delta, bytes;                                          // in the workspace
+  size_t delta, dy_norm, v_norm, largest_norms, bytes;          // in the workspace
   int Nqp, Nkp;
 };
 Layout layout(const flare_attention_args_t& a, bool backward) {
@@ -269,7 +313,11 @@ Layout layout(const flare_attention_args_t& a, bool backward) {
   l.ends = take((size_t)a.B * 4);
   l.plan_bytes = at;
   if (a.plan != nullptr) at = 0;
+  const bool norms = backward && a.dtype == FLARE_F16;
   l.delta = take(backward ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
+  l.dy_norm = take(norms ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
+  l.v_norm = take(norms ? (size_t)a.B * a.J * l.Nqp * 4 : 0);
+  l.largest_norms = take(norms ? (size_t)a.B * a.J * 8 : 0);
   l.bytes = at;
   return l;
 }
@@ -717,7 +765,7 @@ size_t flare_attention_forward_workspace_bytes(const flare_attention_args_t* arg
   return layout(*args, false).bytes;
 }
 size_t flare_attention_backward_workspace_bytes(const flare_attention_args_t* args) {
-  if (args == nullptr || args->B <= 0 || args->Nq <= 0 || args->Nk <= 0 || args->H <= 0) return 0;
+  if (args == nullptr || args->B <= 0 || args->Nq <= 0 || args->Nk <= 0 || args->H <= 0 || args->J <= 0) return 0;
   return layout(*args, true).bytes;
 }
 
@@ -742,8 +790,11 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   if (!workspace_fits(a, l)) return FLARE_ERR_WORKSPACE;
   AttnParams p;
   if (const int rc = begin(a, l, p, true, stream)) return rc;
-  float* const delta = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.workspace) + l.delta);
-  p.delta = delta;
+  uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
+  const auto floats = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
+  p.delta = floats(l.delta);
+  p.dy_norm = floats(l.dy_norm);
+  p.largest_norms = floats(l.largest_norms);
   const int lanes = a.D <= 64 ? 8 : 16;
   const int64_t blocks = ((int64_t)l.Nqp * a.H * lanes + 255) / 256;
   if (blocks * (256 / lanes) > UINT_MAX - 256 || a.B > 65535) return FLARE_ERR_UNSUPPORTED;
@@ -757,10 +808,17 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
     d.k_b = a.k_stride_b; d.k_n = a.k_stride_n; d.k_h = a.k_stride_h;
     d.v_b = a.v_stride_b; d.v_n = a.v_stride_n; d.v_h = a.v_stride_h;
     d.dy_b = a.dy_stride_b; d.dy_n = a.dy_stride_n; d.dy_h = a.dy_stride_h;
-    d.delta = delta;
+    d.delta = floats(l.delta);
+    d.dy_norm = floats(l.dy_norm);
+    d.v_norm = floats(l.v_norm);
     auto* const kernel = a.dtype == FLARE_F16 ? (lanes == 8 ? delta_kernel<__half, 8> : delta_kernel<__half, 16>)
                                               : (lanes == 8 ? delta_kernel<__nv_bfloat16, 8> : delta_kernel<__nv_bfloat16, 16>);
     FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(256), 0, stream, d));
+  }
+  if (a.dtype == FLARE_F16) {
+    LaunchTimer timer("attention_largest_norms_kernel", stream);
+    FLARE_CUDA_CHECK(launch_pdl(largest_norms_kernel, dim3((unsigned)a.J, (unsigned)a.B), dim3(1024), 0, stream, p.dy_norm, (const float*)floats(l.v_norm),
+                                floats(l.largest_norms), a.H / a.J, l.Nqp));
   }
   return launch_backward_tc(a, p, stream);
 }

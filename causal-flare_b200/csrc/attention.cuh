@@ -29,6 +29,9 @@ struct AttnParams {
   const float* slopes;
   float* lse;          // forward: written, may be null; backward: read
   const float* delta;  // backward: [B][H][Nqp] -<dy, y>
+  // backward, fp16: |dy|^2 of every query and head, [B][H][Nqp]; the largest |dy|^2 and |v|^2 of a key head's tokens, [B][J][2].  Padding, and norms
+  // that are not finite, count as 0.
+  const float *dy_norm, *largest_norms;
   void *y, *dq, *dk, *dv;
   int* err;
   int B, Nq, Nk, H, J, D;

@@ -11,6 +11,11 @@
 // other tile, with eight warps each (32 of the 64 columns a warp), so that one's exponentials run under the other's products.
 // B200, B=2 N=4096 H=16 D=128 bf16: 550 us for both kernels (0.67 of the measured matrix rate for 18 D), with a cap 632.
 //
+// fp16 holds 40 powers of two, and dS of ordinary gradients (1e-6) and of scaled ones (1e5) lie at its ends or behind them: dS is laid down times a
+// power of two, taken out again with the last product's factor.  |dS| <= 2 |dY| |V| of the longest rows, so 2^e |dS| <= 2^14 (and a factor of four
+// in hand for P above 1, which is as far off as large scores are): one e for a query, and for a key head's dK one for the row of the batch.  The sizes above:
+// 590 us in fp16, of which the norms that e is taken from are 20.
+//
 // Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P is rounded once, to the type of the
 // operands it meets; dS goes to its product as a rounded value and what that lost, rounded again: rounded once it made dK and dQ 1.6 times as far
 // off as their own rounding does.  Everything in front of that, and the sums, is fp32.
@@ -43,6 +48,14 @@ struct Layout {
   static constexpr int OWN = DB * 16384, TILE = DB * 8192;
   static constexpr int Y = 2 * OWN, MISC = Y + kStages * 2 * TILE, BYTES = MISC + (int)sizeof(Misc) + 1024;
 };
+
+// e of 2^e |dS| <= 2^14, |dS| <= 2 |dy| |v| (squares given; nothing to scale: 0).  Norms of fp16 rows are below 2^20: e >= -28; up to 60, where fp32
+// still holds everything.
+__device__ __forceinline__ int range_exponent(float dy2, float v2) {
+  const float bound = sqrtf(dy2) * sqrtf(v2);
+  return bound > 0.0f ? min(12 - ilogbf(bound), 60) : 0;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
 // contiguous bytes, 16-byte aligned on both sides
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -181,11 +194,23 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + slot * 128 + half * 32, td = ts + 64;
     float lse = -INFINITY, delta = 0.0f;  // (signs changed)
     int2 keys = make_int2(0, 0);
+    // fp16: dS times `up`, the sums of its products times `down`.  (Queries: P is not laid down, so that `up` can be part of it.)
+    float up = 1.0f, down = 1.0f;
+    const float* const norms = F16 ? p.largest_norms + ((int64_t)b * p.J + (KEYS ? head : head / group)) * 2 : nullptr;
     if (!KEYS) {
       const int64_t at = ((int64_t)b * p.H + head) * p.masks.Nqp + row;
       lse = p.lse[at];
       delta = p.delta[at];
       keys = p.masks.range[(int64_t)b * p.masks.Nqp + row];
+      if (F16) {
+        const int e = range_exponent(p.dy_norm[at], norms[1]);
+        lse += (float)e;
+        down = power_of_two(-e);
+      }
+    } else if (F16) {
+      const int e = range_exponent(norms[0], norms[1]);
+      up = power_of_two(e);
+      down = power_of_two(-e);
     }
     ScoreScale sc = score_scale(p, KEYS ? head * group : head);
     const CapSeries series(sc.in);
@@ -280,7 +305,8 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
               w0 = ex2_approx(w0);
               w1 = ex2_approx(w1);
               uint64_t g = f2_mul(f2_pack(w0, w1), f2_add(f2_pack(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), e ? d4.y : d4.x));
-              if (CAP) g = f2_mul(g, f2_fma(f2_mul(t, twice(-1.0f)), t, twice(1.0f)));
+              if (CAP) g = f2_mul(g, f2_fma(f2_mul(t, twice(-up)), t, twice(up)));
+              else if (F16 && KEYS) g = f2_mul(g, twice(up));
               f2_unpack(g, g0, g1);
               if (MASKED) {
                 w0 = on >> k & 1 ? w0 : 0.0f;
@@ -326,10 +352,10 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
       if (KEYS) {  // a sum for the groups of a slot, half the columns each
 #pragma unroll
         for (int c = 0; c < DB; ++c)
-          if (slot == 0) put(p.dk, T_DS, half * DB + c, p.scale);
+          if (slot == 0) put(p.dk, T_DS, half * DB + c, p.scale * down);
           else put(p.dv, T_P, half * DB + c, 1.0f);
       } else if (slot * 2 + half < 2 * DB) {  // 32 columns each
-        put(p.dq, T_DS, slot * 2 + half, p.scale);
+        put(p.dq, T_DS, slot * 2 + half, p.scale * down);
       }
     }
   }

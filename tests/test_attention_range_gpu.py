@@ -1,0 +1,135 @@
+"""gpu: attention at the ends of what its types hold: gradients in fp16 that are small or large."""
+import pytest
+import torch
+
+import causal_flare as cf
+from oracle import mixers_oracle as orc
+
+pytestmark = pytest.mark.gpu
+HALF = 2.0 ** -11  # half a step of fp16
+STEP = 2.0 ** -25  # half the smallest step of fp16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def gradients(q, k, v, dy, **how):
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    y = cf.flare_causal_attention(q, k, v, **how)
+    return torch.autograd.grad(y, (q, k, v), dy)
+
+
+def exact(q, k, v, dy, scale, **how):
+    see = orc.in_sight(q.shape[1], how.get("documents"), None, how.get("window")).to(q.device)
+    s = how.get("slopes")
+    o = orc.Attention(q.double(), k.double(), v.double(), see, scale, how.get("cap"), None if s is None else s.double(), dy=dy.double())
+    return o.dq, o.dk, o.dv
+
+
+def near(got, want, off, what):
+    """Norms: `off` of the result's, and the rounding of values below fp16's normal numbers."""
+    assert torch.isfinite(got).all(), what
+    err, ref = float((got.double() - want).norm()), float(want.norm())
+    assert err <= off * ref + STEP * want.numel() ** 0.5, f"{what}: {err / ref:.2e}, {off:.2e} allowed"
+
+
+# Rows of at most 32 keys sum P dP itself, so dQ and dK are as near as their own rounding (1.01: of what is not quite the result), dS in two parts (half^2)
+# and fp32 allow.  fp32: exponents of up to 17 (scores up to 12) are off by 2^-22 a few times over, dP - delta is a third of either: 100 2^-22.
+OFF = 1.01 * HALF + HALF ** 2 + 100 * 2.0 ** -22
+
+
+SIZES = [  # of dy and of v; scale
+    (1e-6, 1, 16), (1e-5, 1, 16), (1e-4, 1, 16), (1, 1, 16), (1e-3, 1e-3, 16), (1e3, 1, 0.01), (3e3, 8, 0.01), (2, 1e4, 0.01),
+]
+
+
+@pytest.mark.parametrize("cap", [None, 20.0])
+@pytest.mark.parametrize("wide", ["q", "k"])
+@pytest.mark.parametrize("size, values, scale", SIZES)
+def test_gradients_in_fp16_of_every_size(size, values, scale, wide, cap):
+    # dS of 1e-6 has five bits in fp16, and one of 1e5 none; dQ = scale dS K (`wide`: or dK) is a normal number in either case.  Scores have a deviation of 2.
+    B, N, H, J, D = 2, 300, 4, 2, 64
+    g = gen(int(1000 * size) + 3)
+    one = max(1.0, (0.25 / scale) ** 0.5)
+    q_size, k_size = (one, 0.25 / scale / one) if wide == "q" else (0.25 / scale / one, one)
+    q, k = (randn(g, B, N, H, D) * q_size).half(), (randn(g, B, N, J, D) * k_size).half()
+    v, dy = (randn(g, B, N, J, D) * values).half(), (randn(g, B, N, H, D) * size).half()
+    how = dict(window=32, cap=cap)
+    got, want = gradients(q, k, v, dy, scale=scale, **how), exact(q, k, v, dy, scale, **how)
+    near(got[0], want[0], OFF, "dq")
+    near(got[1], want[1], OFF, "dk")
+    near(got[2], want[2], OFF + 1.01 * HALF, "dv")  # (every weight rounded once as well)
+
+
+def test_rows_of_very_different_gradients_in_fp16():
+    # a document whose gradients are ten thousand times another's, in one row, and a row between theirs
+    B, N, H, D, scale = 2, 400, 2, 64, 16
+    g = gen(1)
+    q, k, v = (randn(g, B, N, H, D) * (0.25 / scale)).half(), randn(g, B, N, H, D, dtype=torch.float16), randn(g, B, N, H, D, dtype=torch.float16)
+    docs = (torch.arange(N, device="cuda")[None].repeat(B, 1) >= 170).int()
+    size = torch.where(docs == 0, 1.0, 1e-4)
+    size[1] = 1e-2
+    dy = (randn(g, B, N, H, D) * size[..., None, None]).half()
+    how = dict(window=32, documents=docs)
+    got, want = gradients(q, k, v, dy, scale=scale, **how), exact(q, k, v, dy, scale, **how)
+    for name, a, b in zip(("dq", "dk"), got, want):
+        for row, part in ((0, slice(0, 170)), (0, slice(170, N)), (1, slice(0, N))):
+            # (dK's sums go by the row's largest |dY| |V|: with a second part that ends 2^38 below it, terms of 1e-4 of that keep 24 bits)
+            near(a[row, part], b[row, part], OFF, name)
+
+
+def test_a_row_whose_gradient_is_not_finite_leaves_the_others_alone():
+    B, N, H, D = 2, 200, 2, 64
+    g = gen(2)
+    q, k, v, dy = (randn(g, B, N, H, D, dtype=torch.float16) for _ in range(4))
+    docs = (torch.arange(N, device="cuda")[None].repeat(B, 1) >= 100).int()
+    clean = gradients(q, k, v, dy, documents=docs)
+    for value in (float("inf"), float("nan")):
+        bad = dy.clone()
+        bad[0, 150, 1, 3] = value
+        got = gradients(q, k, v, bad, documents=docs)
+        # another document: all but dV, whose products have 0 times what is not finite, as they have in any form with matrix products
+        assert torch.equal(got[0][0, :100], clean[0][0, :100]) and torch.equal(got[1][0, :100], clean[1][0, :100])
+        for a, c in zip(got, clean):
+            assert torch.equal(a[1], c[1]) and torch.equal(a[0, :, 0], c[0, :, 0])  # another row of the batch, another head
+
+
+def test_gradients_of_nothing_are_nothing():
+    g = gen(4)
+    q, k, v = (randn(g, 1, 70, 2, 64, dtype=torch.float16) for _ in range(3))
+    for t in gradients(q, k, v, torch.zeros_like(q)):
+        assert not t.any()
+    dq, dk, dv = gradients(q, k, torch.zeros_like(v), torch.ones_like(q))
+    assert not dq.any() and not dk.any() and dv.any()
+
+
+def test_gradients_in_fp16_from_a_graph():
+    # replayed with gradients of another size: what they are scaled by is found anew
+    B, N, H, D = 2, 150, 2, 64
+    g = gen(5)
+    q, k, v, dy = (randn(g, B, N, H, D, dtype=torch.float16) for _ in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        return torch.autograd.grad(cf.flare_causal_attention(*leaves), leaves, dy)
+
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for size in (1, 1e3, 1e-4):
+        dy.copy_(randn(gen(6), B, N, H, D) * size)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
