@@ -170,7 +170,7 @@ struct DeltaParams {
   AttnParams p;
   const void *q, *k, *v, *dy;
   int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, dy_b, dy_n, dy_h;
-  float *delta, *dy_norm, *v_norm;  // (v_norm: [B][J][Nqp])
+  float *delta, *dy_norm, *v_norm, *lse_lifted;  // (v_norm: [B][J][Nqp])
 };
 // Keys up to which a row's delta is the sum of P dP itself.  <dy, y> has y's rounding and that of the weights in y, about 2^-9 |dy| |v| / sqrt(keys),
 // which dS = P (dP - delta) keeps: with two to five keys dQ and dK were 1.7 to 4 times as far off as their own rounding, with 50 and more 1.1.
@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
     unpack8(own_value, v);
     const float dy_norm = joined(dot(dy, dy)), v_norm = joined(dot(v, v));
     if (live && lane == 0) {  // (comparisons with what is no number are false)
+      d.lse_lifted[at] = p.lse[at] + (float)kWeightLift;
       d.dy_norm[at] = keys > 0 && dy_norm < INFINITY ? dy_norm : 0.0f;
       if (h == kv * (p.H / p.J)) d.v_norm[((int64_t)b * p.J + kv) * p.masks.Nqp + i] = keys > 0 && v_norm < INFINITY ? v_norm : 0.0f;
     }
@@ -292,8 +293,8 @@ __global__ void __launch_bounds__(1024) largest_norms_kernel(const float* dy_nor
 }
 
 struct Layout {
-  size_t range, query_span, key_span, dirty, ends, plan_bytes;  // in `plan`, or in front of the workspace
-  size_t delta, dy_norm, v_norm, largest_norms, bytes;          // in the workspace
+  size_t range, query_span, key_span, dirty, ends, plan_bytes;      // in `plan`, or in front of the workspace
+  size_t delta, dy_norm, v_norm, largest_norms, lse_lifted, bytes;  // in the workspace
   int Nqp, Nkp;
 };
 Layout layout(const flare_attention_args_t& a, bool backward) {
@@ -313,11 +314,12 @@ Layout layout(const flare_attention_args_t& a, bool backward) {
   l.ends = take((size_t)a.B * 4);
   l.plan_bytes = at;
   if (a.plan != nullptr) at = 0;
-  const bool norms = backward && a.dtype == FLARE_F16;
+  const bool f16 = backward && a.dtype == FLARE_F16;
   l.delta = take(backward ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
-  l.dy_norm = take(norms ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
-  l.v_norm = take(norms ? (size_t)a.B * a.J * l.Nqp * 4 : 0);
-  l.largest_norms = take(norms ? (size_t)a.B * a.J * 8 : 0);
+  l.dy_norm = take(f16 ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
+  l.lse_lifted = take(f16 ? (size_t)a.B * a.H * l.Nqp * 4 : 0);
+  l.v_norm = take(f16 ? (size_t)a.B * a.J * l.Nqp * 4 : 0);
+  l.largest_norms = take(f16 ? (size_t)a.B * a.J * 8 : 0);
   l.bytes = at;
   return l;
 }
@@ -600,7 +602,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * HALVES; ++e) {
-        s[n][e] = sm100::ex2_approx(s[n][e] - (top[e >> 1] == -INFINITY ? 0.0f : top[e >> 1]));
+        s[n][e] = sm100::ex2_approx(s[n][e] - (top[e >> 1] == -INFINITY ? 0.0f : top[e >> 1] - kFrameLift<F16>));
         sum[e >> 1] += s[n][e];
       }
     uint32_t w[2 * HALVES];
@@ -795,6 +797,7 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   p.delta = floats(l.delta);
   p.dy_norm = floats(l.dy_norm);
   p.largest_norms = floats(l.largest_norms);
+  p.lse_lifted = floats(l.lse_lifted);
   const int lanes = a.D <= 64 ? 8 : 16;
   const int64_t blocks = ((int64_t)l.Nqp * a.H * lanes + 255) / 256;
   if (blocks * (256 / lanes) > UINT_MAX - 256 || a.B > 65535) return FLARE_ERR_UNSUPPORTED;
@@ -811,6 +814,7 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
     d.delta = floats(l.delta);
     d.dy_norm = floats(l.dy_norm);
     d.v_norm = floats(l.v_norm);
+    d.lse_lifted = floats(l.lse_lifted);
     auto* const kernel = a.dtype == FLARE_F16 ? (lanes == 8 ? delta_kernel<__half, 8> : delta_kernel<__half, 16>)
                                               : (lanes == 8 ? delta_kernel<__nv_bfloat16, 8> : delta_kernel<__nv_bfloat16, 16>);
     FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(256), 0, stream, d));

@@ -8,6 +8,12 @@ namespace attn {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Powers of two by which fp16 weights are laid down above their value, so that those far below one (long rows, a key that takes nearly all) are normal
+// numbers too: forward, where the frame lets them grow to 2^8, and backward, where they are at most one (with a factor of four in hand).
+template <bool F16>
+constexpr float kFrameLift = F16 ? 7.0f : 0.0f;
+constexpr int kWeightLift = 14;
+
 // Which keys a query sees is always one interval, and both its ends grow with the query: whatever the mask, it is two numbers
 // per query, and the keys of a tile of queries (the queries of a tile of keys) are one interval too.
 struct Masks {
@@ -32,6 +38,7 @@ struct AttnParams {
   // backward, fp16: |dy|^2 of every query and head, [B][H][Nqp]; the largest |dy|^2 and |v|^2 of a key head's tokens, [B][J][2].  Padding, and norms
   // that are not finite, count as 0.
   const float *dy_norm, *largest_norms;
+  const float* lse_lifted;  // backward, fp16: lse + kWeightLift, for the kernel that lays weights down
   void *y, *dq, *dk, *dv;
   int* err;
   int B, Nq, Nk, H, J, D;

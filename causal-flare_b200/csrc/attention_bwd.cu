@@ -14,10 +14,10 @@
 // fp16 holds 40 powers of two, and dS of ordinary gradients (1e-6) and of scaled ones (1e5) lie at its ends or behind them: dS is laid down times a
 // power of two, taken out again with the last product's factor.  |dS| <= 2 |dY| |V| of the longest rows, so 2^e |dS| <= 2^14 (and a factor of four
 // in hand for P above 1, which is as far off as large scores are): one e for a query, and for a key head's dK one for the row of the batch.  The sizes above:
-// 590 us in fp16, of which the norms that e is taken from are 20.
+// 595 us in fp16, of which the norms that e is taken from are 20.
 //
 // Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P is rounded once, to the type of the
-// operands it meets; dS goes to its product as a rounded value and what that lost, rounded again: rounded once it made dK and dQ 1.6 times as far
+// operands it meets (in fp16 times 2^14: weights of 1e-5, of rows of 1e5 keys, lost two bits); dS goes to its product as a rounded value and what that lost, rounded again: rounded once it made dK and dQ 1.6 times as far
 // off as their own rounding does.  Everything in front of that, and the sums, is fp32.
 #include "attention_tc.cuh"
 
@@ -132,7 +132,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
         }
         if (KEYS) {
           const int64_t at = ((int64_t)b * p.H + hd) * p.masks.Nqp + row;
-          bulk_load(misc->stats[s].lse, p.lse + at, kWalk * 4, &misc->full[s]);
+          bulk_load(misc->stats[s].lse, (F16 ? p.lse_lifted : p.lse) + at, kWalk * 4, &misc->full[s]);
           bulk_load(misc->stats[s].delta, p.delta + at, kWalk * 4, &misc->full[s]);
           bulk_load(misc->stats[s].keys, p.masks.range + (int64_t)b * p.masks.Nqp + row, kWalk * 8, &misc->full[s]);
         }
@@ -194,7 +194,8 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + slot * 128 + half * 32, td = ts + 64;
     float lse = -INFINITY, delta = 0.0f;  // (signs changed)
     int2 keys = make_int2(0, 0);
-    // fp16: dS times `up`, the sums of its products times `down`.  (Queries: P is not laid down, so that `up` can be part of it.)
+    // fp16: dS times `up`, the sums of its products times `down`.  (Queries: P is not laid down, so that `up` can be part of it.  Keys: P has a factor of
+    // its own, which is part of lse.)
     float up = 1.0f, down = 1.0f;
     const float* const norms = F16 ? p.largest_norms + ((int64_t)b * p.J + (KEYS ? head : head / group)) * 2 : nullptr;
     if (!KEYS) {
@@ -209,7 +210,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
       }
     } else if (F16) {
       const int e = range_exponent(norms[0], norms[1]);
-      up = power_of_two(e);
+      up = power_of_two(e - kWeightLift);
       down = power_of_two(-e);
     }
     ScoreScale sc = score_scale(p, KEYS ? head * group : head);
@@ -353,7 +354,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
 #pragma unroll
         for (int c = 0; c < DB; ++c)
           if (slot == 0) put(p.dk, T_DS, half * DB + c, p.scale * down);
-          else put(p.dv, T_P, half * DB + c, 1.0f);
+          else put(p.dv, T_P, half * DB + c, F16 ? power_of_two(-kWeightLift) : 1.0f);
       } else if (slot * 2 + half < 2 * DB) {  // 32 columns each
         put(p.dq, T_DS, slot * 2 + half, p.scale * down);
       }

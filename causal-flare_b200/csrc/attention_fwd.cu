@@ -6,7 +6,8 @@
 // scores when it is done with a tile; with one buffer of 128 keys it waited
 // for its own two products and their hand-overs every time: 5 100 cycles for 128 keys, of which its own work took 3 000.
 // O stays in tensor memory; it is rescaled only where the maximum has grown by
-// more than 2^8 since the frame was set (exact: the frame cancels in O / l; P up to 2^8 is still far from the end of fp16).
+// more than 2^8 since the frame was set (exact: the frame cancels in O / l).  In fp16 P is laid down times 2^7: up to 2^15, and normal numbers down to
+// 2^-21 (a weight of 1.4 2^-20 beside one of 1 was 1.4 % off).
 // Sums are of the unrounded weights, in fp32; P is rounded once, to the type of V, which is what the products take.
 //
 // Tensor memory: S / P of the groups, two buffers each, at 0 and 128, O at 256 and 384.  Shared memory (D = 128): Q 64 KB, the
@@ -208,7 +209,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
       float part[4], t4[4];
       const auto weights = [&](auto raw_) {  // raw: the scores are products still
         constexpr bool RAW = decltype(raw_)::value;
-        const uint64_t frame2 = twice(m == -INFINITY ? 0.0f : -m), unit2 = twice(unit);
+        const uint64_t frame2 = twice(m == -INFINITY ? 0.0f : kFrameLift<F16> - m), unit2 = twice(unit);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -307,7 +308,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
         if (i < p.Nq) store_columns<F16>(y, c * 32, p.D, o, inv);
       }
       // with its sign changed, as the backward adds it (a query without keys: -inf, so that every weight formed with it is 0)
-      if (p.lse != nullptr && inside) p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum == 0.0f ? -INFINITY : -(m + __log2f(sum));
+      if (p.lse != nullptr && inside) p.lse[((int64_t)b * p.H + h) * p.masks.Nqp + i] = sum == 0.0f ? -INFINITY : -(m + (__log2f(sum) - kFrameLift<F16>));
     }
   }
   if (!ok) {

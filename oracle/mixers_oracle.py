@@ -93,12 +93,11 @@ def in_sight(N, documents=None, prefix=None, window=None):
 class Attention:
     """Softmax attention of q [B, N, H, D] over k, v [B, M, J, D] where ``see`` [B or 1, N, M] holds; positions of the queries: first
     [B] + 0..N-1.  With ``dy`` the gradients, in closed form.  ``eps``: half a step of the type that weights and outputs are rounded to; the
-    ``*_off`` are then bounds on how far a kernel that rounds P, dS and its outputs once, and computes in fp32 otherwise, may be off.  A
-    value below the type's normal numbers is off by up to half its smallest step, ``tiny``, instead (2^-25 in fp16, where a weight dS
-    of 2^-20 keeps four bits: the sum dk = scale sum dS q of n such terms may then be off by scale n 2^-25 |q|)."""
+    ``*_off`` are then bounds on how far a kernel that rounds P, dS and its outputs once, and computes in fp32 otherwise, may be off.  fp16 has steps of
+    2^-24 at its lower end, where half of one is what a value is off by: 2^-32 for weights that are laid down times 2^7, 2^-37 |dy| |v| (of the longest
+    rows) for dS that is laid down times the power of two that takes its bound, 2 |dy| |v|, to 2^13 at least."""
 
     def __init__(self, q, k, v, see, scale, cap=None, slopes=None, first=None, dy=None, eps=0.0):
-        tiny = 2.0 ** -25 if eps == 2.0 ** -11 else 0.0
         B, N, H, D = q.shape
         M, J = k.shape[1], k.shape[2]
         qh = q.transpose(1, 2)
@@ -117,8 +116,9 @@ class Attention:
         y = p @ vh
         # fp32: scores and exponents, a few units of 2^-22 of the largest score in sight
         f = 2.0 ** -21 * (1 + (s.abs() * see).amax((-1, -2), keepdim=True))
-        rounded = lambda x: torch.maximum(eps * x.abs(), torch.full_like(x, tiny)) * see  # noqa: E731
-        y_off = (rounded(p) + f * p) @ vh.abs() + eps * y.abs()
+        fp16 = eps == 2.0 ** -11
+        rounded = lambda x, floor=0.0: (eps * x.abs()).clamp(min=floor if fp16 else 0.0) * see  # noqa: E731
+        y_off = (rounded(p, 2.0 ** -32) + f * p) @ vh.abs() + eps * y.abs()
         back = lambda x: x.transpose(1, 2)  # noqa: E731
         fold = lambda x: back(x).reshape(B, M, J, H // J, D).sum(3)  # noqa: E731
         self.y, self.y_off = back(y), back(y_off)
@@ -129,8 +129,9 @@ class Attention:
         slope = 1 - t * t
         raw = p * (dp - (g * y).sum(-1, keepdim=True)) * some
         ds = raw * slope
-        ds_off = rounded(ds) + (ds.abs() + raw.abs()) * f + p * ((g.abs() * y_off).sum(-1, keepdim=True) + f * (g.abs() @ vh.abs().transpose(2, 3)))
+        floor = 2.0 ** -37 * float(dy.norm(dim=-1).amax() * v.norm(dim=-1).amax())
+        ds_off = rounded(ds, floor) + (ds.abs() + raw.abs()) * f + p * ((g.abs() * y_off).sum(-1, keepdim=True) + f * (g.abs() @ vh.abs().transpose(2, 3)))
         self.dq, self.dk, self.dv = back(scale * ds @ kh), fold(scale * ds.transpose(2, 3) @ qh), fold(p.transpose(2, 3) @ g)
         self.dq_off = back(scale * ds_off @ kh.abs()) + eps * self.dq.abs()
         self.dk_off = fold(scale * ds_off.transpose(2, 3) @ qh.abs()) + eps * self.dk.abs()
-        self.dv_off = fold((rounded(p) + f * p).transpose(2, 3) @ g.abs()) + eps * self.dv.abs()
+        self.dv_off = fold((rounded(p, 2.0 ** -32) + f * p).transpose(2, 3) @ g.abs()) + eps * self.dv.abs()

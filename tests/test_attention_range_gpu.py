@@ -1,4 +1,4 @@
-"""gpu: attention at the ends of what its types hold: gradients in fp16 that are small or large."""
+"""gpu: attention at the ends of what its types hold: gradients in fp16 that are small or large, weights below fp16's normal numbers."""
 import pytest
 import torch
 
@@ -133,3 +133,38 @@ def test_gradients_in_fp16_from_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("form", ["whole", "prompt", "step"])
+def test_small_weights_beside_a_large_one_in_fp16(form):
+    # the first key has a weight of one and a value of zero, the others 1.4 2^-20: fp16's steps there are a twenty-second of that.  Tolerance: half a step for a
+    # weight and for what comes out, scores of 20 that are off by 2^-19 in all, and products that add 16 tokens at a time, each sum cut off in its last bit (2^-23).
+    N, D = 3000, 64
+    q, k = torch.zeros(1, N, 1, D, device="cuda").half(), torch.zeros(1, N, 1, D, device="cuda").half()
+    v = torch.ones(1, N, 1, D, device="cuda").half()
+    q[..., 0] = 1
+    k[:, 0, :, 0] = 13.53
+    v[:, 0] = 0
+    w = torch.exp(-k[0, 0, 0, 0].double())
+    i = torch.arange(N, device="cuda", dtype=torch.float64)
+    want = i * w / (1 + i * w)
+    off = 2 * HALF + 2.0 ** -19 + N / 16 * 2.0 ** -23
+    if form == "whole":
+        y = cf.flare_causal_attention(q, k, v, scale=1.0)[0, :, 0]
+        dv = gradients(q, k, v, torch.full_like(v, 500), scale=1.0)[2][0, 1:, 0].double()
+        each = (500 * w / (1 + i * w)).flip(0).cumsum(0).flip(0)[1:, None]
+        normal = each[:, 0] > 2.0 ** -14
+        assert normal.sum() > 2900 and float(((dv - each).abs() / each)[normal].max()) <= off
+    else:
+        kc, vc = k.clone(), v.clone()
+        if form == "prompt":
+            y = cf.flare_causal_attention_prefill(q, k, v, kc, vc, scale=1.0)[0, :, 0]
+        else:
+            # so many rows that a cache is read by one block: a quarter of the keys meet the large one
+            want, rows = want[-1:], 75
+            kc, vc = (t.expand(rows, N, 8, D).contiguous() for t in (kc, vc))
+            one = [t[:, -1].expand(rows, 8, D).contiguous() for t in (q, k, v)]
+            y = cf.flare_causal_attention_decode(*one, kc, vc, torch.full((rows,), N - 1, device="cuda", dtype=torch.int32), scale=1.0)[0, :1]
+    assert float(((y.double() - want[:, None]).abs() - STEP).max() / want.max()) <= off
+    many = want > 0.1 * want.max()  # (of the others y is a few of fp16's smallest steps)
+    assert float(((y.double() - want[:, None]).abs() / want[:, None])[many].max()) <= off
