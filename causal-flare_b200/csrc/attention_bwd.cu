@@ -286,7 +286,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap tm_x0, const __gri
               for (int k = 0; k < 16; ++k)
                 if (!(on >> k & 1)) s[k] = 0u;
             }
-            cap_scores(s, series, sc.in);
+            cap_scores(s, series);
           }
 #pragma unroll
           for (int k4 = 0; k4 < 16; k4 += 4) {

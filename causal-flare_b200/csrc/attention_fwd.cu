@@ -234,7 +234,7 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
         f2_unpack(sum2[0], part[0], part[1]);
         f2_unpack(sum2[1], part[2], part[3]);
       };
-      const bool at_once = n > 0 && full && (!CAP || all_small(s[0], s[1], sc.in));
+      const bool at_once = n > 0 && full && (!CAP || all_small(s[0], s[1], series));
       if (at_once) {
         weights(std::true_type());
       } else {
@@ -246,8 +246,8 @@ attention_forward_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_
               for (int k = 0; k < 32; ++k)
                 if (!(in_sight[c] >> k & 1)) s[c][k] = 0u;
           }
-          cap_scores(s[0], series, sc.in);
-          cap_scores(s[1], series, sc.in);
+          cap_scores(s[0], series);
+          cap_scores(s[1], series);
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c)

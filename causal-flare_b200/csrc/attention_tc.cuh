@@ -27,10 +27,12 @@ __device__ __forceinline__ ScoreScale score_scale(const AttnParams& p, int h) {
   return s;
 }
 __device__ __forceinline__ uint64_t twice(float x) { return f2_pack(x, x); }
-// the polynomial's coefficients, for raw products
+// the polynomial's coefficients, for raw products.  The last one holds in^7: where that is no normal number of fp32 (scale / cap below 2^-17 or above 2^17)
+// the coefficients would be rounded to multiples of the smallest one, or infinite, and no score is small enough for them.
 struct CapSeries {
   uint64_t c[4];
-  __device__ __forceinline__ explicit CapSeries(float in) {
+  float in, limit;  // of |x|
+  __device__ __forceinline__ explicit CapSeries(float in_) : in(in_), limit(in_ >= 0x1p-17f && in_ <= 0x1p17f ? 0.35f : -1.0f) {
     const float q = in * in;
     c[0] = twice(0.9999998211860657f * in);
     c[1] = twice(-0.3333165645599365f * in * q);
@@ -54,14 +56,14 @@ __device__ __forceinline__ float largest(const uint32_t (&s)[N]) {
   return most;
 }
 // may the whole warp's raw products take the polynomial?
-__device__ __forceinline__ bool all_small(const uint32_t (&a)[32], const uint32_t (&b)[32], float in) {
-  return __all_sync(0xffffffffu, fmaxf(largest(a), largest(b)) * in <= 0.35f) != 0;
+__device__ __forceinline__ bool all_small(const uint32_t (&a)[32], const uint32_t (&b)[32], const CapSeries& series) {
+  return __all_sync(0xffffffffu, fmaxf(largest(a), largest(b)) * series.in <= series.limit) != 0;
 }
 
 // raw products, in place: tanh of the capped score.  Whole warp.
 template <int N>
-__device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const CapSeries& series, float in) {
-  if (__all_sync(0xffffffffu, largest(s) * in <= 0.35f)) {
+__device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const CapSeries& series) {
+  if (__all_sync(0xffffffffu, largest(s) * series.in <= series.limit)) {
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
       float lo, hi;
@@ -71,7 +73,7 @@ __device__ __forceinline__ void cap_scores(uint32_t (&s)[N], const CapSeries& se
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) s[k] = __float_as_uint(tanh_any(__uint_as_float(s[k]) * in));
+    for (int k = 0; k < N; ++k) s[k] = __float_as_uint(tanh_any(__uint_as_float(s[k]) * series.in));
   }
 }
 

@@ -1,4 +1,5 @@
-"""gpu: attention at the ends of what its types hold: gradients in fp16 that are small or large, weights below fp16's normal numbers."""
+"""gpu: attention at the ends of what its types hold: gradients in fp16 that are small or large, weights below fp16's normal numbers, scales
+and caps whose quotient is far from one."""
 import pytest
 import torch
 
@@ -168,3 +169,27 @@ def test_small_weights_beside_a_large_one_in_fp16(form):
     assert float(((y.double() - want[:, None]).abs() - STEP).max() / want.max()) <= off
     many = want > 0.1 * want.max()  # (of the others y is a few of fp16's smallest steps)
     assert float(((y.double() - want[:, None]).abs() / want[:, None])[many].max()) <= off
+
+
+@pytest.mark.parametrize("scale, cap", [(5e-4, 1024.0), (1e-5, 1000.0), (2e-9, 300.0), (1e4, 0.01), (0.125, 50.0)])
+def test_scales_and_caps_whose_quotient_is_far_from_one(scale, cap):
+    # Two keys, a score of 0.349 (before tanh) and one of 0, and a bias that makes them equal: y is the mean, and moves by half of what the
+    # score is off.  That is cap 2^-21 at most, and half a step for the weights and for y.
+    D = 64
+    side = (0.349 * cap / scale / D) ** 0.5
+    q = torch.full((1, 2, 1, D), side, device="cuda").half()
+    k = q.clone()
+    k[:, 1] = 0
+    score = cap * torch.tanh(scale * (q[0, 1, 0].double() @ k[0, 0, 0].double()) / cap)
+    v = torch.ones(1, 2, 1, D, device="cuda").half()
+    v[:, 1] = -1
+    dy = torch.ones_like(q)
+    how = dict(cap=cap, slopes=score[None].float())
+    score_off = cap * 2.0 ** -21 + 2 * float(score) * 2.0 ** -24
+    y = cf.flare_causal_attention(q, k, v, scale=scale, **how)
+    o = orc.Attention(q.double(), k.double(), v.double(), orc.in_sight(2).cuda(), scale, cap, how["slopes"].double())
+    assert float((y.double() - o.y).abs().max()) <= score_off / 2 + 2 * HALF
+    for name, a, b in zip(("dq", "dk", "dv"), gradients(q, k, v, dy, scale=scale, **how), exact(q, k, v, dy, scale, **how)):
+        near(a, b, OFF + score_off + HALF, name)
+    zero = torch.zeros_like(q)
+    assert torch.equal(cf.flare_causal_attention(zero, zero, v, scale=scale, cap=cap)[0, 1], torch.zeros(1, D, device="cuda").half())
