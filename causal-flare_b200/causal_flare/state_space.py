@@ -155,7 +155,7 @@ def flare_causal_conv_decode(x, weight, bias=None, state=None, *, activation=Non
     has_shape(name, "state", state, (B, W - 1, channels))
     same_dtype(name, x, state=state)
     same_device(name, x, state=state)
-    state = torch.zeros((B, W - 1, channels), device=x.device, dtype=x.dtype) if state is None else state.detach().contiguous()
+    given, state = state, torch.zeros((B, W - 1, channels), device=x.device, dtype=x.dtype) if state is None else state.detach().contiguous()
     y = torch.empty(shape, device=x.device, dtype=x.dtype)
     if y.numel():
         x, weight = rows(x), weight.contiguous()
@@ -164,7 +164,7 @@ def flare_causal_conv_decode(x, weight, bias=None, state=None, *, activation=Non
         a.state_out, a.y = state.data_ptr(), y.data_ptr()
         _mixers.run("flare_conv_decode", a, x.device)
         _mixers.written(state)
-    return y, state
+    return y, state if given is None or not given.is_contiguous() else given
 
 
 # ---- selective scan ----------------------------------------------------------------------------------------------------
@@ -341,11 +341,17 @@ def flare_selective_scan_decode(x, dt, A, B, C, state=None, *, D=None, z=None, d
         x, dt, B, C = (t[:, 0] if t.dim() >= 3 and t.shape[1] == 1 else t for t in (x, dt, B, C))
         z = z[:, 0] if z is not None and z.dim() == 3 and z.shape[1] == 1 else z
     B, C = _scan_args(name, x, dt, A, B, C, D, z, dt_bias, False)
-    state = _scan_state(name, x, state, A.shape[1])
+    given, state = state, _scan_state(name, x, state, A.shape[1])
     y = torch.empty(shape, device=x.device, dtype=x.dtype)
     if x.numel():
         a, held = _fill_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus)
         a.state_out, a.y = state.data_ptr(), y.data_ptr()
         _mixers.run("flare_scan_decode", a, x.device)
         _mixers.written(state)
-    return y, state
+    if given is None or not given.is_contiguous():
+        return y, state
+    if given.data_ptr() != state.data_ptr():  # (at an address that the kernel does not take)
+        with torch.inference_mode():
+            given.copy_(state)
+        _mixers.written(given)
+    return y, given
