@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
     }
     const int64_t row = (int64_t)b * a.H + h0 + h;
     if (p.splits == 1) {
-      store1(a.y, a.dtype, row * a.D + d, idle ? 0.0f : v / l);
+      store1(a.y, a.dtype, row * a.D + d, l == 0.0f ? 0.0f : v / l);  // (0: an idle row, or no score above -infinity)
     } else if (p.cluster) {
       joined[0][h][d] = v;  // (no other thread reads this one)
       if (d == 0) {
@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) decode_kernel(const DecodeP
           l = fmaf(sm100::ld_cluster_f32(sm100::mapa_shared(ends + h * 8 + 4, s)), f, l);
           v = fmaf(sm100::ld_cluster_f32(sm100::mapa_shared(sums + (h * (64 * DB + 2) + d) * 4, s)), f, v);
         }
-      store1(a.y, a.dtype, ((int64_t)b * a.H + h0 + h) * a.D + d, l == 0.0f ? 0.0f : v / l);  // (0: an idle row)
+      store1(a.y, a.dtype, ((int64_t)b * a.H + h0 + h) * a.D + d, l == 0.0f ? 0.0f : v / l);  // (0: see above)
     }
     __syncwarp();
     sm100::cluster_sync_all();  // (a block's shared memory is read by others until here)
@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeParams p) 
     l = fmaf(in[a.D + 1], f, l);
     v = fmaf(in[d], f, v);
   }
-  store1(a.y, a.dtype, idx, l == 0.0f ? 0.0f : v / l);  // (0: an idle row)
+  store1(a.y, a.dtype, idx, l == 0.0f ? 0.0f : v / l);  // (0: an idle row, or no score above -infinity)
 }
 
 int check_cache(const flare_cache_args_t* args, bool decode) {

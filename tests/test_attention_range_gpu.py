@@ -1,5 +1,5 @@
 """gpu: attention at the ends of what its types hold: gradients in fp16 that are small or large, weights below fp16's normal numbers, scales
-and caps whose quotient is far from one."""
+and caps whose quotient is far from one, scores of minus infinity."""
 import pytest
 import torch
 
@@ -193,3 +193,12 @@ def test_scales_and_caps_whose_quotient_is_far_from_one(scale, cap):
         near(a, b, OFF + score_off + HALF, name)
     zero = torch.zeros_like(q)
     assert torch.equal(cf.flare_causal_attention(zero, zero, v, scale=scale, cap=cap)[0, 1], torch.zeros(1, D, device="cuda").half())
+
+
+@pytest.mark.parametrize("L", [60, 700, 3000])
+def test_a_token_none_of_whose_scores_is_above_minus_infinity(L):
+    # no weights: zeros, in however many parts the cache is read
+    q, k = torch.full((2, 4, 64), 1e30, device="cuda").bfloat16(), torch.full((2, 2, 64), -1e30, device="cuda").bfloat16()
+    kc, vc = k[:, None].expand(2, L, 2, 64).contiguous(), torch.ones(2, L, 2, 64, device="cuda").bfloat16()
+    y = cf.flare_causal_attention_decode(q, k, torch.ones_like(k), kc, vc, torch.tensor([L - 1, 3], device="cuda", dtype=torch.int32))
+    assert not y.any()
