@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
         weighted = on ? fmaf(w, dp, weighted) : weighted;
       }
     }
-    if (few) sum = weighted / weights;
+    if (few) sum = weights == 0.0f ? 0.0f : weighted / weights;  // (0: no score above -infinity, and y is 0)
   }
   if (keys <= 0) sum = 0.0f;
   const int64_t at = ((int64_t)b * p.H + h) * p.masks.Nqp + i;

@@ -202,3 +202,12 @@ def test_a_token_none_of_whose_scores_is_above_minus_infinity(L):
     kc, vc = k[:, None].expand(2, L, 2, 64).contiguous(), torch.ones(2, L, 2, 64, device="cuda").bfloat16()
     y = cf.flare_causal_attention_decode(q, k, torch.ones_like(k), kc, vc, torch.tensor([L - 1, 3], device="cuda", dtype=torch.int32))
     assert not y.any()
+
+
+@pytest.mark.parametrize("N", [5, 200])
+def test_rows_none_of_whose_scores_is_above_minus_infinity(N):
+    q, k = torch.full((1, N, 2, 64), 1e30, device="cuda").bfloat16(), torch.full((1, N, 2, 64), -1e30, device="cuda").bfloat16()
+    v = torch.ones_like(k)
+    assert not cf.flare_causal_attention(q, k, v).any()
+    for t in gradients(q, k, v, torch.ones_like(q)):
+        assert not t.any()
