@@ -532,8 +532,10 @@ int flare_conv_backward(const flare_conv_args_t* args, flare_stream_t stream) {
 }
 
 int flare_conv_decode(const flare_conv_args_t* args, flare_stream_t stream) {
-  if (const int rc = check(args)) return rc;
-  const flare_conv_args_t& a = *args;
+  if (args == nullptr) return FLARE_ERR_BAD_POINTER;
+  flare_conv_args_t a = *args;
+  a.N = 1;
+  if (const int rc = check(&a)) return rc;
   if (a.y == nullptr || a.state_out == nullptr) return FLARE_ERR_BAD_POINTER;
   ConvParams p;
   p.a = a;
