@@ -26,7 +26,7 @@ from ._common import _resolve_attn_scale
 from ._mixers import has_shape, on_gpu, put_strides, same_device, same_dtype, tiled, whole_numbers
 
 
-def _attention_args(name, q, k, v, scale, cap, slopes, window, tokens):
+def _attention_args(name, q, k, v, scale, cap, slopes, window, tokens, differentiable=False):
     """Checks of what the three forms share; returns (scale, cap, window) as the kernels take them."""
     dims, layout = (4, "[B, N, heads, D]") if tokens else (3, "[B, heads, D] or [B, 1, heads, D]")
     if q.dim() != dims or k.dim() != dims or v.dim() != dims:
@@ -54,7 +54,7 @@ def _attention_args(name, q, k, v, scale, cap, slopes, window, tokens):
     has_shape(name, "slopes", slopes, (H,))
     if slopes is not None and slopes.dtype != torch.float32:
         raise ValueError(f"{name} expects slopes in torch.float32. Got {slopes.dtype}.")
-    if slopes is not None and slopes.requires_grad:
+    if differentiable and slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} forms no gradient of the slopes: pass them detached.")
     on_gpu(name, q)
     same_device(name, q, k=k, v=v, slopes=slopes)
@@ -124,15 +124,15 @@ class CausalAttention(autograd.Function):
 def flare_causal_attention(q, k, v, *, scale=None, cap=None, slopes=None, window=None, documents=None, prefix=None):
     """Causal attention (differentiable in q, k, v).  q [B, N, H, D]; k, v [B, N, J, D], bf16 or fp16, D a multiple of 8 up to 128.
 
-    ``scale`` defaults to D ** -0.5 (1 for D = 8, as in the FLARE operators); ``cap``, ``slopes`` [H] fp32, ``window``, ``documents`` and ``prefix`` as the module says.  Returns y
-    [B, N, H, D].  Softmax statistics and sums are in fp32; its weights meet V in the inputs' type.  The gradients are the same bits
+    ``scale`` defaults to D ** -0.5 (1 for D = 8, as in the FLARE operators); ``cap``, ``slopes`` [H] fp32 (which get no
+    gradient: while gradients are recorded they have to be detached), ``window``, ``documents`` and ``prefix`` as the module says.  Returns y [B, N, H, D].  Softmax statistics and sums are in fp32; its weights meet V in the inputs' type.  The gradients are the same bits
     in every call."""
     if q.is_cuda:
         y = _mixers.host().attention(q, k, v, scale, cap, slopes, window, documents, prefix)
         if y is not None:
             return y
     name = "flare_causal_attention"
-    how = _attention_args(name, q, k, v, scale, cap, slopes, window, True)
+    how = _attention_args(name, q, k, v, scale, cap, slopes, window, True, differentiable=True)
     documents = whole_numbers(name, "documents", documents, q.shape[:2])
     prefix = _truth(name, prefix, q.shape[:2])
     same_device(name, q, documents=documents, prefix=prefix)

@@ -492,10 +492,7 @@ bool score_inputs(const Tensor& q, const py::object& scale, const py::object& ca
     if (s->window > INT_MAX) s->window = INT_MAX;
   }
   if (!tensor_or_none(slopes, &s->slopes) || !fp32(s->slopes, q) || !vector(s->slopes, q.size(-2))) return false;
-  if (s->slopes.defined()) {
-    if (s->slopes.requires_grad()) return false;
-    s->slopes = s->slopes.contiguous();
-  }
+  if (s->slopes.defined()) s->slopes = s->slopes.detach().contiguous();
   return true;
 }
 bool truth(const py::object& o, const Tensor& x, Tensor* out) {
@@ -566,6 +563,7 @@ py::object attention(const Tensor& q, const Tensor& k, const Tensor& v, const py
   Scores s;
   Tensor ids, led;
   if (!plain_attention(q, k, v, 4) || !score_inputs(q, scale, cap, slopes, window, &s) || !truth(prefix, q, &led)) return py::none();
+  if (!slopes.is_none() && wants_grad(THPVariable_Unpack(slopes.ptr()))) return py::none();  // (they have no gradient)
   const c10::cuda::CUDAGuard guard(q.device());
   if (!whole(documents, q, q.sizes().slice(0, 2), &ids, true)) return py::none();
   if (wants_grad(q, k, v)) return py::cast(AttentionNode::apply(q, k, v, s.scale, s.cap, s.window, maybe(s.slopes), maybe(ids), maybe(led))[0]);

@@ -1,4 +1,4 @@
-"""gpu: calls of the mixers that their documentation allows: states at odd addresses."""
+"""gpu: calls of the mixers that their documentation allows: states at odd addresses, slopes that are parameters."""
 import pytest
 import torch
 
@@ -46,3 +46,25 @@ def test_a_captured_step_updates_a_state_at_an_odd_address():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want) and torch.equal(moved, state)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_slopes_that_are_parameters(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_mixers, "_host", Nothing())
+    g = gen(33)
+    q, k = randn(g, 2, 9, 4, 64, dtype=torch.float16), randn(g, 2, 9, 2, 64, dtype=torch.float16)
+    fixed = torch.rand(4, generator=g, device="cuda")
+    slopes = fixed.clone().requires_grad_()
+
+    def served(s):
+        kc, vc = (torch.zeros(2, 20, 2, 64, device="cuda", dtype=torch.float16) for _ in range(2))
+        y = cf.flare_causal_attention_prefill(q, k, k, kc, vc, slopes=s)
+        return y, cf.flare_causal_attention_decode(q[:, 0], k[:, 0], k[:, 0], kc, vc, torch.tensor([9, 3], device="cuda"), slopes=s)
+
+    for a, b in zip(served(slopes), served(fixed)):
+        assert torch.equal(a, b) and not a.requires_grad
+    with torch.no_grad():
+        assert torch.equal(cf.flare_causal_attention(q, k, k, slopes=slopes), cf.flare_causal_attention(q, k, k, slopes=fixed))
+    with pytest.raises(ValueError, match="no gradient of the slopes"):
+        cf.flare_causal_attention(q, k, k, slopes=slopes)
