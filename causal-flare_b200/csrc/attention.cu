@@ -170,14 +170,14 @@ struct DeltaParams {
   AttnParams p;
   const void *q, *k, *v, *dy;
   int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, dy_b, dy_n, dy_h;
-  float *delta, *dy_norm, *v_norm, *lse_lifted;  // (v_norm: [B][J][Nqp])
+  float *delta, *dy_norm, *v_norm;  // (v_norm: [B][J][Nqp])
 };
 // Keys up to which a row's delta is the sum of P dP itself.  <dy, y> has y's rounding and that of the weights in y, about 2^-9 |dy| |v| / sqrt(keys),
 // which dS = P (dP - delta) keeps: with two to five keys dQ and dK were 1.7 to 4 times as far off as their own rounding, with 50 and more 1.1.
 constexpr int kFewKeys = 32;
 
 // -delta, delta = sum P dP = <dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  For fp16 the norms too
-// from which the kernels behind it know how large dS can be.  Bound by memory: B=2 N=4096 H=16 D=128 29 us, in fp16 with the values' rows 45.
+// from which the kernels behind it know how large dS can be.  Bound by memory: B=2 N=4096 H=16 D=128 29 us, in fp16 with the values' rows 46.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ DeltaParams d) {
   pdl_begin();
@@ -255,16 +255,18 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Delt
     unpack8(own_value, v);
     const float dy_norm = joined(dot(dy, dy)), v_norm = joined(dot(v, v));
     if (live && lane == 0) {  // (comparisons with what is no number are false)
-      d.lse_lifted[at] = p.lse[at] + (float)kWeightLift;
       d.dy_norm[at] = keys > 0 && dy_norm < INFINITY ? dy_norm : 0.0f;
       if (h == kv * (p.H / p.J)) d.v_norm[((int64_t)b * p.J + kv) * p.masks.Nqp + i] = keys > 0 && v_norm < INFINITY ? v_norm : 0.0f;
     }
   }
 }
 
-// The largest norms of a key head's tokens: |dy|^2 of its query heads, |v|^2.  One block for each: 6.5 us for two times 4 096 of them.
-__global__ void __launch_bounds__(1024) largest_norms_kernel(const float* dy_norm, const float* v_norm, float* out, int group, int Nqp) {
-  pdl_begin();
+// The largest norms of a key head's tokens: |dy|^2 of its query heads, |v|^2; on the way the queries' lse for lifted weights (rows of [.., Nqp], as the
+// norms are).  One block for a key head: two times 4 096 norms are 7 us at most (the wait for the kernel in front is part of it).
+__global__ void __launch_bounds__(1024) largest_norms_kernel(const float* dy_norm, const float* v_norm, const float* lse, float* lse_lifted, float* out, int group,
+                                                             int Nqp) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t head = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;  // key head of the batch
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __shared__ float tops[2][32];
@@ -278,7 +280,13 @@ __global__ void __launch_bounds__(1024) largest_norms_kernel(const float* dy_nor
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     return top;
   };
-  const float dy = largest(dy_norm + head * group * Nqp, (int64_t)group * Nqp), v = largest(v_norm + head * Nqp, Nqp);
+  const int64_t first = head * group * Nqp, queries = (int64_t)group * Nqp;
+  for (int64_t i = threadIdx.x; i < queries / 4; i += 1024) {
+    constexpr float up = (float)kWeightLift;
+    const float4 v = reinterpret_cast<const float4*>(lse + first)[i];
+    reinterpret_cast<float4*>(lse_lifted + first)[i] = make_float4(v.x + up, v.y + up, v.z + up, v.w + up);
+  }
+  const float dy = largest(dy_norm + first, queries), v = largest(v_norm + head * Nqp, Nqp);
   if (lane == 0) {
     tops[0][warp] = dy;
     tops[1][warp] = v;
@@ -814,7 +822,6 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
     d.delta = floats(l.delta);
     d.dy_norm = floats(l.dy_norm);
     d.v_norm = floats(l.v_norm);
-    d.lse_lifted = floats(l.lse_lifted);
     auto* const kernel = a.dtype == FLARE_F16 ? (lanes == 8 ? delta_kernel<__half, 8> : delta_kernel<__half, 16>)
                                               : (lanes == 8 ? delta_kernel<__nv_bfloat16, 8> : delta_kernel<__nv_bfloat16, 16>);
     FLARE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(256), 0, stream, d));
@@ -822,7 +829,7 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   if (a.dtype == FLARE_F16) {
     LaunchTimer timer("attention_largest_norms_kernel", stream);
     FLARE_CUDA_CHECK(launch_pdl(largest_norms_kernel, dim3((unsigned)a.J, (unsigned)a.B), dim3(1024), 0, stream, p.dy_norm, (const float*)floats(l.v_norm),
-                                floats(l.largest_norms), a.H / a.J, l.Nqp));
+                                (const float*)a.lse, floats(l.lse_lifted), floats(l.largest_norms), a.H / a.J, l.Nqp));
   }
   return launch_backward_tc(a, p, stream);
 }
