@@ -175,6 +175,7 @@ struct DeltaParams {
 // Keys up to which a row's delta is the sum of P dP itself.  <dy, y> has y's rounding and that of the weights in y, about 2^-9 |dy| |v| / sqrt(keys),
 // which dS = P (dP - delta) keeps: with two to five keys dQ and dK were 1.7 to 4 times as far off as their own rounding, with 50 and more 1.1.
 constexpr int kFewKeys = 32;
+constexpr int kRows = 32768;  // rows of the batch along a grid's second dimension
 
 // -delta, delta = sum P dP = <dy, y>, LANES threads per row and head; 0 for queries without keys (their dy may hold anything).  For fp16 the norms too
 // from which the kernels behind it know how large dS can be.  Bound by memory: B=2 N=4096 H=16 D=128 29 us, in fp16 with the values' rows 46.
@@ -182,7 +183,8 @@ template <typename T, int LANES>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ DeltaParams d) {
   pdl_begin();
   const AttnParams& p = d.p;
-  const int lane = threadIdx.x % LANES, b = blockIdx.y;
+  const int lane = threadIdx.x % LANES, b = blockIdx.z * kRows + blockIdx.y;  // (a grid's second dimension ends at 65 535)
+  if (b >= p.B) return;
   const unsigned idx = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int i = (int)(idx / (unsigned)p.H), h = (int)(idx % (unsigned)p.H);
   const bool live = i < p.masks.Nqp, mine = live && i < p.Nq && lane * 8 < p.D;
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(1024) largest_norms_kernel(const float* dy_nor
                                                              int Nqp) {
   pdl_wait();
   pdl_trigger();
-  const int64_t head = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;  // key head of the batch
+  const int64_t head = blockIdx.x;  // key head of the batch
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __shared__ float tops[2][32];
   const auto largest = [&](const float* from, int64_t n) {  // (n: a multiple of 128)
@@ -808,10 +810,10 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   p.lse_lifted = floats(l.lse_lifted);
   const int lanes = a.D <= 64 ? 8 : 16;
   const int64_t blocks = ((int64_t)l.Nqp * a.H * lanes + 255) / 256;
-  if (blocks * (256 / lanes) > UINT_MAX - 256 || a.B > 65535) return FLARE_ERR_UNSUPPORTED;
+  if (blocks * (256 / lanes) > UINT_MAX - 256 || (int64_t)a.B * a.J > INT_MAX) return FLARE_ERR_UNSUPPORTED;
   {
     LaunchTimer timer("attention_delta_kernel", stream);
-    const dim3 grid((unsigned)blocks, (unsigned)a.B);
+    const dim3 grid((unsigned)blocks, (unsigned)(a.B < kRows ? a.B : kRows), (unsigned)((a.B + (int64_t)kRows - 1) / kRows));
     DeltaParams d;
     d.p = p;
     d.q = a.q; d.k = a.k; d.v = a.v; d.dy = a.dy;
@@ -828,7 +830,7 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
   }
   if (a.dtype == FLARE_F16) {
     LaunchTimer timer("attention_largest_norms_kernel", stream);
-    FLARE_CUDA_CHECK(launch_pdl(largest_norms_kernel, dim3((unsigned)a.J, (unsigned)a.B), dim3(1024), 0, stream, p.dy_norm, (const float*)floats(l.v_norm),
+    FLARE_CUDA_CHECK(launch_pdl(largest_norms_kernel, dim3((unsigned)(a.J * a.B)), dim3(1024), 0, stream, p.dy_norm, (const float*)floats(l.v_norm),
                                 (const float*)a.lse, floats(l.lse_lifted), floats(l.largest_norms), a.H / a.J, l.Nqp));
   }
   return launch_backward_tc(a, p, stream);

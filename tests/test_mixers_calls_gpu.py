@@ -1,4 +1,5 @@
-"""gpu: calls of the mixers that their documentation allows: states at odd addresses, slopes that are parameters."""
+"""gpu: calls of the mixers that their documentation allows: states at odd addresses, slopes that are parameters, batches
+of many rows."""
 import pytest
 import torch
 
@@ -68,3 +69,20 @@ def test_slopes_that_are_parameters(native, monkeypatch):
         assert torch.equal(cf.flare_causal_attention(q, k, k, slopes=slopes), cf.flare_causal_attention(q, k, k, slopes=fixed))
     with pytest.raises(ValueError, match="no gradient of the slopes"):
         cf.flare_causal_attention(q, k, k, slopes=slopes)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_more_rows_than_a_grids_second_dimension_holds(dtype):
+    # what the forward takes the backward takes too; every row is its own, so the last ones are those of a small batch
+    B, N, H, J, D = 65_539, 3, 2, 1, 8
+    g = gen(34)
+    q, k, v, dy = (randn(g, B, N, h, D, dtype=dtype) for h in (H, J, J, H))
+
+    def run(rows):
+        leaves = [t[rows].detach().requires_grad_() for t in (q, k, v)]
+        y = cf.flare_causal_attention(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy[rows])]
+
+    for rows in (slice(0, 5), slice(65_530, B)):
+        for a, b in zip(run(slice(0, B)), run(rows)):
+            assert torch.equal(a[rows], b)
