@@ -11,6 +11,9 @@ The score of the query at position i for the key at position j is ``cap * tanh(s
   padding: it sees nothing and nobody sees it, output and gradients are 0.
 * ``window``: only the keys j > i - window.
 * ``prefix`` [B, N] truth values: the tokens with which a document begins and for which it holds are seen by all of the document.
+
+A token that sees nothing, or none of whose scores is above -infinity, has output and gradients 0.  ``scale`` is D ** -0.5 unless it is given, but 1 for
+heads that are 8 wide: the convention of all operators of this package (pass ``scale=8 ** -0.5`` for the usual one).
 """
 
 from __future__ import annotations
@@ -124,8 +127,8 @@ class CausalAttention(autograd.Function):
 def flare_causal_attention(q, k, v, *, scale=None, cap=None, slopes=None, window=None, documents=None, prefix=None):
     """Causal attention (differentiable in q, k, v).  q [B, N, H, D]; k, v [B, N, J, D], bf16 or fp16, D a multiple of 8 up to 128.
 
-    ``scale`` defaults to D ** -0.5 (1 for D = 8, as in the FLARE operators); ``cap``, ``slopes`` [H] fp32 (which get no
-    gradient: while gradients are recorded they have to be detached), ``window``, ``documents`` and ``prefix`` as the module says.  Returns y [B, N, H, D].  Softmax statistics and sums are in fp32; its weights meet V in the inputs' type.  The gradients are the same bits
+    ``scale`` (D ** -0.5, for D = 8 it is 1), ``cap``, ``slopes`` [H] fp32 (which get no gradient: while gradients are recorded they have to be
+    detached), ``window``, ``documents`` and ``prefix`` as the module says.  Returns y [B, N, H, D].  Softmax statistics and sums are in fp32; its weights meet V in the inputs' type.  The gradients are the same bits
     in every call."""
     if q.is_cuda:
         y = _mixers.host().attention(q, k, v, scale, cap, slopes, window, documents, prefix)
@@ -173,7 +176,8 @@ def flare_causal_attention_prefill(q, k, v, k_cache, v_cache, *, cached=None, le
     The new keys and values are written into the caches, at positions cached[b] and on, and the queries see them and everything in
     front.  ``lengths`` [B]: tokens of row b (None: N); what lies behind is padding: nothing is written for it and y is 0.  A token
     whose position lies outside the cache is treated the same way (a row whose ``cached`` does: all of it).  ``prefix`` marks tokens of
-    the prompt's beginning that all new tokens see.  Returns y [B, N, H, D]; not differentiable."""
+    the prompt's beginning that all new tokens see.  ``scale`` (D ** -0.5, for D = 8 it is 1) and the rest as the module says.  Returns y [B, N, H, D]; not
+    differentiable."""
     if q.is_cuda:
         y = _mixers.host().attention_prefill(q, k, v, k_cache, v_cache, cached, lengths, scale, cap, slopes, window, prefix)
         if y is not None:
@@ -208,7 +212,7 @@ def flare_causal_attention_decode(q, k, v, k_cache, v_cache, cached, *, scale=No
 
     Its key and value are written to position cached[b] of the caches [B, L, J, D] and it sees them and the cached[b] in front; the
     caller counts ``cached`` up.  A row whose position lies outside the cache is idle: y is 0 and nothing is written (-1 for an empty
-    slot of a batch).  Returns y in q's shape; not differentiable."""
+    slot of a batch).  ``scale`` (D ** -0.5, for D = 8 it is 1) and the rest as the module says.  Returns y in q's shape; not differentiable."""
     if q.is_cuda:
         y = _mixers.host().attention_decode(q, k, v, k_cache, v_cache, cached, scale, cap, slopes, window)
         if y is not None:

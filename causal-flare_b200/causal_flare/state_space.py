@@ -330,7 +330,7 @@ def flare_selective_scan_decode(x, dt, A, B, C, state=None, *, D=None, z=None, d
     """One token: x, dt, z [B, C] or [B, 1, C]; B, C [B, S], [B, G, S] or [B, 1, G, S] with the same extra dimension as x.
 
     Returns ``(y in x's shape, state)``.  The state is updated IN PLACE when it is contiguous (the returned one is then the
-    same tensor); not differentiable."""
+    same tensor; one whose address is no multiple of 16 bytes costs two copies); not differentiable."""
     if x.is_cuda:
         out = _mixers.host().scan_decode(x, dt, A, B, C, state, D, z, dt_bias, bool(dt_softplus))
         if out is not None:

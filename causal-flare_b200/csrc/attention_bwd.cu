@@ -1,6 +1,7 @@
 // Attention backward on tcgen05, deterministic: one kernel for dK and dV, one for dQ, the same code on either side.
 //
-//   P = exp2(scores - lse),  dS = P (dP - delta), dP = dY V^T, delta = <dY, y>; behind the cap dS *= 1 - tanh^2 = 4 r (1 - r)
+//   P = exp2(scores - lse),  dS = P (dP - delta), dP = dY V^T, delta = <dY, y>; behind the cap dS *= 1 - tanh^2
+//   (of a saturated score that is off by up to 2^-23, as tanh itself is)
 //   dV = P^T dY,  dK = scale dS^T Q,  dQ = scale dS K
 //
 // A CTA keeps 128 rows of its own side (KEYS: K and V; else Q and dY) and walks tiles of 64 rows of the other: S = X0 Y0^T and

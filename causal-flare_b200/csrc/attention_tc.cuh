@@ -11,9 +11,9 @@ using namespace tc;
 
 // Scores, in units of log 2 once they are multiplied by `unit`.  CAP: cap tanh(x), x = scale <q, k> / cap.  The special-function
 // unit would give tanh as 1 - 2 / (exp(2 x) + 1), two results of it per score where the softmax itself takes one (tanh.approx is off by 2^-11 of
-// cap, hundredths of a nat); for |x| <= 0.35, where caps leave nearly all scores, an odd polynomial does it on the FMA pipe: the
-// least largest error of x p(x^2) with four coefficients there is 5.9e-9 (a weighted least-squares fit, repeated until its
-// error is level), with fp32 arithmetic 3.9e-8.  A warp that meets a larger |x| takes the exponential form.
+// cap, hundredths of a nat); for |x| <= 0.35, where caps leave nearly all scores, an odd polynomial does it on the FMA pipe: a
+// weighted least-squares fit of x p(x^2) with four coefficients, repeated until its error was level (5.9e-9).  With the first one in fp32 it is off by 1.5e-8 at
+// most (1.8e-7 of small x), in fp32 arithmetic by 4.8e-8.  A warp that meets a larger |x| takes the exponential form.
 struct ScoreScale {
   float unit;   // scale log2 e, or cap log2 e
   float in;     // scale / cap

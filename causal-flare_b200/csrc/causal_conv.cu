@@ -144,7 +144,7 @@ __device__ __forceinline__ Pairs<V> taps(const Pairs<V> (&w)[W], const Pairs<V>&
   return v;
 }
 
-// (WIDE: every thread has eight channels and 16-byte pieces)
+// (WIDE: every thread has all of its channels, in one aligned piece: 16 bytes, or 8 for 16-bit types)
 template <typename T, int W, bool DOCS, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps, kForwardBlocks) conv_forward_kernel(const ConvParams p) {
   constexpr int V = kForwardChannels;

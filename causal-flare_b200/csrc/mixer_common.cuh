@@ -128,8 +128,6 @@ __device__ __forceinline__ void store_all(T* p, const float (&x)[V], int count, 
       if (i < count) p[i] = from_float<T>(x[i]);
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8], int count, bool wide) { store_all<T, 8>(p, x, count, wide); }
 
 // 1 / (1 + exp(-x)): both functions within a few units in the last place, exp(-x) = inf gives 0
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }

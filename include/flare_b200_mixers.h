@@ -110,7 +110,7 @@ int flare_scan_decode(const flare_scan_args_t* args, flare_stream_t stream);
  *   cap tanh(scale <q, k> / cap) - slopes[h] |i - j|          (cap = 0: scale <q, k>, at most 1024; slopes NULL: no bias)
  * and token i sees the keys j <= i of its document, with `window` > 0 only j > i - window; where `prefix` [B, N] (bytes,
  * non-zero: true) holds for the first tokens of a document, all tokens of the document see those.  Without a key in
- * sight y and all gradients are 0.
+ * sight, or without a score above -infinity, y and all gradients are 0.
  *
  * Whole sequences (cached = NULL): Nk = Nq.  Prompts behind a cache (`cached` [B] int32: tokens that it holds): k and v are the
  * caches [B, Nk, J, D] with the new tokens in place (flare_attention_append), the Nq queries of row b lie at positions
@@ -154,6 +154,7 @@ int flare_attention_backward(const flare_attention_args_t* args, flare_stream_t 
  * append: new_k[b, t] goes to position cached[b] + t for t < lengths[b] (NULL: N); positions outside [0, L) are left out.
  * decode: one token per row, q, y [B, H, D], new_k, new_v [B, J, D].  The row's keys are the first cached[b] of its cache and the
  * new one, which is written to position cached[b].  A row whose position lies outside [0, L) is idle: y = 0, nothing is written.
+ * At most 65 535 rows in either.
  */
 typedef struct flare_cache_args {
   const void* q;
