@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import causal_flare as cf
+from causal_flare import _mixers, attention
 from oracle import mixers_oracle as orc
 
 pytestmark = pytest.mark.gpu
@@ -98,6 +99,39 @@ def test_a_row_whose_gradient_is_not_finite_leaves_the_others_alone():
         assert torch.equal(got[0][0, :100], clean[0][0, :100]) and torch.equal(got[1][0, :100], clean[1][0, :100])
         for a, c in zip(got, clean):
             assert torch.equal(a[1], c[1]) and torch.equal(a[0, :, 0], c[0, :, 0])  # another row of the batch, another head
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 6e4])
+def test_padding_does_not_count_in_fp16(value):
+    # neither for the norms by which dS is scaled, nor for anything else
+    B, N, H, J, D = 2, 300, 4, 2, 64
+    g = gen(7)
+    q, k, v, dy = (randn(g, B, N, h, D, dtype=torch.float16) for h in (H, J, J, H))
+    docs = (torch.rand(B, N, generator=g, device="cuda") < 0.015).int().cumsum(1).int()
+    docs = torch.where(docs % 3 == 0, -1, docs)
+    pad = (docs < 0)[..., None, None]
+    assert pad.any()
+    clean = gradients(q, k, v, dy, documents=docs)
+    for a, c in zip(gradients(*(t.masked_fill(pad, value) for t in (q, k, v, dy)), documents=docs), clean):
+        assert torch.equal(a, c)
+
+
+def test_a_backward_without_the_forwards_plan_in_fp16():
+    B, N, H, J, D = 2, 300, 4, 2, 64
+    g = gen(8)
+    q, k, v, dy = (randn(g, B, N, h, D, dtype=torch.float16) for h in (H, J, J, H))
+    want = gradients(q, k, v, dy, window=100)
+    a = attention._fill(q, k, v, (D ** -0.5, 0.0, 100), None)
+    out, lse = torch.empty_like(q), torch.empty(B, H, 384, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    a.y, a.lse = out.data_ptr(), lse.data_ptr()
+    _mixers.run("flare_attention_forward", a, q.device, "flare_attention_forward_workspace_bytes")
+    a.dy = dy.data_ptr()
+    _mixers.put_strides(a, "dy", dy, "bnh")
+    a.dq, a.dk, a.dv = (t.data_ptr() for t in grads)
+    _mixers.run("flare_attention_backward", a, q.device, "flare_attention_backward_workspace_bytes")
+    for x, z in zip(grads, want):
+        assert torch.equal(x, z)
 
 
 def test_gradients_of_nothing_are_nothing():
