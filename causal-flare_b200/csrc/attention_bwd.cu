@@ -15,11 +15,11 @@
 // fp16 holds 40 powers of two, and dS of ordinary gradients (1e-6) and of scaled ones (1e5) lie at its ends or behind them: dS is laid down times a
 // power of two, taken out again with the last product's factor.  |dS| <= 2 |dY| |V| of the longest rows, so 2^e |dS| <= 2^14 (and a factor of four
 // in hand for P above 1, which is as far off as large scores are): one e for a query, and for a key head's dK one for the row of the batch.  The sizes above:
-// 595 us in fp16, of which the norms that e is taken from are 20.
+// 590 us in fp16, of which the norms that e is taken from are 20.
 //
 // Tensor memory: two slots of S 64, dP 64; sums of dS and P products at 256 and 384 (the queries' kernel: its own tiles at 384).  P is rounded once, to the type of the
-// operands it meets (in fp16 times 2^14: weights of 1e-5, of rows of 1e5 keys, lost two bits); dS goes to its product as a rounded value and what that lost, rounded again: rounded once it made dK and dQ 1.6 times as far
-// off as their own rounding does.  Everything in front of that, and the sums, is fp32.
+// operands it meets (in fp16 times 2^14: weights of 1e-5, of rows of 1e5 keys, lost two bits); dS goes to its product as a rounded value and what that
+// lost, rounded again: rounded once it made dK and dQ 1.6 times as far off as their own rounding does.  Everything in front of that, and the sums, is fp32.
 #include "attention_tc.cuh"
 
 namespace flare {
